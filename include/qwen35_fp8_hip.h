@@ -23,6 +23,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "qh_paged_types.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -396,6 +398,63 @@ int qh_gdn_chunk(const void* qn, const void* kn, const void* y, const float* g, 
 
 /* m = bf16(bf16(silu(g)) * u), the M > 1 MLP glue (replaces main.py:1213-1215). */
 int qh_silu_mul(const void* g, const void* u, void* m, size_t n, qh_stream_t stream);
+
+/* ---- paged KV cache ------------------------------------------------------
+ * No counterparts in the reference, which serves one sequence from a dense bf16
+ * cache (main.py:1034-1059).  `pages` [n_seqs][max_pages] (int32) names the pages
+ * of each sequence in order: position j lies on page pages[b][j / page_size], slot
+ * j % page_size.  Pages may be shared by sequences.  What the device-resident
+ * indexes name outside their ranges is never touched:
+ *   - prep leaves out a token whose seq is outside [0, n_seqs), whose at is outside
+ *     [0, max_pages * page_size), whose page id is outside [0, n_pages) or one of
+ *     whose rotary positions is outside [0, max_pos): none of its rows is written,
+ *     in the cache or in q_out (rows of padding: seq or at = -1);
+ *   - read and attention take last[b] < 0 as an empty sequence and end at the
+ *     table's last position; positions on a page id outside [0, n_pages) are left
+ *     out. */
+
+/* T tokens of several sequences on their way into the cache.  Per token and head:
+ * (1+w) RMSNorm of q and k (norm weights null: none), rotary positions on the axes
+ * of `rope` (null or rot 0: none; pos [n_axes][T] int32), all in fp32; q to q_out
+ * [T][n_heads][D] (bf16, or fp32 with q_f32), K and V to slot at[t] of sequence
+ * seq[t] (seq null: sequence t, T <= n_seqs).  An E4M3 row has the scale
+ * max(amax / 448, 2^-100), amax over its finite values; a value that is not finite
+ * is stored as NaN.  q null: only K and V.  Token t's head h starts at
+ * q + t * q_tstride + h * q_hstride, k + t * k_tstride + h * D, v likewise
+ * (elements; multiples of 8; 16-byte aligned pointers).  q_out must not overlap an
+ * input.  Two tokens of one call must not name the same slot. */
+int qh_attn_prep_paged(const qh_paged_cache* cache, const qh_rope_axes* rope, const void* q,
+                       long long q_tstride, long long q_hstride, const void* k, long long k_tstride,
+                       const void* v, long long v_tstride, const float* q_norm_w,
+                       const float* k_norm_w, float eps, const int* pos, const int* seq, const int* at,
+                       int T, const int* pages, int n_seqs, int max_pages, void* q_out, int q_f32,
+                       int n_heads, qh_stream_t stream);
+
+/* Positions 0 .. last[b] of each sequence as dense bf16 rows: k_out, v_out
+ * [n_seqs][n_kv][max_seq][D], the layout qh_attn_prefill reads (one sequence of it:
+ * its k_cache, v_cache and max_seq).  Rows behind last[b] keep what they hold. */
+int qh_kv_read_paged(const qh_paged_cache* cache, const int* pages, int n_seqs, int max_pages,
+                     const int* last, void* k_out, void* v_out, int max_seq, qh_stream_t stream);
+
+/* Workspace bytes of qh_attn_decode_paged, for any number of sequences and any
+ * length (0 for head counts it does not take). */
+size_t qh_attn_decode_paged_workspace_size(int n_heads, int n_kv, int head_dim);
+
+/* Attention of one new token of each sequence: softmax(q . K^T / sqrt(D)) V over
+ * positions 0 .. last[b] (whose rows, the new token's among them, are in the
+ * cache), times sigmoid(gate) with a gate; out [n_seqs][n_heads][D] bf16, zeros for
+ * a sequence with no visible position.  q (bf16, normalised and rotated) has
+ * sequence b's head h at q + b * q_bstride + h * q_hstride, the gate likewise
+ * (elements; multiples of 8; 16-byte aligned pointers).  n_heads / n_kv <= 16, at
+ * most 4096 sequences and 65536 (sequence, KV head) pairs.  ws:
+ * qh_attn_decode_paged_workspace_size bytes, 256-byte aligned, zeroed once when it
+ * is allocated (the kernel returns its counters to zero); calls that share a
+ * workspace must not overlap. */
+int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, long long q_bstride,
+                         long long q_hstride, const void* gate, long long g_bstride,
+                         long long g_hstride, const int* pages, int n_seqs, int max_pages,
+                         const int* last, int n_heads, void* out, void* ws, size_t ws_bytes,
+                         qh_stream_t stream);
 
 #ifdef __cplusplus
 }

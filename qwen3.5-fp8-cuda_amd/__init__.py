@@ -10,9 +10,10 @@ Modules:
   ops     reference-named wrappers: fp8_linear, maybe_fp8_linear, fused_qkv, ...
   config  model shape (config.json keys)
   synth   seeded synthetic weights, reference block quantizer
+  paged   paged KV cache for several sequences: write, read back, decode attention
   engine  decode engine: per-token launch sequence and HIP-graph replay
   build   hipcc build of the shared library
 """
-from . import abi, config, ops, synth  # noqa: F401
+from . import abi, config, ops, paged, synth  # noqa: F401
 
-__all__ = ["abi", "config", "ops", "synth", "engine"]
+__all__ = ["abi", "config", "ops", "paged", "synth", "engine"]

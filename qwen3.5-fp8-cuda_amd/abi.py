@@ -23,6 +23,20 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _u64 = ctypes.c_uint64
+_ll = ctypes.c_longlong
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """qh_paged_cache (include/qh_paged_types.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_pages", _i),
+                ("page_size", _i), ("n_kv", _i), ("head_dim", _i), ("fp8", _i)]
+
+
+class RopeAxesDesc(ctypes.Structure):
+    """qh_rope_axes (include/qh_paged_types.h)."""
+    _fields_ = [("cos_t", _vp), ("sin_t", _vp), ("max_pos", _i), ("rot", _i), ("n_axes", _i),
+                ("interleaved", _i), ("section", _i * 4)]
+
 
 # Reference ABI (fused_kernels.cu:940-1356, fp8_kernels.cu:68-91); argtypes as
 # declared by main.py:108-240.
@@ -97,6 +111,11 @@ NATIVE_SIGNATURES = {
     "qh_gdn_chunk_workspace_size": (_sz, [_i, _i]),
     "qh_gdn_chunk": (_i, [_vp] * 9 + [_i] * 5 + [_f, _vp, _sz, _vp]),
     "qh_silu_mul": (_i, [_vp, _vp, _vp, _sz, _vp]),
+    "qh_attn_prep_paged": (_i, [_vp, _vp, _vp, _ll, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _f, _vp, _vp, _vp, _i,
+                                _vp, _i, _i, _vp, _i, _i, _vp]),
+    "qh_kv_read_paged": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
+    "qh_attn_decode_paged_workspace_size": (_sz, [_i, _i, _i]),
+    "qh_attn_decode_paged": (_i, [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _vp, _i, _vp, _vp, _sz, _vp]),
 }
 
 

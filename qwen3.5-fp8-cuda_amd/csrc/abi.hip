@@ -18,6 +18,7 @@
 #include "qh_attn.h"
 #include "qh_gdn.h"
 #include "qh_gemm.h"
+#include "qh_paged.h"
 #include "qh_prefill.h"
 #include "qh_sample.h"
 #include "qh_kernels.h"
@@ -940,4 +941,112 @@ QH_EXPORT int qh_silu_mul(const void* g, const void* u, void* m, size_t n, hipSt
   if (qh_launch_silu_mul((const uint16_t*)g, (const uint16_t*)u, (uint16_t*)m, n, stream) != 0)
     return -1;
   return check_launch("qh_silu_mul");
+}
+
+// ---- paged KV cache (no counterpart in the reference, which serves one sequence
+// from a dense cache, main.py:1034-1059) -------------------------------------------
+// Head norm, rotary positions on several axes and the (quantising) cache write of
+// T tokens of several sequences; q is handed on in bf16 or fp32.
+QH_EXPORT int qh_attn_prep_paged(const qh_paged_cache* cache, const qh_rope_axes* rope, const void* q,
+                                 long long q_tstride, long long q_hstride, const void* k, long long k_tstride,
+                                 const void* v, long long v_tstride, const float* q_norm_w, const float* k_norm_w,
+                                 float eps, const int* pos, const int* seq, const int* at, int T, const int* pages,
+                                 int n_seqs, int max_pages, void* q_out, int q_f32, int n_heads, hipStream_t stream) {
+  QhPagedPrepParams p;
+  memset(&p, 0, sizeof(p));
+  if (qh_paged_view(cache, pages, n_seqs, max_pages, "attn_prep_paged", &p.c) != 0) return -1;
+  p.q = (const uint16_t*)q;
+  p.q_ts = q_tstride;
+  p.q_hs = q_hstride;
+  p.k = (const uint16_t*)k;
+  p.k_ts = k_tstride;
+  p.v = (const uint16_t*)v;
+  p.v_ts = v_tstride;
+  p.q_norm_w = q_norm_w;
+  p.k_norm_w = k_norm_w;
+  p.eps = eps;
+  if (rope) p.rope = *rope;
+  if (p.rope.rot == 0) p.rope.n_axes = 0;
+  p.pos = pos;
+  p.seq = seq;
+  p.at = at;
+  p.T = T;
+  p.q_out = q_out;
+  p.q_f32 = q_f32;
+  p.n_heads = n_heads;
+  if (qh_launch_paged_prep(p, cache->head_dim, stream) != 0) return -1;
+  if (T == 0) return 0;
+  return check_launch("qh_attn_prep_paged");
+}
+
+// Positions 0 .. last[b] of each sequence as dense bf16 rows [n_seqs, n_kv, max_seq, D].
+QH_EXPORT int qh_kv_read_paged(const qh_paged_cache* cache, const int* pages, int n_seqs, int max_pages,
+                               const int* last, void* k_out, void* v_out, int max_seq, hipStream_t stream) {
+  QhPagedReadParams p;
+  memset(&p, 0, sizeof(p));
+  if (qh_paged_view(cache, pages, n_seqs, max_pages, "kv_read_paged", &p.c) != 0) return -1;
+  p.last = last;
+  p.k_out = (uint16_t*)k_out;
+  p.v_out = (uint16_t*)v_out;
+  p.max_seq = max_seq;
+  if (qh_launch_paged_read(p, cache->head_dim, stream) != 0) return -1;
+  if (n_seqs == 0) return 0;
+  return check_launch("qh_kv_read_paged");
+}
+
+QH_EXPORT size_t qh_attn_decode_paged_workspace_size(int n_heads, int n_kv, int head_dim) {
+  return qh_paged_attn_ws_bytes(n_heads, n_kv, head_dim);
+}
+
+// Attention of one new token of each sequence over positions 0 .. last[b].
+QH_EXPORT int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, long long q_bstride,
+                                   long long q_hstride, const void* gate, long long g_bstride, long long g_hstride,
+                                   const int* pages, int n_seqs, int max_pages, const int* last, int n_heads,
+                                   void* out, void* ws, size_t ws_bytes, hipStream_t stream) {
+  QhPagedAttnParams p;
+  memset(&p, 0, sizeof(p));
+  const char* what = "attn_decode_paged";
+  if (qh_paged_view(cache, pages, n_seqs, max_pages, what, &p.c) != 0) return -1;
+  if (n_heads < 1 || n_heads % p.c.n_kv != 0 || n_heads / p.c.n_kv > 16) {
+    qh_set_error("%s: n_heads=%d n_kv=%d unsupported (group size must divide and be <= 16)", what, n_heads, p.c.n_kv);
+    return -1;
+  }
+  if (n_seqs > kPagedMaxSeqs || (long long)n_seqs * p.c.n_kv > kPagedMaxUnits) {
+    qh_set_error("%s: n_seqs=%d n_kv=%d (at most %d sequences, %d pairs)", what, n_seqs, p.c.n_kv, kPagedMaxSeqs,
+                 kPagedMaxUnits);
+    return -1;
+  }
+  if (n_seqs == 0) return 0;
+  if (!q || !last || !out || !ws) {
+    qh_set_error("%s: null pointer", what);
+    return -1;
+  }
+  if (out == q || out == gate) {
+    qh_set_error("%s: out must not alias q or the gate", what);
+    return -1;
+  }
+  if (((uintptr_t)q | (uintptr_t)gate | (uintptr_t)out) % 16 != 0 || q_bstride % 8 || q_hstride % 8 || g_bstride % 8 ||
+      g_hstride % 8) {
+    qh_set_error("%s: pointers must be 16-byte aligned and strides multiples of 8", what);
+    return -1;
+  }
+  const size_t need = qh_paged_attn_ws_bytes(n_heads, p.c.n_kv, cache->head_dim);
+  if (ws_bytes < need || (uintptr_t)ws % 256 != 0) {
+    qh_set_error("%s: workspace of %zu bytes must be 256-byte aligned and at least "
+                 "qh_attn_decode_paged_workspace_size (%zu)", what, ws_bytes, need);
+    return -1;
+  }
+  p.q = (const uint16_t*)q;
+  p.q_bs = q_bstride;
+  p.q_hs = q_hstride;
+  p.gate = (const uint16_t*)gate;
+  p.g_bs = g_bstride;
+  p.g_hs = g_hstride;
+  p.last = last;
+  p.n_heads = n_heads;
+  p.out = (uint16_t*)out;
+  p.counters = (unsigned*)ws;
+  p.part = (float*)((unsigned*)ws + kPagedMaxUnits);
+  if (qh_launch_paged_attn(p, cache->head_dim, stream) != 0) return -1;
+  return check_launch("qh_attn_decode_paged");
 }
