@@ -1016,6 +1016,11 @@ QH_EXPORT int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, l
                  kPagedMaxUnits);
     return -1;
   }
+  if ((long long)n_seqs * p.c.n_kv * ((p.c.capacity + 31LL) / 32) > 0x7FFF0000LL) {
+    qh_set_error("%s: %d sequences of %d KV heads with tables of %d positions are more than 2^31 tiles of 32", what,
+                 n_seqs, p.c.n_kv, p.c.capacity);
+    return -1;
+  }
   if (n_seqs == 0) return 0;
   if (!q || !last || !out || !ws) {
     qh_set_error("%s: null pointer", what);

@@ -69,7 +69,7 @@ struct QhPagedAttnParams {
 
 // (sequence, kv head) pairs that one call of the decode attention takes, and its sequences.
 constexpr int kPagedMaxUnits = 65536;
-constexpr int kPagedMaxSeqs = 4096;
+constexpr int kPagedMaxSeqs = 2048;
 
 int qh_paged_view(const qh_paged_cache* c, const int* pages, int n_seqs, int max_pages, const char* what,
                   QhPagedView* out);

@@ -412,6 +412,25 @@ def test_attend_one_sequence(n, H, kv, D, page, fp8):
     check_attend(parts, on_gpu(parts), bf(randn(g, 1, H, D, std=2.0)), table, torch.tensor([n - 1], dtype=torch.int32))
 
 
+@pytest.mark.parametrize("B,H,kv,D", [(2048, 16, 1, 256), (513, 8, 8, 128), (700, 32, 32, 128)])
+def test_attend_many_sequences(B, H, kv, D):
+    """The most sequences that a call takes with the widest group, and counts that fit nothing: lengths of
+    0 to 70 with a few long ones in between."""
+    g = gen(B)
+    page = 8
+    lens = torch.randint(0, 70, (B,), generator=g).tolist()
+    lens[0], lens[B // 2], lens[B - 1] = 0, 900, 1500
+    table, n_pages = tables(g, lens, page)
+    parts = pool(g, n_pages, kv, page, D, True)
+    q, last = bf(randn(g, B, H, D)), torch.tensor(lens, dtype=torch.int32) - 1
+    out = on_gpu(parts).attend(q.to(DEV), table.to(DEV), last.to(DEV), paged.attn_workspace(H, kv, D)).cpu()
+    empty = last < 0
+    assert bool((out[empty] == 0).all()) and bool(torch.isfinite(out).all())
+    some = [0, 1, 2, B // 2 - 1, B // 2, B // 2 + 1, B - 2, B - 1] + torch.randint(0, B, (60,), generator=g).tolist()
+    want, tol = ref.attend(q[some], *parts, table[some], last[some])
+    assert bool(((out[some].double() - want).abs() <= HALF_BF16 * (want.abs() + tol) + tol).all())
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 def test_attend_strided_q_and_gate(fp8):
     """q and its gate interleaved per head, as the gated q projection leaves them."""

@@ -138,7 +138,7 @@ def test_read_refusals(bad):
     (dict(heads=18), "n_heads"),
     (dict(heads=0), "n_heads"),
     (dict(heads=68), "n_heads"),           # 17 query heads to a KV head
-    (dict(n_seqs=4097), "at most 4096"),
+    (dict(n_seqs=2049), "at most 2048"),
     (dict(q=None), "null pointer"),
     (dict(last=None), "null pointer"),
     (dict(out=None), "null pointer"),
@@ -157,8 +157,10 @@ def test_attention_refusals(bad, said):
 
 
 def test_attention_pairs_limit():
-    assert attend(cache(n_kv=32), n_seqs=4096, heads=32) == -1
+    assert attend(cache(n_kv=64), n_seqs=2048, heads=64) == -1
     assert "pairs" in abi.last_error()
+    assert attend(cache(n_kv=32), n_seqs=2048, heads=32, max_pages=1 << 17) == -1
+    assert "tiles" in abi.last_error()
 
 
 def test_workspace_size():
