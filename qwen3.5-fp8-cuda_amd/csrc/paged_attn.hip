@@ -26,26 +26,25 @@
 // needs no exchange between lanes and no rescaling.
 //
 // Work split: the tiles (32 positions of one KV head of one sequence) of the whole
-// batch form one line, cut into equal shares of consecutive tiles, one a workgroup (one
-// workgroup per CU), so ragged batches load all CUs alike; a share's tiles go round its
-// waves in turn wherever sequences end.  The rows of a wave's next tile are on their way
-// while it computes, across sequences too, and the page ids of the one after.  A
-// (sequence, KV head) inside one share is written out; one that several shares cut
-// leaves a partial record a piece (maximum, sum, outputs), and the last piece to arrive
-// joins them in their order: the result does not depend on who comes last.
-#include <type_traits>
-
+// batch form one line, cut into equal shares of consecutive tiles, one a wave, so ragged
+// batches load all CUs alike.  The rows of a wave's next tile are on their way while it
+// computes, across sequences too, and the page ids of the one after.  A (sequence, KV
+// head) inside one wave's share is written out from its registers.  One that waves of a
+// workgroup cut is joined once, at the share's end, through LDS; one that workgroups cut
+// leaves a partial record a piece (maximum, sum, outputs) in the workspace, and the last
+// piece to arrive joins them.  All joins go in the order of the pieces: the result does
+// not depend on who comes last.
 #include "qh_common.h"
 #include "qh_paged.h"
 
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 32;                    // positions per wave and step
-constexpr int kMaxWG = 256;                  // workgroups that hold a share
+constexpr int kTile = 32;    // positions per wave and step
+constexpr int kMaxWG = 256;  // workgroups that hold a share (one per CU)
 constexpr int kMaxG = 16;
-constexpr int kWhole = 3 * kWaves;           // tiles of a pair that one workgroup takes rather than join pieces
+// Waves of a workgroup: two to a SIMD; one where a tile of bf16 rows of 256 fills the
+// registers, or where the LDS has no room for the partial results of eight.
+constexpr int waves_of(int G, int D, bool fp8) { return D == 256 && (!fp8 || G > 8) ? 4 : 8; }
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
@@ -76,16 +75,14 @@ struct Tile {
   f32x4 ks[2], vs[2];                                // scales of positions 8 g .. 8 g + 7
 };
 
-// Rows of a record: [G][D] outputs, [16] maxima, [16] sums.
+// A partial result, in LDS or in the workspace: the G heads' outputs, 4 dims at a time as
+// lane (r < G, g) of a wave holds them ([D / 16][4 G] x 16 bytes), [16] maxima, [16] sums.
 __host__ __device__ constexpr int rec_floats(int G, int D) { return G * D + 2 * kMaxG; }
 
-// LDS bytes: the waves' outputs (and the joining of pieces, which comes after them),
-// the query rows, per sequence its positions and the running sum of tiles.
-constexpr int head_floats(int D) { return D + 4; }   // between heads: no bank conflict
-constexpr int q_stride(int D) { return D + 8; }      // between query rows (bf16)
-size_t lds_bytes(int G, int D, int B) {
-  const size_t outs = (size_t)kWaves * G * head_floats(D) * 4, join = (size_t)2 * kMaxWG * G * 4 + kThreads * 16;
-  return (outs > join ? outs : join) + (size_t)kMaxG * q_stride(D) * 2 + (size_t)B * 8;
+// LDS floats: two partial results a wave (later, the threads' sums), 8 bytes a sequence.
+__host__ __device__ constexpr int slot_floats(int G, int D, int waves) {
+  const int slots = 2 * waves * rec_floats(G, D), sums = waves * 64 * 6;
+  return slots > sums ? slots : sums;
 }
 
 // A tile on the line: its sequence and KV head, and the tiles [u0, u1) of that pair.
@@ -110,30 +107,30 @@ __device__ __forceinline__ int wave_isum(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnParams p) {
+template <int D, bool FP8, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhPagedAttnParams p) {
   using T = Tile<D, FP8>;
+  constexpr int kThreads = 64 * kWaves;
+  constexpr int kWhole = 2 * kWaves;                 // tiles of a pair that one workgroup takes rather than join pieces
   constexpr int DT = D / 16;                         // 16-dim tiles of the output
-  constexpr int HS = D + 4, QS = D + 8;
+  constexpr int KK = D / 32;                         // products of a score tile
+  constexpr int RUN = FP8 ? DT : 8;                  // consecutive dims of a lane
   __shared__ int s_tot[kWaves];
-  __shared__ float s_m[kWaves][kMaxG], s_l[kWaves][kMaxG];
-  __shared__ float s_sum[kMaxG];
+  __shared__ int s_end[kWaves];                      // where the pair that a wave did not begin ends (0: none)
   __shared__ int s_last[2];
-  extern __shared__ __align__(16) float s_o[];       // [kWaves][G][HS]
+  extern __shared__ __align__(16) float s_o[];
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int B = p.c.n_seqs, Hkv = p.c.n_kv, G = p.n_heads / Hkv, ps = p.c.page_size;
   const int wg = blockIdx.x;
-  const int out_floats = kWaves * G * HS, join_floats = 2 * kMaxWG * G + kThreads * 4;
-  uint16_t* s_q = (uint16_t*)(s_o + (out_floats > join_floats ? out_floats : join_floats));  // [kMaxG][QS]
-  int* s_n = (int*)(s_q + kMaxG * QS);               // [B] positions of sequence b
+  int* s_n = (int*)(s_o + slot_floats(G, D, kWaves));  // [B] positions of sequence b
   int* s_cum = s_n + B;                              // [B] tiles (of one KV head) of sequences 0 .. b
 
-  // ---- this workgroup's part of the work: tiles [start, end) from `seg` on ---------------
+  // ---- this workgroup's part of the work: tiles [start, end), each wave's `ws` of them ----
   Place seg;
   int start = 0, end = 0, share = 0, w0 = -1;        // w0 >= 0: pieces of one pair, the first of them here
-  int pieces = 0;
+  int pieces = 0, ws = 0;
   auto zeros = [&](int b) {                          // an empty sequence
     for (int i = tid; i < p.n_heads * D / 8; i += kThreads)
       *(u32x4*)(p.out + (size_t)b * p.n_heads * D + i * 8) = u32x4{0u, 0u, 0u, 0u};
@@ -150,7 +147,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
     else if (4 * B <= slots) share = max(kWaves, (sum + slots - B - 1) / (slots - B));
     by_pair = share > 0;
     if (by_pair) {
-      share = (share + kWaves - 1) / kWaves * kWaves;
       const int pc = (tl + share - 1) / share;
       int cum = pc;
 #pragma unroll
@@ -173,6 +169,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
       seg.u1 = (seg.n + kTile - 1) / kTile;
       start = seg.k = j * share;
       end = min(seg.u1, start + share);
+      ws = (end - start + kWaves - 1) / kWaves;
     }
   }
   if (!by_pair) {
@@ -207,7 +204,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
     const int total = __builtin_amdgcn_readfirstlane(all) * Hkv;
     __syncthreads();
     share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    share = max(kWaves, (share + kWaves - 1) / kWaves * kWaves);
+    ws = max(1, (share + kWaves - 1) / kWaves);
+    share = ws * kWaves;
     for (int b = wg; b < B; b += gridDim.x)
       if (s_n[b] == 0) zeros(b);
     start = wg * share;
@@ -241,6 +239,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
     }
     return c;
   };
+  const int k0 = start + wid * ws, k1 = min(end, k0 + ws);  // this wave's tiles
   const float qscale = (D == 256 ? 0.0625f : 0.08838834764831845f) * 1.4426950408889634f;  // log2(e) / sqrt(D)
 
   // Page ids and slots of the lane's two groups of 8 positions (K: r / 4, V: g) of a tile.
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
     return x;
   };
   auto row_of = [&](const Place& c, int id, int off) {
-    const bool ok = c.k < end;
+    const bool ok = c.k < k1;
     return ((long long)(ok && (unsigned)id < (unsigned)p.c.n_pages ? id : 0) * Hkv + c.kvh) * ps + (ok ? off : 0);
   };
   T t;
@@ -299,53 +298,50 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
       }
     }
   };
-  // The 16 bytes of a pair's query rows that this thread moves to LDS (rows above G: none).
-  auto q_of = [&](const Place& c) {
-    u32x4 x = {0u, 0u, 0u, 0u};
-    const int h = tid / (D / 8), d = tid % (D / 8) * 8;
-    if (h < G) x = *(const u32x4*)(p.q + c.b * p.q_bs + (long long)(c.kvh * G + h) * p.q_hs + d);
-    return x;
-  };
-  auto q_put = [&](u32x4 x) {
-    const int h = tid / (D / 8), d = tid % (D / 8) * 8;
-    if (h < kMaxG) *(u32x4*)(s_q + h * QS + d) = x;
+  // this lane's query dims: head r (those above G repeat head 0; nothing of theirs is used)
+  u32x4 q[KK];
+  auto load_q = [&](const Place& c) {
+    const uint16_t* src = p.q + c.b * p.q_bs + (long long)(c.kvh * G + (r < G ? r : 0)) * p.q_hs;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      q[kk] = *(const u32x4*)(src + (FP8 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
   };
 
   // ---- the first tile on its way, the ids of the second --------------------------------
   Place A = seg, C;           // the tile whose rows are in t; the next one of this wave
-  Ids ai = {}, ci = {};
-  A.k = start + wid;
-  if (A.k < end) A = walk(A, A.k);
+  Ids ai, ci;
+  A.k = k0;
+  if (k0 < k1) A = walk(A, k0);
   ai = ids_of(A);
+  load_q(A);
   C = A;
-  C.k = A.k + kWaves;
-  if (C.k < end) C = walk(C, C.k);
+  C.k = k0 + 1;
+  if (C.k < k1) C = walk(C, C.k);
   ci = ids_of(C);
+  // in the order of the loop below: its waits count the loads behind the one they are for
+  asm volatile("" ::: "memory");
   load_k(A, ai);
+  asm volatile("" ::: "memory");
   load_v(A, ai);
-  q_put(q_of(seg));
-  __syncthreads();
+  asm volatile("" ::: "memory");
 
   f32x4 o[DT];
   float m, l;
   auto step = [&]() {
     // ---- scores ----
     f32x4 s[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-    const uint16_t* qr = s_q + r * QS + (FP8 ? 16 : 8) * g;
 #pragma unroll
     for (int j = 0; j < T::KL; ++j) {
       if constexpr (FP8) {
-        const u32x4 q0 = *(const u32x4*)(qr + 64 * j), q1 = *(const u32x4*)(qr + 64 * j + 8);
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
           const u32x4 w = t.k[a][j];
-          s[a] = mfma(u32x4{widen_lo(w.x), widen_hi(w.x), widen_lo(w.y), widen_hi(w.y)}, q0, s[a]);
-          s[a] = mfma(u32x4{widen_lo(w.z), widen_hi(w.z), widen_lo(w.w), widen_hi(w.w)}, q1, s[a]);
+          s[a] = mfma(u32x4{widen_lo(w.x), widen_hi(w.x), widen_lo(w.y), widen_hi(w.y)}, q[2 * j], s[a]);
+          s[a] = mfma(u32x4{widen_lo(w.z), widen_hi(w.z), widen_lo(w.w), widen_hi(w.w)}, q[2 * j + 1], s[a]);
         }
       } else {
-        const u32x4 q0 = *(const u32x4*)(qr + 32 * j);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) s[a] = mfma(t.k[a][j], q0, s[a]);
+        for (int a = 0; a < 2; ++a) s[a] = mfma(t.k[a][j], q[j], s[a]);
       }
     }
     const bool there = (unsigned)ai.vid < (unsigned)p.c.n_pages;
@@ -362,8 +358,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
     load_k(C, ci);
     nx = C;
     ni = ci;
-    C.k += kWaves;
-    if (C.k < end) C = walk(C, C.k);
+    ++C.k;
+    if (C.k < k1) C = walk(C, C.k);
     ci = ids_of(C);
     // ---- weights ----
     float top = x[0];
@@ -438,100 +434,145 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
   };
 
   const int rec = rec_floats(G, D);
-  Pair open0 = {0, 0, 0, 0, 0}, open1 = {0, 0, 0, 0, 0};
-  auto gate_of = [&](const Pair& x, int h, int c) {
-    return p.gate ? *(const u32x2*)(p.gate + x.b * p.g_bs + (long long)(x.kvh * G + h) * p.g_hs + c) : u32x2{0u, 0u};
+  auto gate_of = [&](int b, int head, int c) {
+    return p.gate ? *(const u32x2*)(p.gate + b * p.g_bs + (long long)head * p.g_hs + c) : u32x2{0u, 0u};
   };
-  auto emit = [&](const Pair& x, int h, int c, f32x4 a, float L, u32x2 gt) {
+  auto emit = [&](int b, int head, int c, f32x4 a, float L, u32x2 gt) {
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     if (L == 0.0f) a = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = a[i] * inv;
     if (p.gate) {
-      y[0] *= qh_sigmoid(bf_lo(gt.x)); y[1] *= qh_sigmoid(bf_hi(gt.x));
-      y[2] *= qh_sigmoid(bf_lo(gt.y)); y[3] *= qh_sigmoid(bf_hi(gt.y));
+      y[0] *= qh_sigmoid_bf(bf_lo(gt.x)); y[1] *= qh_sigmoid_bf(bf_hi(gt.x));
+      y[2] *= qh_sigmoid_bf(bf_lo(gt.y)); y[3] *= qh_sigmoid_bf(bf_hi(gt.y));
     }
-    *(u32x2*)(p.out + ((size_t)x.b * p.n_heads + x.kvh * G + h) * D + c) =
-        u32x2{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+    *(u32x2*)(p.out + ((size_t)b * p.n_heads + head) * D + c) = u32x2{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
   };
-  while (true) {
-    const int s1 = min(seg.u1, end);
-    const bool more_seg = s1 < end;
-    Place next = seg;
-    u32x4 qn = {0u, 0u, 0u, 0u};
-    if (more_seg) {
-      next = walk(seg, s1);
-      qn = q_of(next);
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    m = -INFINITY;
-    l = 0.0f;
-    while (A.k < s1) step();
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-
-    // ---- the waves' parts, joined in LDS ----
-    if (g == 0) {
-      s_m[wid][r] = m;
-      s_l[wid][r] = l;
-    }
+  // Item i of a partial result: head and first of its 4 dims.
+  const int items = G * D / 4;
+  struct Item { int h, c; };
+  auto item = [&](int i) {
+    const int k = i / (4 * G), ln = i - k * 4 * G, gg = ln / G, rr = k / (DT / 4), d = k % (DT / 4) * 4;
+    return Item{ln - gg * G, RUN * (4 * gg + rr) + (FP8 ? d : 128 * (d / 8) + d % 8)};
+  };
+  auto slot_of = [&](int s) { return s_o + (size_t)s * rec; };  // 2 w: begun before wave w, 2 w + 1: by it
+  auto put_slot = [&](int s) {
     if (r < G) {
-      float* dst = s_o + ((size_t)wid * G + r) * HS;
-      constexpr int RUN = FP8 ? DT : 8;              // consecutive dims of a lane
+      f32x4* dst = (f32x4*)slot_of(s) + g * G + r;
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr)
-#pragma unroll
-        for (int d = 0; d < DT; d += 4)
-          *(f32x4*)(dst + RUN * (4 * g + rr) + (FP8 ? d : 128 * (d / 8) + d % 8)) =
-              f32x4{o[d][rr], o[d + 1][rr], o[d + 2][rr], o[d + 3][rr]};
-    }
-    __syncthreads();
-    Pair now;
-    now.b = seg.b;
-    now.kvh = seg.kvh;
-    now.pieces = w0 >= 0 ? pieces : (seg.u1 - 1) / share - seg.u0 / share + 1;
-    now.first = w0 >= 0 ? w0 : seg.u0 / share;
-    now.tail = w0 < 0 && seg.u0 != now.first * share ? 1 : 0;
-    float* mine_rec = p.part + (size_t)(2 * wg + (seg.k != start ? 1 : 0)) * rec;
-    const auto out_rsrc = __builtin_amdgcn_make_buffer_rsrc(mine_rec, (short)0, rec * 4, 0x00020000);
-    for (int i = tid; i < G * D / 4; i += kThreads) {
-      const int h = i / (D / 4), c = (i % (D / 4)) * 4;
-      float M = -INFINITY, L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][h]);
-      f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        // a wave that saw nothing (sum 0) counts for nothing; a NaN counts
-        const float f = s_l[w][h] == 0.0f ? 0.0f : exp2f(s_m[w][h] - M);
-        L += s_l[w][h] * f;
-        const f32x4 x = *(const f32x4*)(s_o + ((size_t)w * G + h) * HS + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = f != 0.0f ? fmaf(x[e], f, a[e]) : a[e];
+      for (int i = 0; i < DT; ++i) {
+        const int rr = i / (DT / 4), d = i % (DT / 4) * 4;
+        dst[i * 4 * G] = f32x4{o[d][rr], o[d + 1][rr], o[d + 2][rr], o[d + 3][rr]};
       }
-      if (now.pieces == 1) {
-        emit(now, h, c, a, L, gate_of(now, h, c));
-      } else {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), out_rsrc, (h * D + c) * 4, 0, 16);
-        if (c == 0) {
-          pub_store(mine_rec + G * D + h, M);
-          pub_store(mine_rec + G * D + kMaxG + h, L);
+      if (g == 0) {
+        slot_of(s)[G * D + r] = m;
+        slot_of(s)[G * D + kMaxG + r] = l;
+      }
+    }
+  };
+  // A part that saw nothing (sum 0) counts for nothing; a NaN counts.
+  auto add_part = [&](f32x4& a, float& M, float& L, f32x4 x, float mx, float lx) {
+    const float nm = fmaxf(M, mx);
+    const float fo = L == 0.0f ? 0.0f : exp2f(M - nm), fn = lx == 0.0f ? 0.0f : exp2f(mx - nm);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = fmaf(x[e], fn, a[e] * fo);
+    L = L * fo + lx * fn;
+    M = nm;
+  };
+
+  // ---- this wave's pairs, one after the other -------------------------------------------
+  Place at = A;
+  if (tid < kWaves) s_end[tid] = 0;
+  __syncthreads();
+  if (k0 < k1) {
+    while (true) {
+      const int s1 = min(at.u1, k1);
+      // q is waited for here: where it may be under way in any step, each score would wait
+      // for it, and so for all that was asked for after it
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk]));
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m = -INFINITY;
+      l = 0.0f;
+      while (A.k < s1) step();
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      const Place done = at;
+      const bool more = s1 < k1, begun = done.u0 < k0;
+      if (more) {
+        at = A;
+        load_q(at);
+      }
+      put_slot(2 * wid + (begun ? 0 : 1));
+      if (begun && lane == 0) s_end[wid] = done.u1;
+      if (!begun && done.u1 <= k1) {                 // all of it is here
+        const float* src = slot_of(2 * wid + 1);
+        for (int i = lane; i < items; i += 64) {
+          const Item it = item(i);
+          const int head = done.kvh * G + it.h;
+          emit(done.b, head, it.c, ((const f32x4*)src)[i], src[G * D + kMaxG + it.h], gate_of(done.b, head, it.c));
+        }
+      }
+      if (!more) break;
+    }
+  }
+  // ---- pairs that waves cut: every thread its items, pair by pair -------------------------
+  __syncthreads();
+  Pair open0 = {0, 0, 0, 0, 0}, open1 = {0, 0, 0, 0, 0};
+  auto pair_of = [&](const Place& c) {
+    Pair x;
+    x.b = c.b;
+    x.kvh = c.kvh;
+    x.pieces = w0 >= 0 ? pieces : (c.u1 - 1) / share - c.u0 / share + 1;
+    x.first = w0 >= 0 ? w0 : c.u0 / share;
+    x.tail = w0 < 0 && c.u0 != x.first * share ? 1 : 0;
+    return x;
+  };
+  {
+    Place c = seg;
+    for (int w = 0; w < kWaves; ++w) {
+      // the pair that goes on behind wave w (w = 0: also the one begun before this workgroup)
+#pragma unroll 1
+      for (int part = w == 0 ? 0 : 1; part < 2; ++part) {
+        const int kw = start + w * ws, kn = min(end, kw + ws);
+        if (kw >= end) break;
+        const int k = part == 0 ? kw : kn - 1;
+        if (k >= c.u1) c = walk(c, k);
+        const bool here = c.u0 >= start, all = here && c.u1 <= end;
+        if (part == 0 ? here : !(c.u0 >= kw && c.u1 > kn) && !(c.u0 >= kw && !all)) continue;
+        const int last = (min(c.u1, end) - 1 - start) / ws;
+        float* dst = p.part + (size_t)(2 * wg + (c.u0 > start ? 1 : 0)) * rec;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(dst, (short)0, rec * 4, 0x00020000);
+        for (int i = tid; i < items; i += kThreads) {
+          const Item it = item(i);
+          const int head = c.kvh * G + it.h;
+          const u32x2 gt = all ? gate_of(c.b, head, it.c) : u32x2{0u, 0u};
+          float M = -INFINITY, L = 0.0f;
+          f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int x = w; x <= last; ++x) {
+            const float* src = slot_of(2 * x + (x == w ? part : 0));
+            add_part(a, M, L, ((const f32x4*)src)[i], src[G * D + it.h], src[G * D + kMaxG + it.h]);
+          }
+          if (all) {
+            emit(c.b, head, it.c, a, L, gt);
+          } else {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), rs, i * 16, 0, 16);
+            if (i < 4 * G && i / G == 0) {
+              pub_store(dst + G * D + it.h, M);
+              pub_store(dst + G * D + kMaxG + it.h, L);
+            }
+          }
+        }
+        if (!all) {
+          if (c.u0 > start) open1 = pair_of(c);
+          else open0 = pair_of(c);
         }
       }
     }
-    // A share holds at most two pairs that others hold too, its first and its last: both
-    // arrivals wait for the share's end, when the first one's stores are long done.
-    if (now.pieces > 1) {
-      if (seg.k == start) open0 = now;
-      else open1 = now;
-    }
-    if (!more_seg) break;
-    q_put(qn);                                       // every wave is done with the rows of this pair
-    __syncthreads();                                 // the query rows are there, LDS is free
-    seg = next;
   }
+  // A share holds at most two pairs that other workgroups hold too, its first and its last.
   if (open0.pieces == 0 && open1.pieces == 0) return;
   wait_mem();
   __syncthreads();
@@ -550,59 +591,44 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(QhPagedAttnPara
   for (int which = 0; which < 2; ++which) {
     if (!s_last[which]) continue;
     const Pair x = which == 0 ? open0 : open1;
-    // the pieces' maxima and sums, then their weights, in LDS; then the weighted outputs
     auto rec_of = [&](int j) { return p.part + (size_t)(2 * (x.first + j) + (j == 0 ? x.tail : 0)) * rec; };
-    float *s_w = s_o, *s_s = s_o + kMaxWG * G;
-    f32x4* s_a = (f32x4*)(s_o + 2 * kMaxWG * G);     // [kThreads]
-    for (int i = tid; i < x.pieces * G; i += kThreads) {
-      const int j = i / G, h = i - j * G;
-      s_w[h * kMaxWG + j] = pub_load(rec_of(j) + G * D + h);
-      s_s[h * kMaxWG + j] = pub_load(rec_of(j) + G * D + kMaxG + h);
-    }
-    __syncthreads();
-    for (int h = wid; h < G; h += kWaves) {
-      float M = -INFINITY, L = 0.0f;
-      for (int j = lane; j < x.pieces; j += 64) M = fmaxf(M, s_w[h * kMaxWG + j]);
-      M = wave_max(M);
-      for (int j = lane; j < x.pieces; j += 64) {
-        const float lj = s_s[h * kMaxWG + j], f = lj == 0.0f ? 0.0f : exp2f(s_w[h * kMaxWG + j] - M);
-        s_w[h * kMaxWG + j] = f;
-        L += lj * f;
-      }
-      L = wave_sum(L);
-      if (lane == 0) s_sum[h] = L;
-    }
-    __syncthreads();
-    const int items = G * D / 4, subs = items < kThreads ? kThreads / items : 1;
+    // a thread takes an item, of every subs-th piece where there are threads enough for that
+    const int subs = items < kThreads ? min(kThreads / items, x.pieces) : 1;
+    f32x4* s_a = (f32x4*)s_o;                        // [kThreads]
+    float2* s_ml = (float2*)(s_a + kThreads);        // [kThreads]
     for (int i0 = 0; i0 < items; i0 += kThreads) {
       const int sub = items < kThreads ? tid / items : 0, i = i0 + tid - sub * items;
-      const int h = i / (D / 4), c = (i % (D / 4)) * 4;
+      const Item it = item(min(i, items - 1));
+      const int head = x.kvh * G + it.h;
+      float M = -INFINITY, L = 0.0f;
       f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
       u32x2 gt = {0u, 0u};
       if (i < items && sub < subs) {
-        gt = gate_of(x, h, c);
+        gt = gate_of(x.b, head, it.c);
         constexpr int U = 8;
         for (int j = sub; j < x.pieces; j += U * subs) {
           u32x4 y[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) y[u] = coherent_load(rec_of(min(j + u * subs, x.pieces - 1)) + h * D + c);
+          float my[U], ly[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int jj = j + u * subs;
-            const float f = jj < x.pieces ? s_w[h * kMaxWG + jj] : 0.0f;
-            const f32x4 z = __builtin_bit_cast(f32x4, y[u]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = f != 0.0f ? fmaf(z[e], f, a[e]) : a[e];
+            const float* src = rec_of(min(j + u * subs, x.pieces - 1));
+            y[u] = coherent_load(src + 4 * i);
+            my[u] = pub_load(src + G * D + it.h);
+            ly[u] = pub_load(src + G * D + kMaxG + it.h);
           }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (j + u * subs < x.pieces) add_part(a, M, L, __builtin_bit_cast(f32x4, y[u]), my[u], ly[u]);
         }
       }
       if (subs > 1) {
         s_a[tid] = a;
+        s_ml[tid] = float2{M, L};
         __syncthreads();
         if (sub == 0)
-          for (int k = 1; k < subs; ++k) a += s_a[k * items + i];
+          for (int k = 1; k < subs; ++k) add_part(a, M, L, s_a[k * items + i], s_ml[k * items + i].x, s_ml[k * items + i].y);
       }
-      if (i < items && sub == 0) emit(x, h, c, a, s_sum[h], gt);
+      if (i < items && sub == 0) emit(x.b, head, it.c, a, L, gt);
     }
     if (tid == 0) reset_counter(p.counters + x.b * Hkv + x.kvh);
     __syncthreads();
@@ -616,14 +642,18 @@ size_t qh_paged_attn_ws_bytes(int n_heads, int n_kv, int D) {
   return kPagedMaxUnits * sizeof(unsigned) + (size_t)2 * kMaxWG * rec_floats(n_heads / n_kv, D) * sizeof(float);
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, int kWaves>
 static int launch(const QhPagedAttnParams& p, hipStream_t st) {
-  const size_t lds = lds_bytes(p.n_heads / p.c.n_kv, D, p.c.n_seqs);
-  hipLaunchKernelGGL((paged_attn_kernel<D, FP8>), dim3(kMaxWG), dim3(kThreads), lds, st, p);
+  const size_t lds = (size_t)slot_floats(p.n_heads / p.c.n_kv, D, kWaves) * sizeof(float) + (size_t)p.c.n_seqs * 8;
+  hipLaunchKernelGGL((paged_attn_kernel<D, FP8, kWaves>), dim3(kMaxWG), dim3(64 * kWaves), lds, st, p);
   return 0;
 }
 
 int qh_launch_paged_attn(const QhPagedAttnParams& p, int D, hipStream_t st) {
-  if (D == 256) return p.c.ks ? launch<256, true>(p, st) : launch<256, false>(p, st);
-  return p.c.ks ? launch<128, true>(p, st) : launch<128, false>(p, st);
+  const bool four = waves_of(p.n_heads / p.c.n_kv, D, p.c.ks != nullptr) == 4;
+  if (D == 256) {
+    if (!p.c.ks) return launch<256, false, 4>(p, st);
+    return four ? launch<256, true, 4>(p, st) : launch<256, true, 8>(p, st);
+  }
+  return p.c.ks ? launch<128, true, 8>(p, st) : launch<128, false, 8>(p, st);
 }
