@@ -65,6 +65,26 @@ __device__ __forceinline__ u32x4 coherent_load(const float* src) {
   return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
 }
 
+// Cached rows are read once: non-temporal loads, which also reach 6.8 TB/s where plain
+// ones reach 6.0 (random 8 KB pages, 2.4 GB), if they ask for whole 128-byte lines.
+template <typename V>
+__device__ __forceinline__ V stream_load(const void* p) {
+  return __builtin_nontemporal_load((const V*)p);
+}
+
+// Exchange with the lane whose r differs in bit 1: x becomes the first half, y the second
+// half of the own row's line, of what load_k asked for.
+__device__ __forceinline__ void unpair(u32x4& x, u32x4& y, bool second) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t xo = __builtin_amdgcn_update_dpp(0, (int)x[i], 0x4E, 0xF, 0xF, true);  // quad_perm [2,3,0,1]
+    const uint32_t yo = __builtin_amdgcn_update_dpp(0, (int)y[i], 0x4E, 0xF, 0xF, true);
+    const uint32_t a = second ? yo : x[i], b = second ? y[i] : xo;
+    x[i] = a;
+    y[i] = b;
+  }
+}
+
 // What a wave holds of one tile.
 template <int D, bool FP8>
 struct Tile {
@@ -264,13 +284,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     return ((long long)(ok && (unsigned)id < (unsigned)p.c.n_pages ? id : 0) * Hkv + c.kvh) * ps + (ok ? off : 0);
   };
   T t;
+  // Rows of K come in whole cache lines: in a pair of loads, lanes whose r has bit 1 clear
+  // ask for the first half of a line of rows r and r + 2, the others for the second half
+  // of rows r - 2 and r; unpair() below hands each lane its own row's two halves.
+  const bool second = (r & 2) != 0;
   auto load_k = [&](const Place& c, const Ids& x) {
-    const long long row = row_of(c, x.kid, x.koff) + (r & 3);
+    const long long row = row_of(c, x.kid, x.koff) + (r & 1);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const char* src = (const char*)p.c.k + (row + 4 * a) * (FP8 ? D : 2 * D) + 16 * g;
+      const char* src = (const char*)p.c.k + (row + 4 * a) * (FP8 ? D : 2 * D) + 16 * g + (second ? 64 : 0);
 #pragma unroll
-      for (int j = 0; j < T::KL; ++j) t.k[a][j] = *(const u32x4*)(src + 64 * j);
+      for (int j = 0; j < T::KL; j += 2) {
+        t.k[a][j] = stream_load<u32x4>(src + 64 * j);
+        t.k[a][j + 1] = stream_load<u32x4>(src + 64 * j + 2 * (FP8 ? D : 2 * D));
+      }
     }
     if constexpr (FP8) {
       const long long vrow = row_of(c, x.vid, x.voff);
@@ -292,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       } else {
 #pragma unroll
         for (int j = 0; j < T::VD / 4; ++j) {
-          const u32x4 w = *(const u32x4*)(s + 16 * (r + 16 * j));
+          const u32x4 w = stream_load<u32x4>(s + 16 * (r + 16 * j));
           t.v[i][4 * j] = w.x; t.v[i][4 * j + 1] = w.y; t.v[i][4 * j + 2] = w.z; t.v[i][4 * j + 3] = w.w;
         }
       }
@@ -328,6 +355,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   f32x4 o[DT];
   float m, l;
   auto step = [&]() {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int j = 0; j < T::KL; j += 2) unpair(t.k[a][j], t.k[a][j + 1], second);
     // ---- scores ----
     f32x4 s[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
