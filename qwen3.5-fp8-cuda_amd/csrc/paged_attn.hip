@@ -65,6 +65,30 @@ __device__ __forceinline__ u32x4 coherent_load(const float* src) {
   return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
 }
 
+// 2^x as the hardware has it (1 ulp; results below 2^-126 are zero).
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Joins U more parts (maximum, sum, outputs) to (a, M, L).  One that saw nothing (sum 0,
+// maximum -inf) counts for nothing; a NaN counts.
+template <int U>
+__device__ __forceinline__ void add_parts(f32x4& a, float& M, float& L, const f32x4 (&x)[U], const float (&mx)[U],
+                                          const float (&lx)[U]) {
+  float nm = M;
+#pragma unroll
+  for (int u = 0; u < U; ++u) nm = fmaxf(nm, mx[u]);
+  const float fo = L == 0.0f ? 0.0f : exp2_(M - nm);
+  a *= fo;
+  L *= fo;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float f = lx[u] == 0.0f ? 0.0f : exp2_(mx[u] - nm);
+    L = fmaf(lx[u], f, L);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = fmaf(x[u][e], f, a[e]);
+  }
+  M = nm;
+}
+
 // Cached rows are read once: non-temporal loads, which also reach 6.8 TB/s where plain
 // ones reach 6.0 (random 8 KB pages, 2.4 GB), if they ask for whole 128-byte lines.
 template <typename V>
@@ -116,15 +140,29 @@ struct Pair {
   int b, kvh, pieces, first, tail;
 };
 
-__device__ __forceinline__ int wave_imax(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d, 64));
-  return __builtin_amdgcn_readfirstlane(v);
+// Running sum over the wave's lanes, and the maximum of all, of non-negative values by DPP
+// moves: within rows of 16 lanes, then from row to row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ int wave_isum(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return __builtin_amdgcn_readfirstlane(v);
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_i<0x111, 0xF>(v);  // row_shr:1
+  v += dpp_i<0x112, 0xF>(v);
+  v += dpp_i<0x114, 0xF>(v);
+  v += dpp_i<0x118, 0xF>(v);
+  v += dpp_i<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_i<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_imax(int v) {
+  v = max(v, dpp_i<0x111, 0xF>(v));
+  v = max(v, dpp_i<0x112, 0xF>(v));
+  v = max(v, dpp_i<0x114, 0xF>(v));
+  v = max(v, dpp_i<0x118, 0xF>(v));
+  v = max(v, dpp_i<0x142, 0xA>(v));
+  v = max(v, dpp_i<0x143, 0xC>(v));
+  return __builtin_amdgcn_readlane(v, 63);
 }
 
 template <int D, bool FP8, int kWaves>
@@ -136,7 +174,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   constexpr int KK = D / 32;                         // products of a score tile
   constexpr int RUN = FP8 ? DT : 8;                  // consecutive dims of a lane
   __shared__ int s_tot[kWaves];
-  __shared__ int s_end[kWaves];                      // where the pair that a wave did not begin ends (0: none)
   __shared__ int s_last[2];
   extern __shared__ __align__(16) float s_o[];
 
@@ -155,31 +192,32 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     for (int i = tid; i < p.n_heads * D / 8; i += kThreads)
       *(u32x4*)(p.out + (size_t)b * p.n_heads * D + i * 8) = u32x4{0u, 0u, 0u, 0u};
   };
-  auto tiles_to = [&](int b) { return b < 0 ? 0 : __builtin_amdgcn_readfirstlane(s_cum[b]); };
-  bool by_pair = false;
-  int n_lane = 0;
-  if (B <= 64) {
-    // Few sequences: lane b of every wave has sequence b, nothing goes through LDS.
+  // Up to 64 sequences: lane b of every wave has sequence b, nothing goes through LDS.
+  const bool few = B <= 64;
+  int n_lane = 0, cum_lane = 0;                      // its positions; tiles (of one KV head) of sequences 0 .. b
+  auto tiles_to = [&](int b) {
+    return b < 0 ? 0 : few ? __builtin_amdgcn_readlane(cum_lane, b) : __builtin_amdgcn_readfirstlane(s_cum[b]);
+  };
+  auto length = [&](int b) {
+    return few ? __builtin_amdgcn_readlane(n_lane, b) : __builtin_amdgcn_readfirstlane(s_n[b]);
+  };
+  int total;
+  if (few) {
     n_lane = lane < B ? max(min(p.last[lane], p.c.capacity - 1) + 1, 0) : 0;
-    const int tl = (n_lane + kTile - 1) / kTile, most = wave_imax(tl), sum = wave_isum(tl);
-    const int slots = (int)gridDim.x / Hkv;
+    const int tl = (n_lane + kTile - 1) / kTile, most = wave_imax(tl), slots = (int)gridDim.x / Hkv;
+    cum_lane = wave_scan(tl);
+    const int sum = __builtin_amdgcn_readlane(cum_lane, 63);
+    for (int b = wg; b < B; b += gridDim.x)
+      if (length(b) == 0) zeros(b);
+    total = sum * Hkv;
     if (most <= kWhole && B <= slots) share = kWhole;
     else if (4 * B <= slots) share = max(kWaves, (sum + slots - B - 1) / (slots - B));
-    by_pair = share > 0;
-    if (by_pair) {
-      const int pc = (tl + share - 1) / share;
-      int cum = pc;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(cum, d, 64);
-        cum += lane >= d ? v : 0;
-      }
-      for (int b = wg; b < B; b += gridDim.x)
-        if (__builtin_amdgcn_readlane(n_lane, b) == 0) zeros(b);
+    if (share > 0) {
+      const int pc = (tl + share - 1) / share, cum = wave_scan(pc);
       const unsigned long long past = __ballot(cum * Hkv > wg);
       if (past == 0) return;
       seg.b = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-      seg.n = __builtin_amdgcn_readlane(n_lane, seg.b);
+      seg.n = length(seg.b);
       pieces = __builtin_amdgcn_readlane(pc, seg.b);
       const int i = wg - (__builtin_amdgcn_readlane(cum, seg.b) - pieces) * Hkv;
       seg.kvh = i / pieces;
@@ -191,9 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       end = min(seg.u1, start + share);
       ws = (end - start + kWaves - 1) / kWaves;
     }
-  }
-  if (!by_pair) {
-    // the line of all tiles: a running sum over the sequences, in LDS
+  } else {
     const int per = (B + kThreads - 1) / kThreads, b0 = tid * per;
     int mine = 0;
     for (int i = 0; i < per; ++i) {
@@ -205,12 +241,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         s_cum[b] = mine;
       }
     }
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(sum, d, 64);
-      sum += lane >= d ? v : 0;
-    }
+    const int sum = wave_scan(mine);
     if (lane == 63) s_tot[wid] = sum;
     __syncthreads();
     int before = sum - mine, all = 0;
@@ -221,21 +252,28 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     }
     for (int i = 0; i < per; ++i)
       if (b0 + i < B) s_cum[b0 + i] += before;
-    const int total = __builtin_amdgcn_readfirstlane(all) * Hkv;
+    total = __builtin_amdgcn_readfirstlane(all) * Hkv;
     __syncthreads();
-    share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    ws = max(1, (share + kWaves - 1) / kWaves);
-    share = ws * kWaves;
     for (int b = wg; b < B; b += gridDim.x)
       if (s_n[b] == 0) zeros(b);
+  }
+  if (w0 < 0) {
+    // a share of the line of all tiles
+    ws = max(1, (total + (int)gridDim.x * kWaves - 1) / ((int)gridDim.x * kWaves));
+    share = ws * kWaves;
     start = wg * share;
     end = min(total, start + share);
     if (start >= end) return;
-    int lo = 0, hi = B - 1;  // the sequence of tile `start`: the first whose running sum passes it
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (tiles_to(mid) * Hkv > start) hi = mid;
-      else lo = mid + 1;
+    int lo = 0;                                      // the sequence of tile `start`: the first whose running sum passes it
+    if (few) {
+      lo = __builtin_amdgcn_readfirstlane(__ffsll(__ballot(cum_lane * Hkv > start)) - 1);
+    } else {
+      int hi = B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_to(mid) * Hkv > start) hi = mid;
+        else lo = mid + 1;
+      }
     }
     const int first = tiles_to(lo - 1), tiles = tiles_to(lo) - first;
     seg.k = start;
@@ -243,7 +281,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     seg.kvh = (start - first * Hkv) / tiles;
     seg.u0 = first * Hkv + seg.kvh * tiles;
     seg.u1 = seg.u0 + tiles;
-    seg.n = __builtin_amdgcn_readfirstlane(s_n[lo]);
+    seg.n = length(lo);
   }
   // The pair that holds tile k >= c.u0 of the line, from c on.
   auto walk = [&](Place c, int k) {
@@ -252,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       if (++c.kvh == Hkv) {
         c.kvh = 0;
         do ++c.b; while (tiles_to(c.b) == tiles_to(c.b - 1));
-        c.n = __builtin_amdgcn_readfirstlane(s_n[c.b]);
+        c.n = length(c.b);
       }
       c.u0 = c.u1;
       c.u1 += (c.n + kTile - 1) / kTile;
@@ -400,7 +438,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float nm = fmaxf(m, top);
-      const float corr = m == -INFINITY ? 0.0f : exp2f(m - nm);
+      const float corr = m == -INFINITY ? 0.0f : exp2_(m - nm);
       l *= corr;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= corr;
@@ -410,7 +448,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float e = exp2f(x[i] - ref);
+      const float e = exp2_(x[i] - ref);
       l += e;
       w[i] = FP8 ? (i < left ? e * vs[i] : 0.0f) : e;
     }
@@ -502,20 +540,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       }
     }
   };
-  // A part that saw nothing (sum 0) counts for nothing; a NaN counts.
-  auto add_part = [&](f32x4& a, float& M, float& L, f32x4 x, float mx, float lx) {
-    const float nm = fmaxf(M, mx);
-    const float fo = L == 0.0f ? 0.0f : exp2f(M - nm), fn = lx == 0.0f ? 0.0f : exp2f(mx - nm);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = fmaf(x[e], fn, a[e] * fo);
-    L = L * fo + lx * fn;
-    M = nm;
-  };
-
   // ---- this wave's pairs, one after the other -------------------------------------------
   Place at = A;
-  if (tid < kWaves) s_end[tid] = 0;
-  __syncthreads();
   if (k0 < k1) {
     while (true) {
       const int s1 = min(at.u1, k1);
@@ -537,13 +563,22 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         load_q(at);
       }
       put_slot(2 * wid + (begun ? 0 : 1));
-      if (begun && lane == 0) s_end[wid] = done.u1;
       if (!begun && done.u1 <= k1) {                 // all of it is here
         const float* src = slot_of(2 * wid + 1);
-        for (int i = lane; i < items; i += 64) {
-          const Item it = item(i);
-          const int head = done.kvh * G + it.h;
-          emit(done.b, head, it.c, ((const f32x4*)src)[i], src[G * D + kMaxG + it.h], gate_of(done.b, head, it.c));
+        for (int i0 = lane; i0 < items; i0 += 256) {
+          u32x2 gt[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const Item it = item(min(i0 + 64 * u, items - 1));
+            gt[u] = gate_of(done.b, done.kvh * G + it.h, it.c);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 64 * u;
+            if (i >= items) break;
+            const Item it = item(i);
+            emit(done.b, done.kvh * G + it.h, it.c, ((const f32x4*)src)[i], src[G * D + kMaxG + it.h], gt[u]);
+          }
         }
       }
       if (!more) break;
@@ -563,29 +598,30 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   };
   {
     Place c = seg;
-    for (int w = 0; w < kWaves; ++w) {
-      // the pair that goes on behind wave w (w = 0: also the one begun before this workgroup)
-#pragma unroll 1
-      for (int part = w == 0 ? 0 : 1; part < 2; ++part) {
-        const int kw = start + w * ws, kn = min(end, kw + ws);
-        if (kw >= end) break;
-        const int k = part == 0 ? kw : kn - 1;
-        if (k >= c.u1) c = walk(c, k);
-        const bool here = c.u0 >= start, all = here && c.u1 <= end;
-        if (part == 0 ? here : !(c.u0 >= kw && c.u1 > kn) && !(c.u0 >= kw && !all)) continue;
-        const int last = (min(c.u1, end) - 1 - start) / ws;
+    while (true) {
+      // pair c lies in waves w .. last; wave w began it, or (w = 0) another workgroup
+      const bool begun = c.u0 < start, all = !begun && c.u1 <= end;
+      const int w = begun ? 0 : (c.u0 - start) / ws, last = (min(c.u1, end) - 1 - start) / ws;
+      if (!all || last > w) {
         float* dst = p.part + (size_t)(2 * wg + (c.u0 > start ? 1 : 0)) * rec;
         const auto rs = __builtin_amdgcn_make_buffer_rsrc(dst, (short)0, rec * 4, 0x00020000);
         for (int i = tid; i < items; i += kThreads) {
           const Item it = item(i);
           const int head = c.kvh * G + it.h;
           const u32x2 gt = all ? gate_of(c.b, head, it.c) : u32x2{0u, 0u};
-          float M = -INFINITY, L = 0.0f;
+          f32x4 y[kWaves];
+          float my[kWaves], ly[kWaves], M = -INFINITY, L = 0.0f;
           f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int x = w; x <= last; ++x) {
-            const float* src = slot_of(2 * x + (x == w ? part : 0));
-            add_part(a, M, L, ((const f32x4*)src)[i], src[G * D + it.h], src[G * D + kMaxG + it.h]);
+#pragma unroll
+          for (int u = 0; u < kWaves; ++u) {
+            const bool in = w + u <= last;
+            const int x = min(w + u, last);
+            const float* src = slot_of(2 * x + (x == w && !begun ? 1 : 0));
+            y[u] = in ? ((const f32x4*)src)[i] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            my[u] = in ? src[G * D + it.h] : -INFINITY;
+            ly[u] = in ? src[G * D + kMaxG + it.h] : 0.0f;
           }
+          add_parts(a, M, L, y, my, ly);
           if (all) {
             emit(c.b, head, it.c, a, L, gt);
           } else {
@@ -601,6 +637,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
           else open0 = pair_of(c);
         }
       }
+      if (c.u1 >= end) break;
+      // the next one that waves may cut holds the last tile of a wave, of this one's last or the one after
+      const int kn = min(end, start + (last + 1) * ws);
+      c = walk(c, kn > c.u1 ? kn - 1 : min(end, kn + ws) - 1);
     }
   }
   // A share holds at most two pairs that other workgroups hold too, its first and its last.
@@ -636,20 +676,23 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       u32x2 gt = {0u, 0u};
       if (i < items && sub < subs) {
         gt = gate_of(x.b, head, it.c);
-        constexpr int U = 8;
+        constexpr int U = 16;
         for (int j = sub; j < x.pieces; j += U * subs) {
-          u32x4 y[U];
+          f32x4 y[U];
           float my[U], ly[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const float* src = rec_of(min(j + u * subs, x.pieces - 1));
-            y[u] = coherent_load(src + 4 * i);
-            my[u] = pub_load(src + G * D + it.h);
-            ly[u] = pub_load(src + G * D + kMaxG + it.h);
+            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            my[u] = -INFINITY;
+            ly[u] = 0.0f;
+            if (j + u * subs < x.pieces) {
+              const float* src = rec_of(j + u * subs);
+              y[u] = __builtin_bit_cast(f32x4, coherent_load(src + 4 * i));
+              my[u] = pub_load(src + G * D + it.h);
+              ly[u] = pub_load(src + G * D + kMaxG + it.h);
+            }
           }
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (j + u * subs < x.pieces) add_part(a, M, L, __builtin_bit_cast(f32x4, y[u]), my[u], ly[u]);
+          add_parts(a, M, L, y, my, ly);
         }
       }
       if (subs > 1) {
@@ -657,7 +700,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         s_ml[tid] = float2{M, L};
         __syncthreads();
         if (sub == 0)
-          for (int k = 1; k < subs; ++k) add_part(a, M, L, s_a[k * items + i], s_ml[k * items + i].x, s_ml[k * items + i].y);
+          for (int k = 1; k < subs; ++k) {
+            const f32x4 y[1] = {s_a[k * items + i]};
+            const float my[1] = {s_ml[k * items + i].x}, ly[1] = {s_ml[k * items + i].y};
+            add_parts(a, M, L, y, my, ly);
+          }
       }
       if (i < items && sub == 0) emit(x.b, head, it.c, a, L, gt);
     }
