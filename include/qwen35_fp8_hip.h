@@ -432,7 +432,8 @@ int qh_attn_prep_paged(const qh_paged_cache* cache, const qh_rope_axes* rope, co
 
 /* Positions 0 .. last[b] of each sequence as dense bf16 rows: k_out, v_out
  * [n_seqs][n_kv][max_seq][D], the layout qh_attn_prefill reads (one sequence of it:
- * its k_cache, v_cache and max_seq).  Rows behind last[b] keep what they hold. */
+ * its k_cache, v_cache and max_seq).  Rows behind last[b] keep what they hold.  At most
+ * 65535 (sequence, KV head) pairs; 16-byte aligned outputs. */
 int qh_kv_read_paged(const qh_paged_cache* cache, const int* pages, int n_seqs, int max_pages,
                      const int* last, void* k_out, void* v_out, int max_seq, qh_stream_t stream);
 

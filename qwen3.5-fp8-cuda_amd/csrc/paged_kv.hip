@@ -14,6 +14,8 @@
 // All in fp32 with one rounding at the end: the intermediate bf16 roundings of the
 // dense path (which the reference's tensors have) would be rounded again to three
 // mantissa bits here, and a second rounding moves a value in 16 to another code.
+#include <algorithm>
+
 #include "qh_common.h"
 #include "qh_paged.h"
 
@@ -35,125 +37,262 @@ __device__ __forceinline__ int axis_of(const qh_rope_axes& r, int i) {
   return a;
 }
 
-// Where a token's rows go: the page and the slot in it, or page -1 for a token
-// that is left out (a row of padding, or an index outside its range).
-struct Slot {
-  int page, off;
-};
-__device__ __forceinline__ Slot slot_of(const QhPagedPrepParams& p, int t) {
-  const int s = p.seq ? p.seq[t] : t, at = p.at[t];
-  Slot r = {-1, 0};
-  if (s < 0 || s >= p.c.n_seqs || at < 0 || at >= p.c.capacity) return r;
-  for (int a = 0; a < p.rope.n_axes; ++a) {
-    const int x = p.pos[(size_t)a * p.T + t];
-    if (x < 0 || x >= p.rope.max_pos) return r;
-  }
-  const int pg = page_of(p.c, at);
-  const int id = p.c.pages[(size_t)s * p.c.max_pages + pg];
-  if (id < 0 || id >= p.c.n_pages) return r;
-  r.page = id;
-  r.off = at - pg * p.c.page_size;
-  return r;
-}
-
 constexpr float kMinScale = 7.8886090522101181e-31f;  // 2^-100
 
-// One wave per (token, head row): q heads, then k heads, then v heads.
-template <int D>
-__global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p) {
-  constexpr int NPL = D / 64;
-  const int nq = p.q ? p.n_heads : 0, rows = nq + 2 * p.c.n_kv, lane = threadIdx.x & 63;
-  const long long idx = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (idx >= (long long)p.T * rows) return;
-  const int t = (int)(idx / rows), row = (int)(idx - (long long)t * rows);
-  const Slot slot = slot_of(p, t);
-  if (slot.page < 0) return;
-  const int kind = row < nq ? 0 : row < nq + p.c.n_kv ? 1 : 2;  // q, k, v
-  const int head = kind == 0 ? row : kind == 1 ? row - nq : row - nq - p.c.n_kv;
-  const uint16_t* src = kind == 0   ? p.q + t * p.q_ts + head * p.q_hs
-                        : kind == 1 ? p.k + t * p.k_ts + (long long)head * D
-                                    : p.v + t * p.v_ts + (long long)head * D;
-  const float* nw = kind == 0 ? p.q_norm_w : kind == 1 ? p.k_norm_w : nullptr;
-  float x[NPL];
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) x[i] = bf2f(src[lane * NPL + i]);
-  if (nw) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) ss = fmaf(x[i], x[i], ss);
-    const float r = rsqrtf(wave_sum(ss) / (float)D + p.eps);
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) x[i] = x[i] * r * (1.0f + nw[lane * NPL + i]);
+// Sum and maximum over the row's LPR (16 or 32) lanes, in all of them: DPP moves within
+// 16 lanes, then the neighbouring 16.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+  v = column_sum<16>(v);
+  if constexpr (LPR == 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
   }
-  if (kind < 2 && p.rope.rot > 0) {
-    const int half = p.rope.rot >> 1, dl = half / NPL;  // rot % 16 == 0: partners are whole lanes apart
-    const int c0 = lane * NPL;
-    const int from = c0 < half ? lane + dl : c0 < 2 * half ? lane - dl : lane;
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_src<0xB1, 0xF>(v));
+  v = fmaxf(v, dpp_src<0x4E, 0xF>(v));
+  v = fmaxf(v, dpp_src<0x141, 0xF>(v));
+  v = fmaxf(v, dpp_src<0x140, 0xF>(v));
+  if constexpr (LPR == 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  }
+  return v;
+}
+
+__device__ __forceinline__ void unpack8(float (&x)[8], u32x4 u) {
+  x[0] = bf_lo(u.x); x[1] = bf_hi(u.x); x[2] = bf_lo(u.y); x[3] = bf_hi(u.y);
+  x[4] = bf_lo(u.z); x[5] = bf_hi(u.z); x[6] = bf_lo(u.w); x[7] = bf_hi(u.w);
+}
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  return u32x4{pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
+}
+
+constexpr int kPrepTokens = 8;  // tokens of a workgroup, at most
+
+// How the rows of a launch are dealt out (host).
+struct PrepPlan {
+  int tokens;         // of a workgroup (blockIdx.x)
+  int rows;           // of a token: its q, k and v heads
+  int span;           // rows of a workgroup (blockIdx.y: which of its tokens' rows)
+  uint32_t rows_mul;  // j / rows = umulhi(j, rows_mul) for the row numbers of a workgroup
+};
+
+// E4M3 codes of 4 values: v / s with rs = 1 / s rounded, corrected by the quotient's
+// residual, which gives the correctly rounded quotient (Markstein 1990): a tie between
+// two codes, common for bf16 values, is the tie that the division has.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float s, float rs) {
+  auto div = [&](float v) {
+    const float q = v * rs;
+    return copysignf(fmaf(fmaf(-q, s, v), rs, q), v);  // of -0 the correction makes +0
+  };
+  uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(div(a), div(b), 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(div(c), div(d), w, true);
+}
+
+// D / 8 lanes take a row, 16 bytes of input each, R rows at a time with all of their loads
+// ahead of the first use.  Where the rows of a workgroup's tokens go and the cos and sin
+// of their pairs (which the axes gather from up to four rows of the tables) are found
+// once a token and kept in LDS, behind the request for the first rows.  HBM bounds it
+// for prompts, the chain position -> table and index -> page -> row for single tokens.
+template <int D, int R>
+__global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, PrepPlan pl) {
+  constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a pass
+  __shared__ __align__(16) float s_cos[kPrepTokens * D / 2], s_sin[kPrepTokens * D / 2];
+  __shared__ long long s_row[kPrepTokens];     // the token's slot in its page's first head, -1: left out
+  const int tid = threadIdx.x, t0 = blockIdx.x * pl.tokens, nt = min(pl.tokens, p.T - t0);
+  const int nq = p.q ? p.n_heads : 0, Hkv = p.c.n_kv;
+  const int first = blockIdx.y * pl.span, total = min(nt * pl.rows, first + pl.span);
+  if (first >= total) return;
+  const int half = p.rope.rot >> 1;
+  const int mine = first + tid / LPR, ln = tid % LPR, c0 = ln * 8;
+
+  // Row j of the workgroup's tokens: its token, and which q (kind 0), k (1) or v (2) head.
+  struct Row { int t, head, kind; };
+  auto row_of = [&](int j) {
+    Row r;
+    r.t = pl.tokens == 1 ? 0 : (int)__umulhi((unsigned)j, pl.rows_mul);
+    const int row = j - r.t * pl.rows;
+    r.kind = (row >= nq ? 1 : 0) + (row >= nq + Hkv ? 1 : 0);
+    r.head = row - (r.kind == 0 ? 0 : r.kind == 1 ? nq : nq + Hkv);
+    return r;
+  };
+  u32x4 x0[R];
+  auto fetch = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const float other = __shfl(x[i], from, 64);
-      const int c = c0 + i;
-      if (c < 2 * half) {
-        const int pair = c < half ? c : c - half;
-        const size_t e = (size_t)p.pos[(size_t)axis_of(p.rope, pair) * p.T + t] * p.rope.rot + pair;
-        const float cs = p.rope.cos_t[e], sn = p.rope.sin_t[e];
-        x[i] = c < half ? x[i] * cs - other * sn : x[i] * cs + other * sn;
+    for (int u = 0; u < R; ++u) {
+      const Row r = row_of(min(j0 + u * RPB, total - 1));
+      const uint16_t* src = r.kind == 0 ? p.q : r.kind == 1 ? p.k : p.v;
+      const long long ts = r.kind == 0 ? p.q_ts : r.kind == 1 ? p.k_ts : p.v_ts, hs = r.kind == 0 ? p.q_hs : D;
+      x0[u] = *(const u32x4*)(src + (t0 + r.t) * ts + r.head * hs + c0);
+    }
+  };
+  fetch(mine);
+  // Where token t's rows go.  A row of padding, or an index outside its range: nowhere.
+  if (tid < nt) {
+    const int t = t0 + tid, s = p.seq ? p.seq[t] : t, at = p.at[t];
+    bool ok = s >= 0 && s < p.c.n_seqs && at >= 0 && at < p.c.capacity;
+    const int pg = page_of(p.c, ok ? at : 0), id = p.c.pages[(size_t)(ok ? s : 0) * p.c.max_pages + pg];
+    ok = ok && id >= 0 && id < p.c.n_pages;
+    for (int a = 0; a < p.rope.n_axes; ++a) {
+      const int x = p.pos[(size_t)a * p.T + t];
+      ok = ok && x >= 0 && x < p.rope.max_pos;
+    }
+    s_row[tid] = ok ? (long long)id * Hkv * p.c.page_size + (at - pg * p.c.page_size) : -1;
+  }
+  for (int i = tid; i < nt * half; i += 256) {
+    const int t = i / half, pair = i - t * half;
+    const int x = p.pos[(size_t)axis_of(p.rope, pair) * p.T + t0 + t];
+    const size_t e = (size_t)min(max(x, 0), p.rope.max_pos - 1) * p.rope.rot + pair;
+    s_cos[t * half + pair] = p.rope.cos_t[e];
+    s_sin[t * half + pair] = p.rope.sin_t[e];
+  }
+  f32x4 qw[2], kw[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x4 one = {1.0f, 1.0f, 1.0f, 1.0f};
+    qw[i] = p.q_norm_w ? one + *(const f32x4*)(p.q_norm_w + c0 + 4 * i) : one;
+    kw[i] = p.k_norm_w ? one + *(const f32x4*)(p.k_norm_w + c0 + 4 * i) : one;
+  }
+  __syncthreads();
+
+  const int lane = tid & 63, dl = half / 8;    // rot % 16 == 0: a pair's two halves are whole lanes apart
+  const bool lower = c0 < half, turned = c0 < 2 * half;
+  const int from = 4 * (lower ? lane + dl : turned ? lane - dl : lane);
+  for (int j0 = mine; j0 - mine + first < total; j0 += R * RPB) {
+    u32x4 raw[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) raw[u] = x0[u];
+    if (j0 - mine + first + R * RPB < total) fetch(j0 + R * RPB);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const int j = j0 + u * RPB;
+      if (j - mine + first >= total) break;    // the same for the whole workgroup
+      const Row r = row_of(min(j, total - 1));
+      const long long base = j < total ? s_row[r.t] : -1;
+      float x[8];
+      unpack8(x, raw[u]);
+      if (r.kind == 0 ? p.q_norm_w != nullptr : r.kind == 1 && p.k_norm_w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+        const float rs = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * (r.kind == 0 ? qw[i / 4][i % 4] : kw[i / 4][i % 4]);
+      }
+      if (half > 0 && __any(r.kind < 2)) {
+        // every lane of the wave takes part: its rows may be of different kinds
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          y[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[i])));
+        if (r.kind < 2 && turned) {
+          const int e = r.t * half + (lower ? c0 : c0 - half);
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const f32x4 cs = *(const f32x4*)(s_cos + e + i);
+            f32x4 sn = *(const f32x4*)(s_sin + e + i);
+            if (lower) sn = -sn;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[i + k] = x[i + k] * cs[k] + y[i + k] * sn[k];
+          }
+        }
+      }
+      if (r.kind == 0) {
+        const size_t o = ((size_t)(t0 + r.t) * p.n_heads + r.head) * D + c0;
+        if (base >= 0) {
+          if (p.q_f32) {
+            *(f32x4*)((float*)p.q_out + o) = f32x4{x[0], x[1], x[2], x[3]};
+            *(f32x4*)((float*)p.q_out + o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+          } else {
+            *(u32x4*)((uint16_t*)p.q_out + o) = pack8(x);
+          }
+        }
+        continue;
+      }
+      void* dst = r.kind == 1 ? p.c.k : p.c.v;
+      const long long row = base + (long long)r.head * p.c.page_size;
+      if (!p.c.ks) {
+        if (base >= 0) *(u32x4*)((uint16_t*)dst + row * D + c0) = pack8(x);
+        continue;
+      }
+      float a = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[i]));   // of a NaN and a number: the number
+      a = row_max<LPR>(a);
+      if (a == INFINITY) {                     // the scale is that of the finite values, an infinity a NaN
+        a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = fabsf(x[i]) < INFINITY ? x[i] : NAN;
+          a = fmaxf(a, fabsf(x[i]));
+        }
+        a = row_max<LPR>(a);
+      }
+      const float s = fmaxf(a / 448.0f, kMinScale), rs = 1.0f / s;
+      const u32x2 w = {e4m3x4(x[0], x[1], x[2], x[3], s, rs), e4m3x4(x[4], x[5], x[6], x[7], s, rs)};
+      if (base >= 0) {
+        if (ln == 0) (r.kind == 1 ? p.c.ks : p.c.vs)[row] = s;
+        *(u32x2*)((uint8_t*)dst + row * D + c0) = w;
       }
     }
   }
-  if (kind == 0) {
-    const size_t o = ((size_t)t * p.n_heads + head) * D + lane * NPL;
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      if (p.q_f32) ((float*)p.q_out)[o + i] = x[i];
-      else ((uint16_t*)p.q_out)[o + i] = f2bf(x[i]);
-    }
-    return;
-  }
-  const size_t r = ((size_t)slot.page * p.c.n_kv + head) * p.c.page_size + slot.off;
-  void* dst = kind == 1 ? p.c.k : p.c.v;
-  if (!p.c.ks) {
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) ((uint16_t*)dst)[r * D + lane * NPL + i] = f2bf(x[i]);
-    return;
-  }
-  float a = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) a = fmaxf(a, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
-  const float s = fmaxf(wave_max(a) / 448.0f, kMinScale);
-  if (lane == 0) (kind == 1 ? p.c.ks : p.c.vs)[r] = s;
-#pragma unroll
-  for (int i = 0; i < NPL; i += 2) {
-    const float u = fabsf(x[i]) < INFINITY ? x[i] / s : NAN;
-    const float w = fabsf(x[i + 1]) < INFINITY ? x[i + 1] / s : NAN;
-    ((uint16_t*)dst)[(r * D + lane * NPL + i) / 2] = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(u, w, 0, false);
-  }
 }
 
-// Read back (qh_kv_read_paged): one wave per position and KV head.
+// Read back (qh_kv_read_paged): 16 bytes of a cached row a lane, K and V side by side,
+// kReadRows rows of each under way together.  A workgroup takes positions blockIdx.x,
+// blockIdx.x + gridDim.x, ... (in units of its rows) of one sequence and KV head.
+constexpr int kReadRows = 2;
 template <int D, bool FP8>
 __global__ __launch_bounds__(256) void paged_read_kernel(QhPagedReadParams p) {
-  constexpr int NPL = D / 64;
-  const int b = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 63;
-  const int pos = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int n = min(min(p.last[b], p.max_seq - 1), p.c.capacity - 1);
-  if (pos > n) return;
-  const int pg = page_of(p.c, pos), id = p.c.pages[(size_t)b * p.c.max_pages + pg];
-  if (id < 0 || id >= p.c.n_pages) return;
-  const size_t r = ((size_t)id * p.c.n_kv + head) * p.c.page_size + (pos - pg * p.c.page_size);
-  const size_t o = (((size_t)b * p.c.n_kv + head) * p.max_seq + pos) * D + lane * NPL;
+  constexpr int E = FP8 ? 16 : 8;              // values of 16 cached bytes
+  constexpr int LPR = D / E, RPB = 256 / LPR * kReadRows;
+  const int pair = blockIdx.y, b = pair / p.c.n_kv, head = pair - b * p.c.n_kv;
+  const int n = min(min(p.last[b], p.max_seq - 1), p.c.capacity - 1) + 1;
+  const int* pages = p.c.pages + (size_t)b * p.c.max_pages;
+  const int mine = threadIdx.x / LPR, c = threadIdx.x % LPR * E;
+  for (int p0 = blockIdx.x * RPB; p0 < n; p0 += gridDim.x * RPB) {
+    long long row[kReadRows];
+    u32x4 k[kReadRows], v[kReadRows];
+    float ks[kReadRows], vs[kReadRows];
+    bool ok[kReadRows];
 #pragma unroll
-  for (int i = 0; i < NPL; i += 2) {
-    if constexpr (FP8) {
-      const uint32_t kk = ((const uint16_t*)p.c.k)[(r * D + lane * NPL + i) / 2];
-      const uint32_t vv = ((const uint16_t*)p.c.v)[(r * D + lane * NPL + i) / 2];
-      const qh_f32x2 kf = e4m3x2_lo_f32(kk), vf = e4m3x2_lo_f32(vv);
-      const float ks = p.c.ks[r], vs = p.c.vs[r];
-      *(uint32_t*)(p.k_out + o + i) = pack_bf2(kf.x * ks, kf.y * ks);
-      *(uint32_t*)(p.v_out + o + i) = pack_bf2(vf.x * vs, vf.y * vs);
-    } else {
-      *(uint32_t*)(p.k_out + o + i) = *(const uint32_t*)((const uint16_t*)p.c.k + r * D + lane * NPL + i);
-      *(uint32_t*)(p.v_out + o + i) = *(const uint32_t*)((const uint16_t*)p.c.v + r * D + lane * NPL + i);
+    for (int u = 0; u < kReadRows; ++u) {
+      const int pos = p0 + mine + u * (256 / LPR), at = min(pos, n - 1), pg = page_of(p.c, at), id = pages[pg];
+      ok[u] = pos < n && (unsigned)id < (unsigned)p.c.n_pages;
+      row[u] = ((long long)(ok[u] ? id : 0) * p.c.n_kv + head) * p.c.page_size + (at - pg * p.c.page_size);
+    }
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+      const size_t o = (size_t)row[u] * D + c;
+      k[u] = __builtin_nontemporal_load((const u32x4*)((const char*)p.c.k + o * (16 / E)));
+      v[u] = __builtin_nontemporal_load((const u32x4*)((const char*)p.c.v + o * (16 / E)));
+      ks[u] = FP8 ? p.c.ks[row[u]] : 1.0f;
+      vs[u] = FP8 ? p.c.vs[row[u]] : 1.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+      if (!ok[u]) continue;
+      const size_t o = ((size_t)pair * p.max_seq + p0 + mine + u * (256 / LPR)) * D + c;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          auto four = [](uint32_t x, float s) {
+            const qh_f32x2 lo = e4m3x2_lo_f32(x), hi = e4m3x2_hi_f32(x);
+            return u32x2{pack_bf2(lo.x * s, lo.y * s), pack_bf2(hi.x * s, hi.y * s)};
+          };
+          const u32x2 k0 = four(k[u][i], ks[u]), k1 = four(k[u][i + 1], ks[u]);
+          const u32x2 v0 = four(v[u][i], vs[u]), v1 = four(v[u][i + 1], vs[u]);
+          *(u32x4*)(p.k_out + o + 4 * i) = u32x4{k0.x, k0.y, k1.x, k1.y};
+          *(u32x4*)(p.v_out + o + 4 * i) = u32x4{v0.x, v0.y, v1.x, v1.y};
+        }
+      } else {
+        *(u32x4*)(p.k_out + o) = k[u];
+        *(u32x4*)(p.v_out + o) = v[u];
+      }
     }
   }
 }
@@ -216,8 +355,8 @@ int qh_paged_view(const qh_paged_cache* c, const int* pages, int n_seqs, int max
 
 int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
   const char* what = "attn_prep_paged";
-  if (p.T < 0 || (p.q && p.n_heads < 1)) {
-    qh_set_error("%s: T=%d n_heads=%d", what, p.T, p.n_heads);
+  if (p.T < 0 || (p.q && (p.n_heads < 1 || p.n_heads > 4096)) || p.c.n_kv > 4096) {
+    qh_set_error("%s: T=%d n_heads=%d n_kv=%d (at most 4096 heads)", what, p.T, p.n_heads, p.c.n_kv);
     return -1;
   }
   if (!p.seq && p.T > p.c.n_seqs) {
@@ -265,20 +404,26 @@ int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
       return -1;
     }
   }
-  const long long rows = (long long)p.T * ((p.q ? p.n_heads : 0) + 2LL * p.c.n_kv), blocks = (rows + 3) / 4;
-  if (blocks > 0x7FFFFFFFLL) {
-    qh_set_error("%s: T=%d tokens are more than one launch takes", what, p.T);
-    return -1;
-  }
-  if (D == 256) hipLaunchKernelGGL(paged_prep_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(paged_prep_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  const int rows = (p.q ? p.n_heads : 0) + 2 * p.c.n_kv, pass = 256 / (D / 8);
+  PrepPlan pl;
+  pl.rows = rows;
+  // A row a thread while that leaves no more than some four workgroups a CU; then
+  // workgroups of several tokens that still fill the CUs four times.
+  const bool few = (long long)p.T * ((rows + pass - 1) / pass) <= 1024;
+  pl.tokens = few ? 1 : std::min(kPrepTokens, std::max(1, p.T / 1024));
+  pl.span = few ? pass : pl.tokens * rows;
+  pl.rows_mul = (uint32_t)((1ull << 32) / rows + 1);
+  const dim3 grid((p.T + pl.tokens - 1) / pl.tokens, few ? (rows + pass - 1) / pass : 1);
+  auto fn = D == 256 ? (few ? paged_prep_kernel<256, 1> : paged_prep_kernel<256, 4>)
+                     : (few ? paged_prep_kernel<128, 1> : paged_prep_kernel<128, 4>);
+  hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, p, pl);
   return 0;
 }
 
 int qh_launch_paged_read(const QhPagedReadParams& p, int D, hipStream_t st) {
   const char* what = "kv_read_paged";
-  if (p.max_seq < 1 || p.c.n_kv > 65535) {
-    qh_set_error("%s: max_seq=%d n_kv=%d", what, p.max_seq, p.c.n_kv);
+  if (p.max_seq < 1 || (long long)p.c.n_seqs * p.c.n_kv > 65535) {
+    qh_set_error("%s: max_seq=%d n_seqs=%d n_kv=%d (at most 65535 pairs)", what, p.max_seq, p.c.n_seqs, p.c.n_kv);
     return -1;
   }
   if (p.c.n_seqs == 0) return 0;
@@ -290,8 +435,9 @@ int qh_launch_paged_read(const QhPagedReadParams& p, int D, hipStream_t st) {
     qh_set_error("%s: outputs must be 16-byte aligned", what);
     return -1;
   }
-  const int most = p.max_seq < p.c.capacity ? p.max_seq : p.c.capacity;
-  const dim3 grid((most + 3) / 4, p.c.n_kv, p.c.n_seqs);
+  const int most = std::min(p.max_seq, p.c.capacity), pairs = p.c.n_seqs * p.c.n_kv;
+  const int rows = 256 / (D / (p.c.ks ? 16 : 8)) * kReadRows;
+  const dim3 grid(std::max(1, std::min((most + rows - 1) / rows, 16384 / pairs)), pairs);
   if (D == 256) {
     if (p.c.ks) hipLaunchKernelGGL((paged_read_kernel<256, true>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((paged_read_kernel<256, false>), grid, dim3(256), 0, st, p);

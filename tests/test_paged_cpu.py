@@ -84,6 +84,8 @@ def test_null_descriptor():
 @pytest.mark.parametrize("bad,said", [
     (dict(T=-1), "T=-1"),
     (dict(heads=0), "n_heads"),
+    (dict(heads=4097), "4096 heads"),
+    (dict(c=cache(n_kv=4097)), "4096 heads"),
     (dict(seq=None, T=3), "one per sequence"),
     (dict(k=None), "null pointer"),
     (dict(v=None), "null pointer"),
@@ -97,7 +99,6 @@ def test_null_descriptor():
     (dict(q=ctypes.c_void_p(4098)), "aligned"),
     (dict(q_out=ctypes.c_void_p(4104)), "aligned"),
     (dict(qn=ctypes.c_void_p(4100)), "aligned"),
-    (dict(T=0x7FFFFFFF, heads=16), "one launch"),
 ])
 def test_prep_refusals(bad, said):
     assert prep(**bad) == -1
@@ -154,6 +155,11 @@ def test_read_refusals(bad):
 def test_attention_refusals(bad, said):
     assert attend(**bad) == -1
     assert said in abi.last_error()
+
+
+def test_read_pairs_limit():
+    assert read(cache(n_kv=64), n_seqs=1024) == -1
+    assert "pairs" in abi.last_error()
 
 
 def test_attention_pairs_limit():
