@@ -71,19 +71,11 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return u32x4{pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
 }
 
-constexpr int kPrepTokens = 8;  // tokens of a workgroup, at most
+constexpr int kPrepTokens = 4;  // tokens of a workgroup, at most
 
-// How the rows of a launch are dealt out (host).
-struct PrepPlan {
-  int tokens;         // of a workgroup (blockIdx.x)
-  int rows;           // of a token: its q, k and v heads
-  int span;           // rows of a workgroup (blockIdx.y: which of its tokens' rows)
-  uint32_t rows_mul;  // j / rows = umulhi(j, rows_mul) for the row numbers of a workgroup
-};
-
-// E4M3 codes of 4 values: v / s with rs = 1 / s rounded, corrected by the quotient's
-// residual, which gives the correctly rounded quotient (Markstein 1990): a tie between
-// two codes, common for bf16 values, is the tie that the division has.
+// E4M3 codes of 4 values: v / s with rs close to 1 / s, corrected by the quotient's
+// residual: a tie between two codes, common for bf16 values, is the tie that the exact
+// division has.
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float s, float rs) {
   auto div = [&](float v) {
     const float q = v * rs;
@@ -93,44 +85,40 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, f
   return __builtin_amdgcn_cvt_pk_fp8_f32(div(c), div(d), w, true);
 }
 
-// D / 8 lanes take a row, 16 bytes of input each, R rows at a time with all of their loads
-// ahead of the first use.  Where the rows of a workgroup's tokens go and the cos and sin
-// of their pairs (which the axes gather from up to four rows of the tables) are found
-// once a token and kept in LDS, behind the request for the first rows.  HBM bounds it
-// for prompts, the chain position -> table and index -> page -> row for single tokens.
+// D / 8 lanes take a row, 16 bytes of input each.  A thread has the same R heads in each of
+// its workgroup's tokens (blockIdx.y: which heads), so that what a head needs is found
+// once; the next token's rows are under way while one is computed.  Where the tokens'
+// rows go and the cos and sin of their pairs (which the axes gather from up to four rows
+// of the tables) are found once a token and kept in LDS, behind the request for the
+// first rows.  HBM bounds it for prompts, the chain position -> table and index -> page
+// -> row for single tokens.
 template <int D, int R>
-__global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, PrepPlan pl) {
+__global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, int tokens) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a pass
-  __shared__ __align__(16) float s_cos[kPrepTokens * D / 2], s_sin[kPrepTokens * D / 2];
+  __shared__ __align__(16) float s_cos[kPrepTokens * D / 2], s_sin[2][kPrepTokens * D / 2];  // [0]: -sin
+  __shared__ __align__(16) float s_w[2][D];    // 1 + w of q and k
   __shared__ long long s_row[kPrepTokens];     // the token's slot in its page's first head, -1: left out
-  const int tid = threadIdx.x, t0 = blockIdx.x * pl.tokens, nt = min(pl.tokens, p.T - t0);
-  const int nq = p.q ? p.n_heads : 0, Hkv = p.c.n_kv;
-  const int first = blockIdx.y * pl.span, total = min(nt * pl.rows, first + pl.span);
-  if (first >= total) return;
+  const int tid = threadIdx.x, t0 = blockIdx.x * tokens, nt = min(tokens, p.T - t0);
+  const int nq = p.q ? p.n_heads : 0, Hkv = p.c.n_kv, rows = nq + 2 * Hkv;
   const int half = p.rope.rot >> 1;
-  const int mine = first + tid / LPR, ln = tid % LPR, c0 = ln * 8;
+  const int ln = tid % LPR, c0 = ln * 8;
 
-  // Row j of the workgroup's tokens: its token, and which q (kind 0), k (1) or v (2) head.
-  struct Row { int t, head, kind; };
-  auto row_of = [&](int j) {
-    Row r;
-    r.t = pl.tokens == 1 ? 0 : (int)__umulhi((unsigned)j, pl.rows_mul);
-    const int row = j - r.t * pl.rows;
-    r.kind = (row >= nq ? 1 : 0) + (row >= nq + Hkv ? 1 : 0);
-    r.head = row - (r.kind == 0 ? 0 : r.kind == 1 ? nq : nq + Hkv);
-    return r;
-  };
-  u32x4 x0[R];
-  auto fetch = [&](int j0) {
+  // The thread's heads: q (kind 0), k (1), v (2) or none (3).
+  int kind[R], head[R];
+  const uint16_t* src[R];
+  long long ts[R];
+  u32x4 next[R];
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      const Row r = row_of(min(j0 + u * RPB, total - 1));
-      const uint16_t* src = r.kind == 0 ? p.q : r.kind == 1 ? p.k : p.v;
-      const long long ts = r.kind == 0 ? p.q_ts : r.kind == 1 ? p.k_ts : p.v_ts, hs = r.kind == 0 ? p.q_hs : D;
-      x0[u] = *(const u32x4*)(src + (t0 + r.t) * ts + r.head * hs + c0);
-    }
-  };
-  fetch(mine);
+  for (int u = 0; u < R; ++u) {
+    const int row = (int)(blockIdx.y * R + u) * RPB + tid / LPR;
+    kind[u] = row < nq ? 0 : row < nq + Hkv ? 1 : row < rows ? 2 : 3;
+    head[u] = row - (kind[u] == 0 ? 0 : kind[u] == 1 ? nq : nq + Hkv);
+    if (kind[u] == 3) head[u] = 0;
+    src[u] = kind[u] == 0 ? p.q + head[u] * p.q_hs : (kind[u] == 1 ? p.k : p.v) + (long long)head[u] * D;
+    ts[u] = kind[u] == 0 ? p.q_ts : kind[u] == 1 ? p.k_ts : p.v_ts;
+    src[u] += t0 * ts[u] + c0;
+    next[u] = *(const u32x4*)src[u];
+  }
   // Where token t's rows go.  A row of padding, or an index outside its range: nowhere.
   if (tid < nt) {
     const int t = t0 + tid, s = p.seq ? p.seq[t] : t, at = p.at[t];
@@ -147,76 +135,76 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, Pr
     const int t = i / half, pair = i - t * half;
     const int x = p.pos[(size_t)axis_of(p.rope, pair) * p.T + t0 + t];
     const size_t e = (size_t)min(max(x, 0), p.rope.max_pos - 1) * p.rope.rot + pair;
-    s_cos[t * half + pair] = p.rope.cos_t[e];
-    s_sin[t * half + pair] = p.rope.sin_t[e];
+    const float sn = p.rope.sin_t[e];
+    s_cos[i] = p.rope.cos_t[e];
+    s_sin[0][i] = -sn;
+    s_sin[1][i] = sn;
   }
-  f32x4 qw[2], kw[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const f32x4 one = {1.0f, 1.0f, 1.0f, 1.0f};
-    qw[i] = p.q_norm_w ? one + *(const f32x4*)(p.q_norm_w + c0 + 4 * i) : one;
-    kw[i] = p.k_norm_w ? one + *(const f32x4*)(p.k_norm_w + c0 + 4 * i) : one;
+  if (tid < D) {
+    s_w[0][tid] = p.q_norm_w ? 1.0f + p.q_norm_w[tid] : 1.0f;
+    s_w[1][tid] = p.k_norm_w ? 1.0f + p.k_norm_w[tid] : 1.0f;
   }
   __syncthreads();
 
   const int lane = tid & 63, dl = half / 8;    // rot % 16 == 0: a pair's two halves are whole lanes apart
   const bool lower = c0 < half, turned = c0 < 2 * half;
   const int from = 4 * (lower ? lane + dl : turned ? lane - dl : lane);
-  for (int j0 = mine; j0 - mine + first < total; j0 += R * RPB) {
+  for (int t = 0; t < nt; ++t) {
     u32x4 raw[R];
 #pragma unroll
-    for (int u = 0; u < R; ++u) raw[u] = x0[u];
-    if (j0 - mine + first + R * RPB < total) fetch(j0 + R * RPB);
+    for (int u = 0; u < R; ++u) {
+      raw[u] = next[u];
+      if (t + 1 < nt) next[u] = *(const u32x4*)(src[u] + (t + 1) * ts[u]);
+    }
+    const long long base = s_row[t];
+    if (base < 0) continue;
 #pragma unroll
     for (int u = 0; u < R; ++u) {
-      const int j = j0 + u * RPB;
-      if (j - mine + first >= total) break;    // the same for the whole workgroup
-      const Row r = row_of(min(j, total - 1));
-      const long long base = j < total ? s_row[r.t] : -1;
       float x[8];
       unpack8(x, raw[u]);
-      if (r.kind == 0 ? p.q_norm_w != nullptr : r.kind == 1 && p.k_norm_w) {
+      if (kind[u] == 0 ? p.q_norm_w != nullptr : kind[u] == 1 && p.k_norm_w) {
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
         const float rs = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * (r.kind == 0 ? qw[i / 4][i % 4] : kw[i / 4][i % 4]);
+        for (int i = 0; i < 8; i += 4) {
+          const f32x4 w = *(const f32x4*)(s_w[kind[u]] + c0 + i);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[i + k] = x[i + k] * rs * w[k];
+        }
       }
-      if (half > 0 && __any(r.kind < 2)) {
+      if (half > 0 && __any(kind[u] < 2)) {
         // every lane of the wave takes part: its rows may be of different kinds
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           y[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[i])));
-        if (r.kind < 2 && turned) {
-          const int e = r.t * half + (lower ? c0 : c0 - half);
+        if (kind[u] < 2 && turned) {
+          const int e = t * half + (lower ? c0 : c0 - half);
 #pragma unroll
           for (int i = 0; i < 8; i += 4) {
-            const f32x4 cs = *(const f32x4*)(s_cos + e + i);
-            f32x4 sn = *(const f32x4*)(s_sin + e + i);
-            if (lower) sn = -sn;
+            const f32x4 cs = *(const f32x4*)(s_cos + e + i), sn = *(const f32x4*)(s_sin[lower ? 0 : 1] + e + i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[i + k] = x[i + k] * cs[k] + y[i + k] * sn[k];
           }
         }
       }
-      if (r.kind == 0) {
-        const size_t o = ((size_t)(t0 + r.t) * p.n_heads + r.head) * D + c0;
-        if (base >= 0) {
-          if (p.q_f32) {
-            *(f32x4*)((float*)p.q_out + o) = f32x4{x[0], x[1], x[2], x[3]};
-            *(f32x4*)((float*)p.q_out + o + 4) = f32x4{x[4], x[5], x[6], x[7]};
-          } else {
-            *(u32x4*)((uint16_t*)p.q_out + o) = pack8(x);
-          }
+      if (kind[u] == 0) {
+        const size_t o = ((size_t)(t0 + t) * p.n_heads + head[u]) * D + c0;
+        if (p.q_f32) {
+          *(f32x4*)((float*)p.q_out + o) = f32x4{x[0], x[1], x[2], x[3]};
+          *(f32x4*)((float*)p.q_out + o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        } else {
+          *(u32x4*)((uint16_t*)p.q_out + o) = pack8(x);
         }
         continue;
       }
-      void* dst = r.kind == 1 ? p.c.k : p.c.v;
-      const long long row = base + (long long)r.head * p.c.page_size;
+      if (kind[u] == 3) continue;
+      void* dst = kind[u] == 1 ? p.c.k : p.c.v;
+      const long long row = base + (long long)head[u] * p.c.page_size;
       if (!p.c.ks) {
-        if (base >= 0) *(u32x4*)((uint16_t*)dst + row * D + c0) = pack8(x);
+        *(u32x4*)((uint16_t*)dst + row * D + c0) = pack8(x);
         continue;
       }
       float a = 0.0f;
@@ -232,12 +220,12 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, Pr
         }
         a = row_max<LPR>(a);
       }
-      const float s = fmaxf(a / 448.0f, kMinScale), rs = 1.0f / s;
-      const u32x2 w = {e4m3x4(x[0], x[1], x[2], x[3], s, rs), e4m3x4(x[4], x[5], x[6], x[7], s, rs)};
-      if (base >= 0) {
-        if (ln == 0) (r.kind == 1 ? p.c.ks : p.c.vs)[row] = s;
-        *(u32x2*)((uint8_t*)dst + row * D + c0) = w;
-      }
+      const float s0 = a * (1.0f / 448.0f);    // a / 448, with its residual's correction
+      const float s = fmaxf(fmaf(fmaf(-s0, 448.0f, a), 1.0f / 448.0f, s0), kMinScale);
+      const float r0 = __builtin_amdgcn_rcpf(s), rs = fmaf(fmaf(-s, r0, 1.0f), r0, r0);
+      if (ln == 0) (kind[u] == 1 ? p.c.ks : p.c.vs)[row] = s;
+      *(u32x2*)((uint8_t*)dst + row * D + c0) =
+          u32x2{e4m3x4(x[0], x[1], x[2], x[3], s, rs), e4m3x4(x[4], x[5], x[6], x[7], s, rs)};
     }
   }
 }
@@ -404,19 +392,25 @@ int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
       return -1;
     }
   }
-  const int rows = (p.q ? p.n_heads : 0) + 2 * p.c.n_kv, pass = 256 / (D / 8);
-  PrepPlan pl;
-  pl.rows = rows;
-  // A row a thread while that leaves no more than some four workgroups a CU; then
-  // workgroups of several tokens that still fill the CUs four times.
-  const bool few = (long long)p.T * ((rows + pass - 1) / pass) <= 1024;
-  pl.tokens = few ? 1 : std::min(kPrepTokens, std::max(1, p.T / 1024));
-  pl.span = few ? pass : pl.tokens * rows;
-  pl.rows_mul = (uint32_t)((1ull << 32) / rows + 1);
-  const dim3 grid((p.T + pl.tokens - 1) / pl.tokens, few ? (rows + pass - 1) / pass : 1);
-  auto fn = D == 256 ? (few ? paged_prep_kernel<256, 1> : paged_prep_kernel<256, 4>)
-                     : (few ? paged_prep_kernel<128, 1> : paged_prep_kernel<128, 4>);
-  hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, p, pl);
+  const int rows = (p.q ? p.n_heads : 0) + 2 * p.c.n_kv, pass = 256 / (D / 8), passes = (rows + pass - 1) / pass;
+  // A head a thread while that leaves no more than some four workgroups a CU; then up to 4
+  // of them, and workgroups of up to 4 tokens that still fill the CUs three times (3700
+  // tokens: 38 us with one, 33 with 2 or 4, 37 with 8).
+  int tokens = 1, groups = passes;
+  if ((long long)p.T * passes > 1024) {
+    groups = (passes + 3) / 4;
+    tokens = (int)std::min<long long>(kPrepTokens, std::max<long long>(1, (long long)p.T * groups / 768));
+  }
+  const dim3 grid((p.T + tokens - 1) / tokens, groups);
+  const int R = (passes + groups - 1) / groups;
+  void (*fn)(QhPagedPrepParams, int);
+  if (D == 256)
+    fn = R == 1 ? paged_prep_kernel<256, 1> : R == 2 ? paged_prep_kernel<256, 2>
+         : R == 3 ? paged_prep_kernel<256, 3> : paged_prep_kernel<256, 4>;
+  else
+    fn = R == 1 ? paged_prep_kernel<128, 1> : R == 2 ? paged_prep_kernel<128, 2>
+         : R == 3 ? paged_prep_kernel<128, 3> : paged_prep_kernel<128, 4>;
+  hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, p, tokens);
   return 0;
 }
 

@@ -22,8 +22,16 @@ import torch
 from . import abi
 
 FP8 = torch.float8_e4m3fn
-_INT = torch.int32
-_BF = torch.bfloat16
+_INT, _BF, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
+_NO_STRIDE = (0, 0, 1)
+_current_device = torch.cuda.current_device
+
+
+def _raw_stream(dev):
+    """hipStream_t of the current torch stream of GPU `dev`: torch.cuda.current_stream(dev).cuda_stream
+    without the Stream object."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
 
 
 def _need(t, name, dtype, shape, dev, contiguous=True):
@@ -82,12 +90,13 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv, self.page_size, self.head_dim = k.shape
         self.dev, self.device = dev, k.device
-        self.lib = abi.load()
         self._desc = abi.PagedCacheDesc(k.data_ptr(), v.data_ptr(),
                                         k_scale.data_ptr() if self.fp8 else None,
                                         v_scale.data_ptr() if self.fp8 else None,
                                         self.n_pages, self.page_size, self.n_kv, self.head_dim, int(self.fp8))
         self._ref = ctypes.addressof(self._desc)
+        lib = abi.load()
+        self._prep, self._read, self._attend = lib.qh_attn_prep_paged, lib.qh_kv_read_paged, lib.qh_attn_decode_paged
 
     @classmethod
     def alloc(cls, n_pages, page_size, n_kv, head_dim, dtype=_BF, device="cuda"):
@@ -100,21 +109,16 @@ class PagedKVCache:
 
     def _call(self, what, fn, *args):
         """Launch on the current stream of the cache's device."""
-        if torch.cuda.current_device() == self.dev:
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        if _current_device() == self.dev:
+            rc = fn(*args, _raw_stream(self.dev))
         else:
             with torch.cuda.device(self.dev):
-                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+                rc = fn(*args, _raw_stream(self.dev))
         if rc != 0:
             abi.check(rc, what)
 
-    def _heads(self, t, name, n, heads):
-        """Strides (first, second) of a bf16 [n, heads, head_dim] view whose last axis is dense."""
-        _need(t, name, _BF, (n, heads, self.head_dim), self.dev, contiguous=False)
-        a, b, c = t.stride()
-        if c != 1:
-            raise ValueError(f"{name}: the last axis must be contiguous")
-        return a, b
+    # Each call checks its tensors in one expression, which costs a decode step's host a
+    # few microseconds; only where it fails are they gone through one by one, for the message.
 
     def prep(self, k, v, pages, at, seq=None, q=None, q_out=None, rope=None, pos=None, q_norm=None, k_norm=None,
              eps=1e-6):
@@ -126,12 +130,61 @@ class PagedKVCache:
         default) or fp32 (what qh_attn_prefill takes).  rope: RopeAxes with pos int32
         [axes, T] (or [T] for one axis).  A token with an index out of range (padding:
         -1) is left out altogether.  Returns q_out."""
-        D, dev = self.head_dim, self.dev
-        T = k.shape[0]
-        ks, kh = self._heads(k, "k", T, self.n_kv)
-        vs, vh = self._heads(v, "v", T, self.n_kv)
-        if T > 0 and self.n_kv > 1 and (kh != D or vh != D):
-            raise ValueError("k, v: a token's heads must be contiguous")
+        dev, D, n_kv = self.dev, self.head_dim, self.n_kv
+        T = len(k)
+        H = 0
+        shape, row = (T, n_kv, D), (T,)
+        ks, vs, pn = k.stride(), v.stride(), pages.shape
+        good = (k.dtype is _BF and v.dtype is _BF and pages.dtype is _INT and at.dtype is _INT
+                and k.get_device() == dev and v.get_device() == dev and pages.get_device() == dev
+                and at.get_device() == dev and k.shape == shape and v.shape == shape and at.shape == row
+                and len(pn) == 2 and pages.is_contiguous() and at.is_contiguous()
+                and ks[2] == 1 and vs[2] == 1 and (n_kv == 1 or ks[1] == D and vs[1] == D))
+        p_seq = p_q = p_out = p_rope = p_pos = p_qn = p_kn = None
+        f32 = qs = qh = 0
+        if good and seq is not None:
+            good = seq.dtype is _INT and seq.get_device() == dev and seq.shape == row and seq.is_contiguous()
+            p_seq = seq.data_ptr()
+        if good and rope is not None:
+            good = (pos is not None and pos.dtype is _INT and pos.get_device() == dev and rope.dev == dev
+                    and (pos.shape == (rope.n_axes, T) or rope.n_axes == 1 and pos.shape == row)
+                    and pos.is_contiguous())
+            p_rope, p_pos = rope._ref, pos.data_ptr() if good else None
+        if good and q_norm is not None:
+            good = (q_norm.dtype is _F32 and q_norm.get_device() == dev and q_norm.shape == (D,)
+                    and q_norm.is_contiguous())
+            p_qn = q_norm.data_ptr()
+        if good and k_norm is not None:
+            good = (k_norm.dtype is _F32 and k_norm.get_device() == dev and k_norm.shape == (D,)
+                    and k_norm.is_contiguous())
+            p_kn = k_norm.data_ptr()
+        if good and q is not None:
+            n = q.shape
+            good = q.dtype is _BF and q.get_device() == dev and len(n) == 3 and n[0] == T and n[2] == D
+            if good:
+                H = n[1]
+                qs, qh, last = q.stride()
+                if q_out is None:
+                    q_out = torch.empty(T, H, D, dtype=_BF, device=self.device)
+                f32 = q_out.dtype is _F32
+                good = (last == 1 and (f32 or q_out.dtype is _BF) and q_out.get_device() == dev and q_out.shape == n
+                        and q_out.is_contiguous())
+                p_q, p_out = q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            good = False
+        if not good:
+            self._refuse_prep(k, v, pages, at, seq, q, q_out, rope, pos, q_norm, k_norm)
+        self._call("attn_prep_paged", self._prep, self._ref, p_rope, p_q, qs, qh, k.data_ptr(), ks[0], v.data_ptr(),
+                   vs[0], p_qn, p_kn, eps, p_pos, p_seq, at.data_ptr(), T, pages.data_ptr(), pn[0], pn[1], p_out, f32, H)
+        return q_out
+
+    def _refuse_prep(self, k, v, pages, at, seq, q, q_out, rope, pos, q_norm, k_norm):
+        """Raise for the first argument of `prep` that it does not take."""
+        D, dev, T = self.head_dim, self.dev, len(k)
+        for t, name in ((k, "k"), (v, "v")):
+            self._need_heads(t, name, T, self.n_kv)
+            if self.n_kv > 1 and t.stride(1) != D:
+                raise ValueError(f"{name}: a token's heads must be contiguous")
         _need(pages, "pages", _INT, (None, None), dev)
         _need(at, "at", _INT, (T,), dev)
         if seq is not None:
@@ -144,36 +197,39 @@ class PagedKVCache:
             _need(pos, "pos", _INT, (T,) if pos.dim() == 1 and rope.n_axes == 1 else (rope.n_axes, T), dev)
         for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
             if w is not None:
-                _need(w, name, torch.float32, (D,), dev)
-        H = qs = qh = 0
-        if q is not None:
-            H = q.shape[1]
-            qs, qh = self._heads(q, "q", T, H)
-            if q_out is None:
-                q_out = torch.empty(T, H, D, dtype=_BF, device=self.device)
-            elif q_out.dtype not in (_BF, torch.float32):
-                raise TypeError("q_out: bf16 or fp32")
-            _need(q_out, "q_out", q_out.dtype, (T, H, D), dev)
-        elif q_out is not None:
+                _need(w, name, _F32, (D,), dev)
+        if q is None:
             raise ValueError("q_out: there is no q")
-        self._call("attn_prep_paged", self.lib.qh_attn_prep_paged, self._ref, None if rope is None else rope._ref,
-                   None if q is None else q.data_ptr(), qs, qh, k.data_ptr(), ks, v.data_ptr(), vs,
-                   None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-                   None if pos is None else pos.data_ptr(), None if seq is None else seq.data_ptr(), at.data_ptr(), T,
-                   pages.data_ptr(), pages.shape[0], pages.shape[1], None if q is None else q_out.data_ptr(),
-                   int(q is not None and q_out.dtype == torch.float32), H)
-        return q_out
+        self._need_heads(q, "q", T, None)
+        if q_out.dtype not in (_BF, _F32):
+            raise TypeError("q_out: bf16 or fp32")
+        _need(q_out, "q_out", q_out.dtype, tuple(q.shape), dev)
+        raise ValueError("prep: arguments that do not fit together")
+
+    def _need_heads(self, t, name, n, heads):
+        """Raise unless t is a bf16 [n, heads, head_dim] view whose last axis is dense."""
+        _need(t, name, _BF, (n, heads, self.head_dim), self.dev, contiguous=False)
+        if t.stride(2) != 1:
+            raise ValueError(f"{name}: the last axis must be contiguous")
 
     def read(self, pages, last, k_out, v_out):
         """Positions 0 .. last[b] (int32 [B]) of each sequence to k_out, v_out bf16
         [B, n_kv, max_seq, D]; rows behind them keep what they hold."""
-        _need(pages, "pages", _INT, (None, None), self.dev)
-        B = pages.shape[0]
-        _need(last, "last", _INT, (B,), self.dev)
-        _need(k_out, "k_out", _BF, (B, self.n_kv, None, self.head_dim), self.dev)
-        _need(v_out, "v_out", _BF, tuple(k_out.shape), self.dev)
-        self._call("kv_read_paged", self.lib.qh_kv_read_paged, self._ref, pages.data_ptr(), B, pages.shape[1],
-                   last.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), k_out.shape[2])
+        dev, pn, n = self.dev, pages.shape, k_out.shape
+        if not (pages.dtype is _INT and last.dtype is _INT and k_out.dtype is _BF and v_out.dtype is _BF
+                and pages.get_device() == dev and last.get_device() == dev and k_out.get_device() == dev
+                and v_out.get_device() == dev and len(pn) == 2 and last.shape == pn[:1] and len(n) == 4
+                and n[0] == pn[0] and n[1] == self.n_kv and n[3] == self.head_dim and v_out.shape == n
+                and pages.is_contiguous() and last.is_contiguous() and k_out.is_contiguous()
+                and v_out.is_contiguous()):
+            B = pn[0]
+            _need(pages, "pages", _INT, (None, None), dev)
+            _need(last, "last", _INT, (B,), dev)
+            _need(k_out, "k_out", _BF, (B, self.n_kv, None, self.head_dim), dev)
+            _need(v_out, "v_out", _BF, tuple(n), dev)
+            raise ValueError("read: arguments that do not fit together")
+        self._call("kv_read_paged", self._read, self._ref, pages.data_ptr(), pn[0], pn[1], last.data_ptr(),
+                   k_out.data_ptr(), v_out.data_ptr(), n[2])
 
     def attend(self, q, pages, last, ws, gate=None, out=None):
         """out[b, h] = softmax(q[b, h] . K^T / sqrt(D)) V over positions 0 .. last[b]
@@ -181,21 +237,35 @@ class PagedKVCache:
         empty sequence (last[b] < 0).  q, gate: bf16 [B, n_heads, D], any strides, q as
         `prep` wrote it; ws: ``attn_workspace`` (calls that share one must not overlap).
         Returns out, bf16 [B, n_heads, D]."""
-        B, H = q.shape[0], q.shape[1]
-        qs, qh = self._heads(q, "q", B, H)
-        gs = gh = 0
-        if gate is not None:
-            gs, gh = self._heads(gate, "gate", B, H)
-        _need(pages, "pages", _INT, (B, None), self.dev)
-        _need(last, "last", _INT, (B,), self.dev)
-        _need(ws, "ws", torch.uint8, (None,), self.dev)
+        dev, n, pn = self.dev, q.shape, pages.shape
+        qs = q.stride()
+        good = (q.dtype is _BF and pages.dtype is _INT and last.dtype is _INT and ws.dtype is _U8
+                and q.get_device() == dev and pages.get_device() == dev and last.get_device() == dev
+                and ws.get_device() == dev and len(n) == 3 and n[2] == self.head_dim and len(pn) == 2
+                and pn[0] == n[0] and last.shape == n[:1] and qs[2] == 1
+                and pages.is_contiguous() and last.is_contiguous() and ws.is_contiguous())
+        p_gate, gs = None, _NO_STRIDE
+        if good and gate is not None:
+            gs = gate.stride()
+            good = gate.dtype is _BF and gate.get_device() == dev and gate.shape == n and gs[2] == 1
+            p_gate = gate.data_ptr()
+        if good and out is not None:
+            good = out.dtype is _BF and out.get_device() == dev and out.shape == n and out.is_contiguous()
+        if not good:
+            B, H = (n[0], n[1]) if len(n) == 3 else (None, None)
+            self._need_heads(q, "q", B, None)
+            if gate is not None:
+                self._need_heads(gate, "gate", B, H)
+            _need(pages, "pages", _INT, (B, None), dev)
+            _need(last, "last", _INT, (B,), dev)
+            _need(ws, "ws", _U8, (None,), dev)
+            if out is not None:
+                _need(out, "out", _BF, tuple(n), dev)
+            raise ValueError("attend: arguments that do not fit together")
         if out is None:
-            out = torch.empty(B, H, self.head_dim, dtype=_BF, device=self.device)
-        else:
-            _need(out, "out", _BF, (B, H, self.head_dim), self.dev)
-        self._call("attn_decode_paged", self.lib.qh_attn_decode_paged, self._ref, q.data_ptr(), qs, qh,
-                   None if gate is None else gate.data_ptr(), gs, gh, pages.data_ptr(), B, pages.shape[1],
-                   last.data_ptr(), H, out.data_ptr(), ws.data_ptr(), ws.numel())
+            out = torch.empty(n, dtype=_BF, device=self.device)
+        self._call("attn_decode_paged", self._attend, self._ref, q.data_ptr(), qs[0], qs[1], p_gate, gs[0], gs[1],
+                   pages.data_ptr(), n[0], pn[1], last.data_ptr(), n[1], out.data_ptr(), ws.data_ptr(), ws.numel())
         return out
 
 

@@ -314,6 +314,17 @@ def test_wrapper_refusals():
         cache.read(pages, at, z(3, 3, 32, 128), z(3, 3, 32, 128))
 
 
+def test_nothing_to_write_read_or_attend_to():
+    cache = paged.PagedKVCache.alloc(4, 16, 2, 128)
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=DEV)   # noqa: E731
+    i32 = torch.int32
+    out = cache.prep(z(0, 2, 128), z(0, 2, 128), z(2, 3, dtype=i32), z(0, dtype=i32), q=z(0, 4, 128))
+    assert out.shape == (0, 4, 128) and out.dtype == torch.bfloat16
+    cache.read(z(0, 3, dtype=i32), z(0, dtype=i32), z(0, 2, 8, 128), z(0, 2, 8, 128))
+    assert cache.attend(z(0, 4, 128), z(0, 3, dtype=i32), z(0, dtype=i32), paged.attn_workspace(4, 2, 128)).shape == (0, 4, 128)
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------ read
 @pytest.mark.parametrize("lens,kv,D,page,fp8,max_seq", [
     ([1], 4, 256, 16, True, 1),
