@@ -56,15 +56,6 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ uint32_t widen_lo(uint32_t x) { return __builtin_bit_cast(uint32_t, e4m3x2_lo_bf16(x)); }
 __device__ __forceinline__ uint32_t widen_hi(uint32_t x) { return __builtin_bit_cast(uint32_t, e4m3x2_hi_bf16(x)); }
 
-// Sixteen bytes that another workgroup published (device-coherent): two 8-byte atomic
-// loads, which the compiler keeps independent of each other.
-__device__ __forceinline__ u32x4 coherent_load(const float* src) {
-  uint64_t* s = (uint64_t*)const_cast<float*>(src);
-  const uint64_t a = __hip_atomic_load(s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const uint64_t b = __hip_atomic_load(s + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
-}
-
 // 2^x as the hardware has it (1 ulp; results below 2^-126 are zero).
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -425,6 +416,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     Place nx = A;
     Ids ni = ai;
     load_k(C, ci);
+    if (C.k < k1 && C.u0 != A.u0) load_q(C);  // the next pair's: this one's scores are done
     nx = C;
     ni = ci;
     ++C.k;
@@ -503,6 +495,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   };
 
   const int rec = rec_floats(G, D);
+  // device-coherent (sc1) accesses: pieces pass between workgroups whose L2 caches are not coherent
+  const auto parts = __builtin_amdgcn_make_buffer_rsrc(p.part, (short)0, 2 * kMaxWG * rec * 4, 0x00020000);
   auto gate_of = [&](int b, int head, int c) {
     return p.gate ? *(const u32x2*)(p.gate + b * p.g_bs + (long long)head * p.g_hs + c) : u32x2{0u, 0u};
   };
@@ -534,10 +528,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         const int rr = i / (DT / 4), d = i % (DT / 4) * 4;
         dst[i * 4 * G] = f32x4{o[d][rr], o[d + 1][rr], o[d + 2][rr], o[d + 3][rr]};
       }
-      if (g == 0) {
-        slot_of(s)[G * D + r] = m;
-        slot_of(s)[G * D + kMaxG + r] = l;
-      }
+      if (g == 0) *(float2*)(slot_of(s) + G * D + 2 * r) = float2{m, l};
     }
   };
   // ---- this wave's pairs, one after the other -------------------------------------------
@@ -545,10 +536,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   if (k0 < k1) {
     while (true) {
       const int s1 = min(at.u1, k1);
-      // q is waited for here: where it may be under way in any step, each score would wait
-      // for it, and so for all that was asked for after it
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk]));
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       m = -INFINITY;
@@ -558,10 +545,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       l += __shfl_xor(l, 32, 64);
       const Place done = at;
       const bool more = s1 < k1, begun = done.u0 < k0;
-      if (more) {
-        at = A;
-        load_q(at);
-      }
+      if (more) at = A;
       put_slot(2 * wid + (begun ? 0 : 1));
       if (!begun && done.u1 <= k1) {                 // all of it is here
         const float* src = slot_of(2 * wid + 1);
@@ -577,7 +561,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
             const int i = i0 + 64 * u;
             if (i >= items) break;
             const Item it = item(i);
-            emit(done.b, done.kvh * G + it.h, it.c, ((const f32x4*)src)[i], src[G * D + kMaxG + it.h], gt[u]);
+            emit(done.b, done.kvh * G + it.h, it.c, ((const f32x4*)src)[i], src[G * D + 2 * it.h + 1], gt[u]);
           }
         }
       }
@@ -603,8 +587,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       const bool begun = c.u0 < start, all = !begun && c.u1 <= end;
       const int w = begun ? 0 : (c.u0 - start) / ws, last = (min(c.u1, end) - 1 - start) / ws;
       if (!all || last > w) {
-        float* dst = p.part + (size_t)(2 * wg + (c.u0 > start ? 1 : 0)) * rec;
-        const auto rs = __builtin_amdgcn_make_buffer_rsrc(dst, (short)0, rec * 4, 0x00020000);
+        const int dst = (2 * wg + (c.u0 > start ? 1 : 0)) * rec * 4;  // bytes from the first record
         for (int i = tid; i < items; i += kThreads) {
           const Item it = item(i);
           const int head = c.kvh * G + it.h;
@@ -618,17 +601,18 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
             const int x = min(w + u, last);
             const float* src = slot_of(2 * x + (x == w && !begun ? 1 : 0));
             y[u] = in ? ((const f32x4*)src)[i] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            my[u] = in ? src[G * D + it.h] : -INFINITY;
-            ly[u] = in ? src[G * D + kMaxG + it.h] : 0.0f;
+            const float2 ml = *(const float2*)(src + G * D + 2 * it.h);
+            my[u] = in ? ml.x : -INFINITY;
+            ly[u] = in ? ml.y : 0.0f;
           }
           add_parts(a, M, L, y, my, ly);
           if (all) {
             emit(c.b, head, it.c, a, L, gt);
           } else {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), rs, i * 16, 0, 16);
-            if (i < 4 * G && i / G == 0) {
-              pub_store(dst + G * D + it.h, M);
-              pub_store(dst + G * D + kMaxG + it.h, L);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), parts, dst + i * 16, 0, 16);
+            if (i < G) {                             // items 0 .. G - 1: one of each head
+              const u32x2 ml = {__float_as_uint(M), __float_as_uint(L)};
+              __builtin_amdgcn_raw_buffer_store_b64(ml, parts, dst + (G * D + 2 * it.h) * 4, 0, 16);
             }
           }
         }
@@ -662,7 +646,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   for (int which = 0; which < 2; ++which) {
     if (!s_last[which]) continue;
     const Pair x = which == 0 ? open0 : open1;
-    auto rec_of = [&](int j) { return p.part + (size_t)(2 * (x.first + j) + (j == 0 ? x.tail : 0)) * rec; };
+    auto rec_of = [&](int j) { return (2 * (x.first + j) + (j == 0 ? x.tail : 0)) * rec * 4; };
     // a thread takes an item, of every subs-th piece where there are threads enough for that
     const int subs = items < kThreads ? min(kThreads / items, x.pieces) : 1;
     f32x4* s_a = (f32x4*)s_o;                        // [kThreads]
@@ -686,10 +670,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
             my[u] = -INFINITY;
             ly[u] = 0.0f;
             if (j + u * subs < x.pieces) {
-              const float* src = rec_of(j + u * subs);
-              y[u] = __builtin_bit_cast(f32x4, coherent_load(src + 4 * i));
-              my[u] = pub_load(src + G * D + it.h);
-              ly[u] = pub_load(src + G * D + kMaxG + it.h);
+              const int src = rec_of(j + u * subs);
+              y[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, src + i * 16, 0, 16));
+              const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(parts, src + (G * D + 2 * it.h) * 4, 0, 16);
+              my[u] = __uint_as_float(ml.x);
+              ly[u] = __uint_as_float(ml.y);
             }
           }
           add_parts(a, M, L, y, my, ly);
