@@ -1016,7 +1016,7 @@ QH_EXPORT int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, l
                  kPagedMaxUnits);
     return -1;
   }
-  if ((long long)n_seqs * p.c.n_kv * ((p.c.capacity + 31LL) / 32) > 0x7FFF0000LL) {
+  if ((long long)n_seqs * p.c.n_kv * ((p.c.capacity + 31LL) / 32 + 1) > 0x7FFF0000LL) {
     qh_set_error("%s: %d sequences of %d KV heads with tables of %d positions are more than 2^31 tiles of 32", what,
                  n_seqs, p.c.n_kv, p.c.capacity);
     return -1;
