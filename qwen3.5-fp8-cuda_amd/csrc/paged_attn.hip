@@ -34,6 +34,8 @@
 // leaves a partial record a piece (maximum, sum, outputs) in the workspace, and the last
 // piece to arrive joins them.  All joins go in the order of the pieces: the result does
 // not depend on who comes last.
+#include <type_traits>
+
 #include "qh_common.h"
 #include "qh_paged.h"
 
@@ -205,7 +207,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       if (length(b) == 0) zeros(b);
     total = sum * Hkv;
     if (most <= kWhole && B <= slots) share = kWhole;
-    else if (4 * B <= slots) share = max(kWaves, (sum + slots - B - 1) / (slots - B));
+    else if (4 * B <= slots) {
+      // equal shares would do if none of them were cut short; that costs a piece a sequence at most
+      share = max(4, (sum + slots - 1) / slots);
+      if (__builtin_amdgcn_readlane(wave_scan((tl + share - 1) / share), 63) > slots)
+        share = max(4, (sum + slots - B - 1) / (slots - B));
+    }
     if (share > 0) {
       const int pc = (tl + share - 1) / share, cum = wave_scan(pc);
       const unsigned long long past = __ballot(cum * Hkv > wg);
@@ -674,25 +681,30 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       u32x2 gt = {0u, 0u};
       if (i < items && sub < subs) {
         gt = gate_of(x.b, head, it.c);
-        constexpr int U = 16;
-        for (int j = sub; j < x.pieces; j += U * subs) {
-          f32x4 y[U];
-          float my[U], ly[U];
+        // 16 pieces under way together, 4 where there are few (the code of 16 alone takes 0.6 us)
+        auto read = [&](auto n) {
+          constexpr int U = decltype(n)::value;
+          for (int j = sub; j < x.pieces; j += U * subs) {
+            f32x4 y[U];
+            float my[U], ly[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            my[u] = -INFINITY;
-            ly[u] = 0.0f;
-            if (j + u * subs < x.pieces) {
-              const int src = rec_of(j + u * subs);
-              y[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, src + i * 16, 0, 16));
-              const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(parts, src + (G * D + 2 * it.h) * 4, 0, 16);
-              my[u] = __uint_as_float(ml.x);
-              ly[u] = __uint_as_float(ml.y);
+            for (int u = 0; u < U; ++u) {
+              y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+              my[u] = -INFINITY;
+              ly[u] = 0.0f;
+              if (j + u * subs < x.pieces) {
+                const int src = rec_of(j + u * subs);
+                y[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, src + i * 16, 0, 16));
+                const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(parts, src + (G * D + 2 * it.h) * 4, 0, 16);
+                my[u] = __uint_as_float(ml.x);
+                ly[u] = __uint_as_float(ml.y);
+              }
             }
+            add_parts(a, M, L, y, my, ly);
           }
-          add_parts(a, M, L, y, my, ly);
-        }
+        };
+        if (x.pieces <= 8) read(std::integral_constant<int, 4>{});
+        else read(std::integral_constant<int, 16>{});
       }
       if (subs > 1) {
         s_a[tid] = a;
