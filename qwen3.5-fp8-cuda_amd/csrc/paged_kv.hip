@@ -8,12 +8,16 @@
 //   y_i   = n_i cos - n_{i+h} sin,  y_{i+h} = n_{i+h} cos + n_i sin,   i < h = rot/2,
 //           at the angle of column i and the position on pair i's axis
 //   q     : y in bf16 or fp32;   K, V : y to slot (page, head, at % page_size),
-//           as bf16, or as E4M3 codes e4m3(y / s) with s = max(amax / 448, 2^-100),
+//           as bf16, or as E4M3 codes e4m3(448 y / amax) with the scale amax / 448,
 //           amax over the row's finite values (E4M3 has no infinity: a value that is
-//           not finite is stored as NaN and leaves the rest of its row as it is)
-// All in fp32 with one rounding at the end: the intermediate bf16 roundings of the
-// dense path (which the reference's tensors have) would be rounded again to three
+//           not finite is stored as NaN and leaves the rest of its row as it is); where
+//           amax / 448 is below 2^-100 the scale is that, and the codes e4m3(y 2^100)
+// q and bf16 rows in fp32 with one rounding at the end: the intermediate bf16 roundings
+// of the dense path (which the reference's tensors have) would be rounded again to three
 // mantissa bits here, and a second rounding moves a value in 16 to another code.
+// E4M3 codes are those of the exact quotient: V's is one of bf16 numbers, rounded to
+// fp32 correctly, which keeps the ties between two codes that such quotients often are;
+// K's, in which the factor rsqrt(..) cancels, is computed in 64 bits (as fast as 32 here).
 #include <algorithm>
 
 #include "qh_common.h"
@@ -73,16 +77,63 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 
 constexpr int kPrepTokens = 4;  // tokens of a workgroup, at most
 
-// E4M3 codes of 4 values: v / s with rs close to 1 / s, corrected by the quotient's
-// residual: a tie between two codes, common for bf16 values, is the tie that the exact
-// division has.
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float s, float rs) {
-  auto div = [&](float v) {
-    const float q = v * rs;
-    return copysignf(fmaf(fmaf(-q, s, v), rs, q), v);  // of -0 the correction makes +0
-  };
-  uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(div(a), div(b), 0, false);
-  return __builtin_amdgcn_cvt_pk_fp8_f32(div(c), div(d), w, true);
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// row_max of 64-bit values.
+template <int LPR>
+__device__ __forceinline__ double row_max(double v) {
+  v = fmax(v, dpp_f64<0xB1>(v));
+  v = fmax(v, dpp_f64<0x4E>(v));
+  v = fmax(v, dpp_f64<0x141>(v));
+  v = fmax(v, dpp_f64<0x140>(v));
+  if constexpr (LPR == 32) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    v = fmax(__builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]),
+             __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]));
+  }
+  return v;
+}
+
+// A row's 8 values of this lane as codes, and its scale (without the factor that cancels).
+// V: 448 x / amax as (x 7/8) / (amax 2^-9), both exact: the quotient by a reciprocal,
+// corrected by its residual.
+__device__ __forceinline__ u32x2 e4m3_row(const float (&x)[8], float amax, float& scale) {
+  const float s0 = amax * (1.0f / 448.0f);         // amax / 448, with its residual's correction
+  scale = fmaf(fmaf(-s0, 448.0f, amax), 1.0f / 448.0f, s0);
+  const bool tiny = scale < kMinScale;
+  if (tiny) scale = kMinScale;
+  const float num = tiny ? 1.0f : 0.875f, den = tiny ? kMinScale : amax * 0.001953125f;
+  const float r0 = __builtin_amdgcn_rcpf(den), r = fmaf(fmaf(-den, r0, 1.0f), r0, r0);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = x[i] * num, q0 = v * r;
+    q[i] = copysignf(fmaf(fmaf(-q0, den, v), r, q0), v);  // of -0 the correction makes +0
+  }
+  return u32x2{e4m3x4(q[0], q[1], q[2], q[3]), e4m3x4(q[4], q[5], q[6], q[7])};
+}
+// K: 64 bits; `factor` is what the values were not multiplied by (the norm's rsqrt, or 1).
+__device__ __forceinline__ u32x2 e4m3_row(const double (&x)[8], double amax, float factor, float& scale) {
+  const double s = amax * factor * (1.0 / 448.0);
+  const bool tiny = !(s >= (double)kMinScale);     // or a NaN: every value is one
+  scale = tiny ? kMinScale : (float)s;
+  const double r = tiny ? (double)factor / kMinScale : 448.0 / amax;
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = (float)(x[i] * r);
+  return u32x2{e4m3x4(q[0], q[1], q[2], q[3]), e4m3x4(q[4], q[5], q[6], q[7])};
 }
 
 // D / 8 lanes take a row, 16 bytes of input each.  A thread has the same R heads in each of
@@ -96,7 +147,7 @@ template <int D, int R>
 __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, int tokens) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a pass
   __shared__ __align__(16) float s_cos[kPrepTokens * D / 2], s_sin[2][kPrepTokens * D / 2];  // [0]: -sin
-  __shared__ __align__(16) float s_w[2][D];    // 1 + w of q and k
+  __shared__ __align__(16) float s_w[2][D];    // 1 + w of q and k (E4M3: w of k)
   __shared__ long long s_row[kPrepTokens];     // the token's slot in its page's first head, -1: left out
   const int tid = threadIdx.x, t0 = blockIdx.x * tokens, nt = min(tokens, p.T - t0);
   const int nq = p.q ? p.n_heads : 0, Hkv = p.c.n_kv, rows = nq + 2 * Hkv;
@@ -142,7 +193,8 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, in
   }
   if (tid < D) {
     s_w[0][tid] = p.q_norm_w ? 1.0f + p.q_norm_w[tid] : 1.0f;
-    s_w[1][tid] = p.k_norm_w ? 1.0f + p.k_norm_w[tid] : 1.0f;
+    const float w = p.k_norm_w ? p.k_norm_w[tid] : 0.0f;
+    s_w[1][tid] = p.c.ks ? w : 1.0f + w;       // E4M3: 1 + w in 64 bits, below
   }
   __syncthreads();
 
@@ -162,26 +214,32 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, in
     for (int u = 0; u < R; ++u) {
       float x[8];
       unpack8(x, raw[u]);
-      if (kind[u] == 0 ? p.q_norm_w != nullptr : kind[u] == 1 && p.k_norm_w) {
+      const bool normed = kind[u] == 0 ? p.q_norm_w != nullptr : kind[u] == 1 && p.k_norm_w;
+      const bool wide = kind[u] == 1 && p.c.ks;  // E4M3 rows of K: x stays as it is for now
+      float rs = 1.0f;
+      if (normed) {
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-        const float rs = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
+        rs = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
+        if (!wide) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          const f32x4 w = *(const f32x4*)(s_w[kind[u]] + c0 + i);
+          for (int i = 0; i < 8; i += 4) {
+            const f32x4 w = *(const f32x4*)(s_w[kind[u]] + c0 + i);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[i + k] = x[i + k] * rs * w[k];
+            for (int k = 0; k < 4; ++k) x[i + k] = x[i + k] * rs * w[k];
+          }
         }
       }
+      float y[8] = {};
+      const bool turn = half > 0 && kind[u] < 2 && turned;
+      const int e = turn ? t * half + (lower ? c0 : c0 - half) : 0;
       if (half > 0 && __any(kind[u] < 2)) {
         // every lane of the wave takes part: its rows may be of different kinds
-        float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           y[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[i])));
-        if (kind[u] < 2 && turned) {
-          const int e = t * half + (lower ? c0 : c0 - half);
+        if (turn && !wide) {
 #pragma unroll
           for (int i = 0; i < 8; i += 4) {
             const f32x4 cs = *(const f32x4*)(s_cos + e + i), sn = *(const f32x4*)(s_sin[lower ? 0 : 1] + e + i);
@@ -207,25 +265,54 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, in
         *(u32x4*)((uint16_t*)dst + row * D + c0) = pack8(x);
         continue;
       }
-      float a = 0.0f;
+      float scale;
+      u32x2 codes;
+      if (wide && (normed || half > 0)) {
+        double z[8];
+        const int other = turn ? (lower ? c0 + half : c0 - half) : c0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[i]));   // of a NaN and a number: the number
-      a = row_max<LPR>(a);
-      if (a == INFINITY) {                     // the scale is that of the finite values, an infinity a NaN
-        a = 0.0f;
+        for (int i = 0; i < 8; i += 4) {
+          const f32x4 w = *(const f32x4*)(s_w[1] + c0 + i), wo = *(const f32x4*)(s_w[1] + other + i);
+          const f32x4 cs = *(const f32x4*)(s_cos + e + i), sn = *(const f32x4*)(s_sin[lower ? 0 : 1] + e + i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = fabsf(x[i]) < INFINITY ? x[i] : NAN;
-          a = fmaxf(a, fabsf(x[i]));
+          for (int k = 0; k < 4; ++k) {
+            const double v = x[i + k] * (1.0 + w[k]);
+            z[i + k] = turn ? v * cs[k] + y[i + k] * (1.0 + wo[k]) * sn[k] : v;
+            if (!(rs < INFINITY)) z[i + k] = NAN;  // a NaN in the row: the norm is NaN
+          }
         }
+        double a = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fmax(a, fabs(z[i]));   // of a NaN and a number: the number
         a = row_max<LPR>(a);
+        if (a == INFINITY) {                   // the scale is that of the finite values, an infinity a NaN
+          a = 0.0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            z[i] = fabs(z[i]) < INFINITY ? z[i] : NAN;
+            a = fmax(a, fabs(z[i]));
+          }
+          a = row_max<LPR>(a);
+        }
+        codes = e4m3_row(z, a, rs, scale);
+      } else {
+        float a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[i]));
+        a = row_max<LPR>(a);
+        if (a == INFINITY) {
+          a = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = fabsf(x[i]) < INFINITY ? x[i] : NAN;
+            a = fmaxf(a, fabsf(x[i]));
+          }
+          a = row_max<LPR>(a);
+        }
+        codes = e4m3_row(x, a, scale);
       }
-      const float s0 = a * (1.0f / 448.0f);    // a / 448, with its residual's correction
-      const float s = fmaxf(fmaf(fmaf(-s0, 448.0f, a), 1.0f / 448.0f, s0), kMinScale);
-      const float r0 = __builtin_amdgcn_rcpf(s), rs = fmaf(fmaf(-s, r0, 1.0f), r0, r0);
-      if (ln == 0) (kind[u] == 1 ? p.c.ks : p.c.vs)[row] = s;
-      *(u32x2*)((uint8_t*)dst + row * D + c0) =
-          u32x2{e4m3x4(x[0], x[1], x[2], x[3], s, rs), e4m3x4(x[4], x[5], x[6], x[7], s, rs)};
+      if (ln == 0) (kind[u] == 1 ? p.c.ks : p.c.vs)[row] = scale;
+      *(u32x2*)((uint8_t*)dst + row * D + c0) = codes;
     }
   }
 }

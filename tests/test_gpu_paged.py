@@ -212,6 +212,58 @@ def test_prep_e4m3_zeros_tiny_and_values_that_are_not_finite():
     assert bool(((codes[4].double() * s[4].double() - y).abs() <= HALF_E4M3 * y.abs()).all())
 
 
+def test_prep_e4m3_normalised_rows_that_are_not_finite():
+    """Through the head norm: a NaN makes the whole row NaN; an infinity itself, the rest zeros (the
+    norm of the row is infinite); a row of zeros stays zeros."""
+    g = gen(17)
+    kv, D, page = 2, 256, 8
+    x = bf(randn(g, 4, kv, D))
+    x[0, 0, 5] = math.nan
+    x[1, 0, 200] = math.inf
+    x[2, 0] = 0
+    cache = paged.PagedKVCache.alloc(1, page, kv, D, dtype=F8)
+    z = torch.zeros(4, dtype=torch.int32, device=DEV)
+    cos, sin = (t.to(DEV) for t in orc.rope_tables(16, 64, 1e4))
+    at = torch.arange(4, dtype=torch.int32, device=DEV)
+    cache.prep(x.to(DEV), x.to(DEV), z[:1].view(1, 1), at, seq=z, rope=paged.RopeAxes(cos, sin), pos=at,
+               k_norm=torch.zeros(D, device=DEV))
+    k, s = cache.k.cpu()[0].float(), cache.k_scale.cpu()[0]
+    assert bool(torch.isnan(k[0, 0]).all()) and s[0, 0] == ref.MIN_SCALE
+    # the infinity's pair (200 is not turned) alone is NaN
+    assert torch.isnan(k[0, 1]).nonzero().flatten().tolist() == [200] and s[0, 1] == ref.MIN_SCALE
+    assert bool((k[0, 1][~torch.isnan(k[0, 1])] == 0).all())
+    assert bool((k[0, 2] == 0).all()) and s[0, 2] == ref.MIN_SCALE
+    for t in range(4):                                 # the other head's rows are rows of their own
+        y = ref.rotate(ref.head_norm(x[t:t + 1, 1:], torch.zeros(D)), cos.cpu(), sin.cpu(), torch.tensor([[t]]), [0] * 32)
+        check_row(cache.k.cpu()[0, 1, t][None, None], s[1, t][None, None], y, ARITH * ref.pair_size(y, 32) * 2, "row")
+
+
+def test_prep_e4m3_codes_are_those_of_64_bits():
+    """K through norm and rotation: no code differs from the exact quotient's but where this lies within
+    fp32's own rounding of a border between two codes; V: none."""
+    g = gen(18)
+    T, kv, D, page, rot = 300, 4, 256, 16, 64
+    k, v = bf(randn(g, T, kv, D)), bf(randn(g, T, kv, D))
+    kn = randn(g, D, std=0.3)
+    cos, sin = orc.rope_tables(512, rot, 1e7)
+    n_pages = -(-T // page)
+    cache = paged.PagedKVCache.alloc(n_pages, page, kv, D, dtype=F8)
+    at = torch.arange(T, dtype=torch.int32, device=DEV)
+    cache.prep(k.to(DEV), v.to(DEV), torch.arange(n_pages, dtype=torch.int32, device=DEV).view(1, -1), at,
+               seq=torch.zeros_like(at), rope=paged.RopeAxes(cos.to(DEV), sin.to(DEV)), pos=at, k_norm=kn.to(DEV))
+    y = ref.rotate(ref.head_norm(k, kn), cos, sin, at.cpu()[None], [0] * (rot // 2))
+    for got, x in ((cache.k, y), (cache.v, v.double())):
+        z = x * 448 / x.abs().amax(-1, keepdim=True)      # of V's bf16 numbers exact where a tie
+        step = torch.exp2(torch.floor(torch.log2(z.abs().clamp(min=2.0 ** -6))) - 3)
+        want = torch.round(z / step) * step
+        codes = got.cpu().view(torch.uint8).view(n_pages, kv, page, D).transpose(1, 2).reshape(-1, kv, D)[:T].view(F8).double()
+        border = ((z / step - torch.floor(z / step)) - 0.5).abs() * step <= 2.0 ** -23 * z.abs()
+        if x is y:
+            assert bool(((codes == want) | border).all())
+        else:
+            assert torch.equal(codes, want)
+
+
 def test_prep_e4m3_code_of_every_rounding():
     """Rows whose scale is 1 (an element of 448): every bf16 value up to 448 takes the code that
     torch's own conversion gives."""
