@@ -640,7 +640,61 @@ def test_attend_is_the_same_each_time_and_in_any_batch():
         assert torch.equal(cache.attend(q, table.to(DEV), last, ws), first)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_attend_takes_every_position_once(seed):
+    """Batches of all kinds (empty, tiny, whole tiles, long) and head counts over the ways that the work
+    is split: with K zero all weights are equal, so an output is the mean of its sequence's values."""
+    g = gen(100 + seed)
+    B = [1, 2, 3, 7, 15, 16, 31, 33, 64, 65, 200, 600][seed % 12]
+    kv = [1, 2, 3, 4, 8][seed % 5]
+    G, D, page, fp8 = 1 + seed % 3, 128 if seed % 2 else 256, [8, 24, 64][seed % 3], seed % 4 < 2
+    hi = [30, 300, 4000, 40000][seed % 4] if B < 8 else [30, 300, 2000][seed % 3]
+    u = torch.rand(B, generator=g)
+    lens = torch.exp(u * math.log(hi)).long()
+    lens = torch.where(u < 0.1, 0, torch.where(u > 0.8, (lens // 32 + 1) * 32, lens)).tolist()
+    table, n_pages = tables(g, lens, page)
+    v = torch.randn(n_pages, kv, page, D, generator=g, dtype=torch.float32)
+    v = v.to(F8) if fp8 else bf(v)
+    k = torch.zeros(n_pages, kv, page, D, dtype=torch.uint8).view(F8) if fp8 else torch.zeros_like(v)
+    sc = [torch.ones(n_pages, kv, page)] * 2 if fp8 else [None, None]
+    cache = on_gpu((k, v, *sc))
+    q = bf(randn(g, B, kv * G, D))
+    last = torch.tensor(lens, dtype=torch.int32) - 1
+    out = cache.attend(q.to(DEV), table.to(DEV), last.to(DEV), paged.attn_workspace(kv * G, kv, D)).cpu().double()
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        j = torch.arange(n)
+        rows = v[table[b].long()[j // page]] if not fp8 else v.view(torch.uint8)[table[b].long()[j // page]].view(F8)
+        mean = rows.double()[j, :, j % page].mean(0).repeat_interleave(G, 0)    # [heads, D]
+        # sums of n fp32 terms of weight 1 in some order, |v| below 6: well within n 2^-24 6 / n each
+        lim = HALF_BF16 * mean.abs() + 6 * 2.0 ** -20
+        assert bool(((out[b] - mean).abs() <= lim).all()), (b, n)
+
+
 # ------------------------------------------------------------------ streams and graphs
+def test_calls_at_once_on_two_streams_with_workspaces_of_their_own():
+    g = gen(31)
+    H, kv, D, page = 16, 4, 256, 16
+    jobs = []
+    for lens in ([3000, 50, 700], [9000]):
+        table, n_pages = tables(g, lens, page)
+        cache = on_gpu(pool(g, n_pages, kv, page, D, True))
+        q, last = bf(randn(g, len(lens), H, D)).to(DEV), (torch.tensor(lens, dtype=torch.int32) - 1).to(DEV)
+        ws = paged.attn_workspace(H, kv, D)
+        jobs.append((cache, q, table.to(DEV), last, ws, cache.attend(q, table.to(DEV), last, ws), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for (cache, q, table, last, ws, _, st), outs in zip(jobs, got):
+            with torch.cuda.stream(st):
+                outs.append(cache.attend(q, table, last, ws))
+    torch.cuda.synchronize()
+    for job, outs in zip(jobs, got):
+        assert all(torch.equal(o, job[5]) for o in outs)
+
+
 def test_graphs_that_share_a_workspace_follow_lengths_tables_and_streams():
     """Two captured decode steps (other batches, one workspace) replayed in turn while lengths,
     tables and inputs change, against eager calls."""
