@@ -34,6 +34,7 @@
 // leaves a partial record a piece (maximum, sum, outputs) in the workspace, and the last
 // piece to arrive joins them.  All joins go in the order of the pieces: the result does
 // not depend on who comes last.
+#include <algorithm>
 #include <type_traits>
 
 #include "qh_common.h"
@@ -161,6 +162,16 @@ __device__ __forceinline__ int wave_imax(int v) {
   return __builtin_amdgcn_readlane(v, 63);
 }
 
+// a / b for quotients below 2^20 (the compiler's division of 32-bit numbers is three times
+// as long, and a wave that divides has nothing else to do).
+__device__ __forceinline__ int small_quotient(int a, int b) {
+  const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b)), rest = a - q * b;
+  return rest < 0 ? q - 1 : rest >= b ? q + 1 : q;
+}
+__device__ __forceinline__ int small_quotient_s(int a, int b) {  // of numbers that the wave's lanes agree on
+  return __builtin_amdgcn_readfirstlane(small_quotient(a, b));
+}
+
 template <int D, bool FP8, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhPagedAttnParams p) {
   using T = Tile<D, FP8>;
@@ -175,7 +186,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int B = p.c.n_seqs, Hkv = p.c.n_kv, G = p.n_heads / Hkv, ps = p.c.page_size;
+  const int B = p.c.n_seqs, Hkv = p.c.n_kv, G = p.group, ps = p.c.page_size;
   const int wg = blockIdx.x;
   int* s_n = (int*)(s_o + slot_floats(G, D, kWaves));  // [B] positions of sequence b
   int* s_cum = s_n + B;                              // [B] places on the line (of one KV head) of sequences 0 .. b
@@ -200,28 +211,28 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   int total;
   if (few) {
     n_lane = lane < B ? max(min(p.last[lane], p.c.capacity - 1) + 1, 0) : 0;
-    const int tl = (n_lane + kTile - 1) / kTile, most = wave_imax(tl), slots = (int)gridDim.x / Hkv;
+    const int tl = (n_lane + kTile - 1) / kTile, most = wave_imax(tl), slots = p.slots;
     cum_lane = wave_scan(tl > 0 ? tl + 1 : 0);
     const int sum = __builtin_amdgcn_readlane(cum_lane, 63);
-    for (int b = wg; b < B; b += gridDim.x)
+    for (int b = wg; b < B; b += kMaxWG)
       if (length(b) == 0) zeros(b);
     total = sum * Hkv;
     if (most <= kWhole && B <= slots) share = kWhole;
     else if (4 * B <= slots) {
       // equal shares would do if none of them were cut short; that costs a piece a sequence at most
       share = max(4, (sum + slots - 1) / slots);
-      if (__builtin_amdgcn_readlane(wave_scan((tl + share - 1) / share), 63) > slots)
+      if (__builtin_amdgcn_readlane(wave_scan(small_quotient(tl + share - 1, share)), 63) > slots)
         share = max(4, (sum + slots - B - 1) / (slots - B));
     }
     if (share > 0) {
-      const int pc = (tl + share - 1) / share, cum = wave_scan(pc);
+      const int pc = small_quotient(tl + share - 1, share), cum = wave_scan(pc);
       const unsigned long long past = __ballot(cum * Hkv > wg);
       if (past == 0) return;
       seg.b = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
       seg.n = length(seg.b);
       pieces = __builtin_amdgcn_readlane(pc, seg.b);
       const int i = wg - (__builtin_amdgcn_readlane(cum, seg.b) - pieces) * Hkv;
-      seg.kvh = i / pieces;
+      seg.kvh = small_quotient_s(i, pieces);
       const int j = i - seg.kvh * pieces;
       w0 = wg - j;
       seg.u0 = 0;
@@ -255,12 +266,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       if (b0 + i < B) s_cum[b0 + i] += before;
     total = __builtin_amdgcn_readfirstlane(all) * Hkv;
     __syncthreads();
-    for (int b = wg; b < B; b += gridDim.x)
+    for (int b = wg; b < B; b += kMaxWG)
       if (s_n[b] == 0) zeros(b);
   }
   if (w0 < 0) {
     // a share of the line of all tiles
-    ws = max(1, (total + (int)gridDim.x * kWaves - 1) / ((int)gridDim.x * kWaves));
+    ws = max(1, (int)((unsigned)(total + kMaxWG * kWaves - 1) / (kMaxWG * kWaves)));
     share = ws * kWaves;
     start = wg * share;
     end = min(total, start + share);
@@ -279,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     const int first = places_to(lo - 1), places = places_to(lo) - first;
     seg.k = start;
     seg.b = lo;
-    seg.kvh = (start - first * Hkv) / places;
+    seg.kvh = small_quotient_s(start - first * Hkv, places);
     seg.u0 = first * Hkv + seg.kvh * places;
     seg.u1 = seg.u0 + places - 1;
     seg.n = length(lo);
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     for (int i = 0; i < 8; ++i) {
       const char* s = src + i * (FP8 ? D : 2 * D);
       if constexpr (T::VD == 2) {
-        const u32x2 w = *(const u32x2*)(s + 8 * r);
+        const u32x2 w = stream_load<u32x2>(s + 8 * r);
         t.v[i][0] = w.x; t.v[i][1] = w.y;
       } else {
 #pragma unroll
@@ -532,9 +543,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   const int items = G * D / 4;
   struct Item { int h, c; };
   auto item = [&](int i) {
-    const int k = i / (4 * G), ln = i - k * 4 * G, gg = ln / G, rr = k / (DT / 4), d = k % (DT / 4) * 4;
+    const int k = (int)((i >> 2) * p.group_mul >> 20), ln = i - k * 4 * G, gg = (int)(ln * p.group_mul >> 20), rr = k / (DT / 4), d = k % (DT / 4) * 4;
     return Item{ln - gg * G, RUN * (4 * gg + rr) + (FP8 ? d : 128 * (d / 8) + d % 8)};
   };
+  // Where the items need no more than half of the threads, these form groups (whole waves).
+  const int gsize = 1 << p.group_shift, groups = kThreads >> p.group_shift;
+  const int group = wid >> (p.group_shift - 6), gtid = tid & (gsize - 1);
   auto slot_of = [&](int s) { return s_o + (size_t)s * rec; };  // 2 w: begun before wave w, 2 w + 1: by it
   auto put_slot = [&](int s) {
     if (r < G) {
@@ -591,24 +605,28 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     Pair x;
     x.b = c.b;
     x.kvh = c.kvh;
-    x.pieces = w0 >= 0 ? pieces : (c.u1 - 1) / share - c.u0 / share + 1;
-    x.first = w0 >= 0 ? w0 : c.u0 / share;
+    x.first = w0 >= 0 ? w0 : small_quotient_s(c.u0, share);
+    x.pieces = w0 >= 0 ? pieces : small_quotient_s(c.u1 - 1, share) - x.first + 1;
     x.tail = w0 < 0 && c.u0 != x.first * share ? 1 : 0;
     return x;
   };
   {
-    // where the items need no more than half of the threads, groups of these take the pairs in turn
-    const int groups = max(1, kThreads / ((items + 63) / 64 * 64)), group = tid / (kThreads / groups), turns = groups;
     int turn = 0;
+    auto wave_of = [&](int k) {                      // place k of the share lies in its tiles
+      int w = 0;
+#pragma unroll
+      for (int u = 1; u < kWaves; ++u) w += k >= start + u * ws ? 1 : 0;
+      return w;
+    };
     Place c = seg;
     while (true) {
       // pair c lies in waves w .. last; wave w began it, or (w = 0) another workgroup
       const bool begun = c.u0 < start, all = !begun && c.u1 <= end;
-      const int w = begun ? 0 : (c.u0 - start) / ws, last = (min(c.u1, end) - 1 - start) / ws;
+      const int w = begun ? 0 : wave_of(c.u0), last = wave_of(min(c.u1, end) - 1);
       if (!all || last > w) {
-        const bool here = turn++ % turns == group;
+        const bool here = (turn++ & (groups - 1)) == group;
         const int dst = (2 * wg + (c.u0 > start ? 1 : 0)) * rec * 4;  // bytes from the first record
-        for (int i = here ? tid % (kThreads / groups) : items; i < items; i += kThreads / groups) {
+        for (int i = here ? gtid : items; i < items; i += gsize) {
           const Item it = item(i);
           const int head = c.kvh * G + it.h;
           const u32x2 gt = all ? gate_of(c.b, head, it.c) : u32x2{0u, 0u};
@@ -668,23 +686,22 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     if (!s_last[which]) continue;
     const Pair x = which == 0 ? open0 : open1;
     auto rec_of = [&](int j) { return (2 * (x.first + j) + (j == 0 ? x.tail : 0)) * rec * 4; };
-    // a thread takes an item, of every subs-th piece where there are threads enough for that
-    const int subs = items < kThreads ? min(kThreads / items, x.pieces) : 1;
+    // a thread takes an item, of every subs-th piece where there are groups enough for that
+    const int subs = min(groups, x.pieces);
     f32x4* s_a = (f32x4*)s_o;                        // [kThreads]
     float2* s_ml = (float2*)(s_a + kThreads);        // [kThreads]
-    for (int i0 = 0; i0 < items; i0 += kThreads) {
-      const int sub = items < kThreads ? tid / items : 0, i = i0 + tid - sub * items;
+    for (int i0 = 0; i0 < items; i0 += gsize) {
+      const int i = i0 + gtid;
       const Item it = item(min(i, items - 1));
-      const int head = x.kvh * G + it.h;
+      const int head = x.kvh * G + it.h, off = min(i, items - 1) * 16, ml_off = (G * D + 2 * it.h) * 4;
       float M = -INFINITY, L = 0.0f;
       f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-      u32x2 gt = {0u, 0u};
-      if (i < items && sub < subs) {
-        gt = gate_of(x.b, head, it.c);
+      const u32x2 gt = gate_of(x.b, head, it.c);
+      if (group < subs) {
         // 16 pieces under way together, 4 where there are few (the code of 16 alone takes 0.6 us)
         auto read = [&](auto n) {
           constexpr int U = decltype(n)::value;
-          for (int j = sub; j < x.pieces; j += U * subs) {
+          for (int j = group; j < x.pieces; j += U * subs) {
             f32x4 y[U];
             float my[U], ly[U];
 #pragma unroll
@@ -694,8 +711,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
               ly[u] = 0.0f;
               if (j + u * subs < x.pieces) {
                 const int src = rec_of(j + u * subs);
-                y[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, src + i * 16, 0, 16));
-                const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(parts, src + (G * D + 2 * it.h) * 4, 0, 16);
+                y[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, off, src, 16));
+                const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(parts, ml_off, src, 16);
                 my[u] = __uint_as_float(ml.x);
                 ly[u] = __uint_as_float(ml.y);
               }
@@ -703,21 +720,22 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
             add_parts(a, M, L, y, my, ly);
           }
         };
-        if (x.pieces <= 8) read(std::integral_constant<int, 4>{});
+        if (x.pieces <= 4 * subs) read(std::integral_constant<int, 4>{});
         else read(std::integral_constant<int, 16>{});
       }
       if (subs > 1) {
         s_a[tid] = a;
         s_ml[tid] = float2{M, L};
         __syncthreads();
-        if (sub == 0)
+        if (group == 0)
           for (int k = 1; k < subs; ++k) {
-            const f32x4 y[1] = {s_a[k * items + i]};
-            const float my[1] = {s_ml[k * items + i].x}, ly[1] = {s_ml[k * items + i].y};
+            const int src = (k << p.group_shift) + gtid;
+            const f32x4 y[1] = {s_a[src]};
+            const float my[1] = {s_ml[src].x}, ly[1] = {s_ml[src].y};
             add_parts(a, M, L, y, my, ly);
           }
       }
-      if (i < items && sub == 0) emit(x.b, head, it.c, a, L, gt);
+      if (i < items && group == 0) emit(x.b, head, it.c, a, L, gt);
     }
     if (tid == 0) reset_counter(p.counters + x.b * Hkv + x.kvh);
     __syncthreads();
@@ -732,14 +750,21 @@ size_t qh_paged_attn_ws_bytes(int n_heads, int n_kv, int D) {
 }
 
 template <int D, bool FP8, int kWaves>
-static int launch(const QhPagedAttnParams& p, hipStream_t st) {
-  const size_t lds = (size_t)slot_floats(p.n_heads / p.c.n_kv, D, kWaves) * sizeof(float) + (size_t)p.c.n_seqs * 8;
+static int launch(QhPagedAttnParams p, hipStream_t st) {
+  const int items = p.group * D / 4;
+  p.group_shift = 6;
+  while ((1 << p.group_shift) < std::min(items, 64 * kWaves)) ++p.group_shift;
+  const size_t lds = (size_t)slot_floats(p.group, D, kWaves) * sizeof(float) + (size_t)p.c.n_seqs * 8;
   hipLaunchKernelGGL((paged_attn_kernel<D, FP8, kWaves>), dim3(kMaxWG), dim3(64 * kWaves), lds, st, p);
   return 0;
 }
 
-int qh_launch_paged_attn(const QhPagedAttnParams& p, int D, hipStream_t st) {
-  const bool four = waves_of(p.n_heads / p.c.n_kv, D, p.c.ks != nullptr) == 4;
+int qh_launch_paged_attn(QhPagedAttnParams p, int D, hipStream_t st) {
+  p.group = p.n_heads / p.c.n_kv;
+  // i < 1024: floor(i group_mul / 2^20) = floor(i / group) (group_mul group - 2^20 < 16)
+  p.group_mul = ((1u << 20) + p.group - 1) / p.group;
+  p.slots = kMaxWG / p.c.n_kv;
+  const bool four = waves_of(p.group, D, p.c.ks != nullptr) == 4;
   if (D == 256) {
     if (!p.c.ks) return launch<256, false, 4>(p, st);
     return four ? launch<256, true, 4>(p, st) : launch<256, true, 8>(p, st);

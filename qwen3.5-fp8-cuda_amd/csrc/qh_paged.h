@@ -65,6 +65,11 @@ struct QhPagedAttnParams {
   uint16_t* out;          // [n_seqs][n_heads][D] bf16
   unsigned* counters;     // [kPagedMaxUnits] zero between calls
   float* part;
+  // what the launch derives for the kernel, which would spend its time on divisions
+  int group;              // heads of a KV head
+  uint32_t group_mul;     // i / group = i * group_mul >> 20 for i < 1024
+  int group_shift;        // log2 of the threads that take a pair's items together
+  int slots;              // workgroups of each KV head
 };
 
 // (sequence, kv head) pairs that one call of the decode attention takes, and its sequences.
@@ -76,7 +81,7 @@ int qh_paged_view(const qh_paged_cache* c, const int* pages, int n_seqs, int max
 int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st);
 int qh_launch_paged_read(const QhPagedReadParams& p, int D, hipStream_t st);
 size_t qh_paged_attn_ws_bytes(int n_heads, int n_kv, int D);
-int qh_launch_paged_attn(const QhPagedAttnParams& p, int D, hipStream_t st);
+int qh_launch_paged_attn(QhPagedAttnParams p, int D, hipStream_t st);
 void qh_set_error(const char* fmt, ...);
 
 #if defined(__HIPCC__)
