@@ -176,7 +176,12 @@ template <int D, bool FP8, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhPagedAttnParams p) {
   using T = Tile<D, FP8>;
   constexpr int kThreads = 64 * kWaves;
-  constexpr int kWhole = 2 * kWaves;                 // tiles of a pair that one workgroup takes rather than join pieces
+  // Tiles of a pair that one workgroup takes rather than join pieces.  A wave's second tile of
+  // 256 E4M3 values takes longer than the join (1 sequence of 400 positions, 16 / 4 heads: 11.0 us
+  // in one workgroup, 9.7 in pieces; 16 of them: 11.9 and 11.4), one of 128 does not (32 / 8 heads:
+  // 8.4 and 8.6; 16 of them: 9.2 and 12.5), nor one of bf16, which has a SIMD to itself (10.4
+  // and 10.6 of 256).
+  constexpr int kWhole = D == 256 && kWaves == 8 ? kWaves : 2 * kWaves;
   constexpr int DT = D / 16;                         // 16-dim tiles of the output
   constexpr int KK = D / 32;                         // products of a score tile
   constexpr int RUN = FP8 ? DT : 8;                  // consecutive dims of a lane
