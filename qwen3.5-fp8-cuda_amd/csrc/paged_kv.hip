@@ -19,6 +19,7 @@
 // fp32 correctly, which keeps the ties between two codes that such quotients often are;
 // K's, in which the factor rsqrt(..) cancels, is computed in 64 bits (as fast as 32 here).
 #include <algorithm>
+#include <type_traits>
 
 #include "qh_common.h"
 #include "qh_paged.h"
@@ -325,21 +326,24 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, in
   }
 }
 
-// Read back (qh_kv_read_paged): 16 bytes of a cached row a lane, K and V side by side,
-// kReadRows rows of each under way together.  A workgroup takes positions blockIdx.x,
-// blockIdx.x + gridDim.x, ... (in units of its rows) of one sequence and KV head.
+// Read back (qh_kv_read_paged): 8 values of a cached row a lane, so that each store writes
+// whole cache lines, K and V side by side, kReadRows rows of each under way together.  A
+// workgroup takes positions blockIdx.x, blockIdx.x + gridDim.x, ... (in units of its rows) of
+// one sequence and KV head.  HBM bounds it: 61700 positions of 4 heads of 256 in E4M3 take 69 us
+// (5.5 TB/s), 82 with 16 values a lane, whose stores write half lines, and 75 with plain stores
+// (bf16, which asks for twice as much for each store: 35 us with plain ones, 37 without).
 constexpr int kReadRows = 2;
 template <int D, bool FP8>
 __global__ __launch_bounds__(256) void paged_read_kernel(QhPagedReadParams p) {
-  constexpr int E = FP8 ? 16 : 8;              // values of 16 cached bytes
-  constexpr int LPR = D / E, RPB = 256 / LPR * kReadRows;
+  using W = typename std::conditional<FP8, u32x2, u32x4>::type;  // 8 values
+  constexpr int LPR = D / 8, RPB = 256 / LPR * kReadRows;
   const int pair = blockIdx.y, b = pair / p.c.n_kv, head = pair - b * p.c.n_kv;
   const int n = min(min(p.last[b], p.max_seq - 1), p.c.capacity - 1) + 1;
   const int* pages = p.c.pages + (size_t)b * p.c.max_pages;
-  const int mine = threadIdx.x / LPR, c = threadIdx.x % LPR * E;
+  const int mine = threadIdx.x / LPR, c = threadIdx.x % LPR * 8;
   for (int p0 = blockIdx.x * RPB; p0 < n; p0 += gridDim.x * RPB) {
     long long row[kReadRows];
-    u32x4 k[kReadRows], v[kReadRows];
+    W k[kReadRows], v[kReadRows];
     float ks[kReadRows], vs[kReadRows];
     bool ok[kReadRows];
 #pragma unroll
@@ -351,8 +355,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(QhPagedReadParams p) {
 #pragma unroll
     for (int u = 0; u < kReadRows; ++u) {
       const size_t o = (size_t)row[u] * D + c;
-      k[u] = __builtin_nontemporal_load((const u32x4*)((const char*)p.c.k + o * (16 / E)));
-      v[u] = __builtin_nontemporal_load((const u32x4*)((const char*)p.c.v + o * (16 / E)));
+      k[u] = __builtin_nontemporal_load((const W*)((const char*)p.c.k + o * (FP8 ? 1 : 2)));
+      v[u] = __builtin_nontemporal_load((const W*)((const char*)p.c.v + o * (FP8 ? 1 : 2)));
       ks[u] = FP8 ? p.c.ks[row[u]] : 1.0f;
       vs[u] = FP8 ? p.c.vs[row[u]] : 1.0f;
     }
@@ -361,17 +365,14 @@ __global__ __launch_bounds__(256) void paged_read_kernel(QhPagedReadParams p) {
       if (!ok[u]) continue;
       const size_t o = ((size_t)pair * p.max_seq + p0 + mine + u * (256 / LPR)) * D + c;
       if constexpr (FP8) {
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          auto four = [](uint32_t x, float s) {
-            const qh_f32x2 lo = e4m3x2_lo_f32(x), hi = e4m3x2_hi_f32(x);
-            return u32x2{pack_bf2(lo.x * s, lo.y * s), pack_bf2(hi.x * s, hi.y * s)};
-          };
-          const u32x2 k0 = four(k[u][i], ks[u]), k1 = four(k[u][i + 1], ks[u]);
-          const u32x2 v0 = four(v[u][i], vs[u]), v1 = four(v[u][i + 1], vs[u]);
-          *(u32x4*)(p.k_out + o + 4 * i) = u32x4{k0.x, k0.y, k1.x, k1.y};
-          *(u32x4*)(p.v_out + o + 4 * i) = u32x4{v0.x, v0.y, v1.x, v1.y};
-        }
+auto four = [](uint32_t x, float s) {
+          const qh_f32x2 lo = e4m3x2_lo_f32(x), hi = e4m3x2_hi_f32(x);
+          return u32x2{pack_bf2(lo.x * s, lo.y * s), pack_bf2(hi.x * s, hi.y * s)};
+        };
+        const u32x2 k0 = four(k[u].x, ks[u]), k1 = four(k[u].y, ks[u]);
+        const u32x2 v0 = four(v[u].x, vs[u]), v1 = four(v[u].y, vs[u]);
+        put(u32x4{k0.x, k0.y, k1.x, k1.y}, p.k_out + o);
+        put(u32x4{v0.x, v0.y, v1.x, v1.y}, p.v_out + o);
       } else {
         *(u32x4*)(p.k_out + o) = k[u];
         *(u32x4*)(p.v_out + o) = v[u];
@@ -525,7 +526,7 @@ int qh_launch_paged_read(const QhPagedReadParams& p, int D, hipStream_t st) {
     return -1;
   }
   const int most = std::min(p.max_seq, p.c.capacity), pairs = p.c.n_seqs * p.c.n_kv;
-  const int rows = 256 / (D / (p.c.ks ? 16 : 8)) * kReadRows;
+  const int rows = 256 / (D / 8) * kReadRows;
   const dim3 grid(std::max(1, std::min((most + rows - 1) / rows, 16384 / pairs)), pairs);
   if (D == 256) {
     if (p.c.ks) hipLaunchKernelGGL((paged_read_kernel<256, true>), grid, dim3(256), 0, st, p);
