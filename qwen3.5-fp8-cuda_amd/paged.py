@@ -24,14 +24,11 @@ from . import abi
 FP8 = torch.float8_e4m3fn
 _INT, _BF, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
 _NO_STRIDE = (0, 0, 1)
-_current_device = torch.cuda.current_device
-
-
-def _raw_stream(dev):
-    """hipStream_t of the current torch stream of GPU `dev`: torch.cuda.current_stream(dev).cuda_stream
-    without the Stream object."""
-    return torch._C._cuda_getCurrentRawStream(dev)
-
+# torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream without the Python
+# around them, which a decode step's host would spend a microsecond on (a torch without a GPU
+# build has neither, and no cache to call them for)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _need(t, name, dtype, shape, dev, contiguous=True):
@@ -131,13 +128,13 @@ class PagedKVCache:
         [axes, T] (or [T] for one axis).  A token with an index out of range (padding:
         -1) is left out altogether.  Returns q_out."""
         dev, D, n_kv = self.dev, self.head_dim, self.n_kv
-        T = len(k)
-        H = 0
-        shape, row = (T, n_kv, D), (T,)
+        kn = k.shape
+        T = kn[0] if kn else 0
+        H, shape, row = 0, (T, n_kv, D), (T,)
         ks, vs, pn = k.stride(), v.stride(), pages.shape
         good = (k.dtype is _BF and v.dtype is _BF and pages.dtype is _INT and at.dtype is _INT
                 and k.get_device() == dev and v.get_device() == dev and pages.get_device() == dev
-                and at.get_device() == dev and k.shape == shape and v.shape == shape and at.shape == row
+                and at.get_device() == dev and kn == shape and v.shape == shape and at.shape == row
                 and len(pn) == 2 and pages.is_contiguous() and at.is_contiguous()
                 and ks[2] == 1 and vs[2] == 1 and (n_kv == 1 or ks[1] == D and vs[1] == D))
         p_seq = p_q = p_out = p_rope = p_pos = p_qn = p_kn = None
@@ -174,13 +171,20 @@ class PagedKVCache:
             good = False
         if not good:
             self._refuse_prep(k, v, pages, at, seq, q, q_out, rope, pos, q_norm, k_norm)
-        self._call("attn_prep_paged", self._prep, self._ref, p_rope, p_q, qs, qh, k.data_ptr(), ks[0], v.data_ptr(),
-                   vs[0], p_qn, p_kn, eps, p_pos, p_seq, at.data_ptr(), T, pages.data_ptr(), pn[0], pn[1], p_out, f32, H)
+        args = (self._ref, p_rope, p_q, qs, qh, k.data_ptr(), ks[0], v.data_ptr(), vs[0], p_qn, p_kn, eps, p_pos, p_seq,
+                at.data_ptr(), T, pages.data_ptr(), pn[0], pn[1], p_out, f32, H, _raw_stream(dev))
+        if _current_device() == dev:
+            rc = self._prep(*args)
+        else:
+            with torch.cuda.device(dev):
+                rc = self._prep(*args)
+        if rc != 0:
+            abi.check(rc, "attn_prep_paged")
         return q_out
 
     def _refuse_prep(self, k, v, pages, at, seq, q, q_out, rope, pos, q_norm, k_norm):
         """Raise for the first argument of `prep` that it does not take."""
-        D, dev, T = self.head_dim, self.dev, len(k)
+        D, dev, T = self.head_dim, self.dev, k.shape[0] if k.dim() else 0
         for t, name in ((k, "k"), (v, "v")):
             self._need_heads(t, name, T, self.n_kv)
             if self.n_kv > 1 and t.stride(1) != D:
