@@ -34,6 +34,11 @@
 // leaves a partial record a piece (maximum, sum, outputs) in the workspace, and the last
 // piece to arrive joins them.  All joins go in the order of the pieces: the result does
 // not depend on who comes last.
+//
+// Measured: 128 sequences of 500 to 6000 positions (64 / 8 heads of 128, bf16) 187 us, 6.2 TB/s;
+// one of 200001 (16 / 4 heads of 256, E4M3) 74 us, 5.7 TB/s, of 4096 12.9 us; 43 of 1 to 8000 32 us,
+// 4.2 TB/s.  With the arithmetic taken out the long ones take as long.  Short ones are a chain of
+// dependent round trips: length, page ids, rows, LDS join, record, arrival, records.
 #include <algorithm>
 #include <type_traits>
 
@@ -46,7 +51,8 @@ constexpr int kTile = 32;    // positions per wave and step
 constexpr int kMaxWG = 256;  // workgroups that hold a share (one per CU)
 constexpr int kMaxG = 16;
 // Waves of a workgroup: two to a SIMD; one where a tile of bf16 rows of 256 fills the
-// registers, or where the LDS has no room for the partial results of eight.
+// registers (16 / 4 heads, 300 positions: 11.9 us with four waves, 16.6 with eight), or where
+// the LDS has no room for the partial results of eight.
 constexpr int waves_of(int G, int D, bool fp8) { return D == 256 && (!fp8 || G > 8) ? 4 : 8; }
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
@@ -126,7 +132,7 @@ __host__ __device__ constexpr int slot_floats(int G, int D, int waves) {
 // A tile on the line: its sequence and KV head, and the tiles [u0, u1) of that pair.  A place
 // of the line is left empty behind each pair: its end costs a wave about a tile's time, and
 // waves with many short pairs held up the others (43 sequences of 1 to 8000 positions,
-// E4M3, 16 / 4 heads of 256: 43.5 us without).
+// E4M3, 16 / 4 heads of 256: 43.5 us without it, 34.8 with).
 struct Place {
   int k, b, kvh, u0, u1, n;
 };

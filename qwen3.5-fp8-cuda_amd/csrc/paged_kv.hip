@@ -150,8 +150,9 @@ __device__ __forceinline__ u32x2 e4m3_row(const double (&x)[8], double amax, flo
 // once; the next token's rows are under way while one is computed.  Where the tokens'
 // rows go and the cos and sin of their pairs (which the axes gather from up to four rows
 // of the tables) are found once a token and kept in LDS, behind the request for the
-// first rows.  HBM bounds it for prompts, the chain position -> table and index -> page
-// -> row for single tokens.
+// first rows.  For prompts HBM bounds it, with the arithmetic close behind (3700 tokens of 16 / 4
+// heads of 256 into E4M3 with fp32 q: 27 to 30 us, 3.9 to 4.2 TB/s, the VALU busy half of
+// it); for single tokens the chain position -> table and index -> page -> row (4.9 us).
 template <int D, int R>
 __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, int tokens) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a pass
@@ -489,11 +490,12 @@ int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
     }
   }
   const int rows = (p.q ? p.n_heads : 0) + 2 * p.c.n_kv, pass = 256 / (D / 8), passes = (rows + pass - 1) / pass;
-  // A head a thread while that leaves no more than some four workgroups a CU; then up to 4
-  // of them, and workgroups of up to 4 tokens that still fill the CUs three times (3700
-  // tokens: 38 us with one, 33 with 2 or 4, 37 with 8).
+  // A head a thread while that leaves no more than six workgroups a CU (16 / 4 heads of 256: 400
+  // tokens, 1200 workgroups, 6.4 us against 7.1 with three heads a thread; 700 tokens, 2100, 10.7
+  // against 8.5); then up to 4 of them, and workgroups of up to 4 tokens that still fill the CUs
+  // three times (3700 tokens: 34.6 us with one, 29.8 with 2, 29.5 with 4, 32.8 with 8).
   int tokens = 1, groups = passes;
-  if ((long long)p.T * passes > 1024) {
+  if ((long long)p.T * passes > 1536) {
     groups = (passes + 3) / 4;
     tokens = (int)std::min<long long>(kPrepTokens, std::max<long long>(1, (long long)p.T * groups / 768));
   }
