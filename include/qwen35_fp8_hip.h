@@ -444,12 +444,12 @@ size_t qh_attn_decode_paged_workspace_size(int n_heads, int n_kv, int head_dim);
 /* Attention of one new token of each sequence: softmax(q . K^T / sqrt(D)) V over
  * positions 0 .. last[b] (whose rows, the new token's among them, are in the
  * cache), times sigmoid(gate) with a gate; out [n_seqs][n_heads][D] bf16, zeros for
- * a sequence with no visible position.  q (bf16, normalised and rotated) has
- * sequence b's head h at q + b * q_bstride + h * q_hstride, the gate likewise
- * (elements; multiples of 8; 16-byte aligned pointers).  n_heads / n_kv <= 16, at
- * most 2048 sequences, 65536 (sequence, KV head) pairs and 2^31 - 65536 tiles of 32
- * positions (n_seqs * n_kv * max_pages * page_size / 32).  out must not overlap q or the
- * gate.  ws:
+ * a sequence with no visible position, or none whose score is above -infinity.
+ * q (bf16, normalised and rotated) has sequence b's head h at q + b * q_bstride +
+ * h * q_hstride, the gate likewise (elements; multiples of 8; 16-byte aligned
+ * pointers); out must not overlap them.  n_heads / n_kv <= 16, at most 2048
+ * sequences, 65536 (sequence, KV head) pairs and 2^31 - 65536 tiles of 32 positions
+ * (n_seqs * n_kv * max_pages * page_size / 32).  ws:
  * qh_attn_decode_paged_workspace_size bytes, 256-byte aligned, zeroed once when it
  * is allocated (the kernel returns its counters to zero); calls that share a
  * workspace must not overlap. */

@@ -539,8 +539,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     return p.gate ? *(const u32x2*)(p.gate + b * p.g_bs + (long long)head * p.g_hs + c) : u32x2{0u, 0u};
   };
   auto emit = [&](int b, int head, int c, f32x4 a, float L, u32x2 gt) {
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (L == 0.0f) a = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float inv = 1.0f / L;
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = a[i] * inv;
@@ -548,7 +547,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       y[0] *= qh_sigmoid_bf(bf_lo(gt.x)); y[1] *= qh_sigmoid_bf(bf_hi(gt.x));
       y[2] *= qh_sigmoid_bf(bf_lo(gt.y)); y[3] *= qh_sigmoid_bf(bf_hi(gt.y));
     }
-    *(u32x2*)(p.out + ((size_t)b * p.n_heads + head) * D + c) = u32x2{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+    u32x2 w = {pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+    if (L == 0.0f) w = u32x2{0u, 0u};                // nothing visible, whatever the gate holds
+    *(u32x2*)(p.out + ((size_t)b * p.n_heads + head) * D + c) = w;
   };
   // Item i of a partial result: head and first of its 4 dims.
   const int items = G * D / 4;

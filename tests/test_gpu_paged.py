@@ -558,6 +558,18 @@ def test_attend_leaves_out_pages_that_do_not_exist_and_ends_at_the_table(fp8):
     assert bool((out[3] == 0).all())
 
 
+@pytest.mark.parametrize("lens", [(0, 40, 900), (0, 40, 40000)])   # in one workgroup, in pieces
+def test_attend_to_nothing_is_zeros_whatever_the_gate_holds(lens):
+    g = gen(30)
+    H, kv, D, page = 8, 2, 256, 16
+    table, n_pages = tables(g, lens, page)
+    table[:] = -1
+    out = on_gpu(pool(g, n_pages, kv, page, D, True)).attend(
+        bf(randn(g, 3, H, D)).to(DEV), table.to(DEV), torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=DEV),
+        paged.attn_workspace(H, kv, D), gate=torch.full((3, H, D), math.nan, dtype=torch.bfloat16, device=DEV))
+    assert bool((out == 0).all())
+
+
 def test_attend_propagates_a_visible_nan():
     g = gen(24)
     H, kv, D, page, n = 4, 2, 128, 8, 300
