@@ -234,6 +234,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       share = max(4, (sum + slots - 1) / slots);
       if (__builtin_amdgcn_readlane(wave_scan(small_quotient(tl + share - 1, share)), 63) > slots)
         share = max(4, (sum + slots - B - 1) / (slots - B));
+      // Four waves have a SIMD each, eight take as long for 5 tiles as for 8; and from some length on
+      // half the pieces are worth a shared SIMD (1 sequence, 32 / 8 heads of 128, E4M3: 2000 positions
+      // 10.2 us with shares of 4, 10.6 of 8, 4096 12.6 and 11.3; 16 / 4 of 256: 3000 12.3 and 13.1,
+      // 6000 15.5 and 14.5; 3 of 3000 in shares of 5: 15.6 and 14.3).
+      if (share < 8 && (share > 4 || most > D / 2)) share = 8;
     }
     if (share > 0) {
       const int pc = small_quotient(tl + share - 1, share), cum = wave_scan(pc);
