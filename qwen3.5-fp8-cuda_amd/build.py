@@ -3,7 +3,8 @@
 Replaces the reference's compile.bat (nvcc -> two Windows DLLs): one shared
 library exporting both the reference's ctypes symbols and the native qh_*
 entry points.  Objects are compiled in parallel; the library is written next
-to this file so it travels with the source tree.
+to this file so it travels with the source tree, as is the extension module
+_paged_host.so (csrc/paged_host.cpp, host code against torch's headers).
 
     python build.py [--jobs N] [--debug]
 """
@@ -13,11 +14,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libqwen35_fp8_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+HOST_PATH = os.path.join(HERE, "_paged_host.so")
 ARCH = os.environ.get("QH_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -52,6 +55,23 @@ def compile_one(cc, src, obj, extra):
     return obj
 
 
+def build_host(extra):
+    """The extension module that checks and launches the paged cache's calls."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    tmp = HOST_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", *extra,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "paged_host.cpp"), "-o", tmp,
+           "-L", os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"paged_host.cpp failed:\n{r.stderr}")
+    os.replace(tmp, HOST_PATH)
+
+
 def build(jobs=None, debug=False, verbose=True):
     cc = hipcc()
     objdir = os.path.join(HERE, "_build")
@@ -61,7 +81,8 @@ def build(jobs=None, debug=False, verbose=True):
     objs = [os.path.join(objdir, os.path.basename(s)[:-4] + ".o") for s in srcs]
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 4)))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        futs = [ex.submit(compile_one, cc, s, o, extra) for s, o in zip(srcs, objs)]
+        futs = [ex.submit(build_host, extra)]
+        futs += [ex.submit(compile_one, cc, s, o, extra) for s, o in zip(srcs, objs)]
         for f in futs:
             f.result()
     tmp = LIB_PATH + ".tmp"

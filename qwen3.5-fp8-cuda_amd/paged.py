@@ -23,12 +23,20 @@ from . import abi
 
 FP8 = torch.float8_e4m3fn
 _INT, _BF, _F32, _U8 = torch.int32, torch.bfloat16, torch.float32, torch.uint8
-_NO_STRIDE = (0, 0, 1)
 # torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream without the Python
 # around them, which a decode step's host would spend a microsecond on (a torch without a GPU
 # build has neither, and no cache to call them for)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _host():
+    """The extension module that checks and launches the calls (csrc/paged_host.cpp)."""
+    try:
+        from . import _paged_host
+    except ImportError as e:
+        raise ImportError("_paged_host.so does not load: build it with `python qwen3.5-fp8-cuda_amd/build.py`") from e
+    return _paged_host
 
 
 def _need(t, name, dtype, shape, dev, contiguous=True):
@@ -92,8 +100,10 @@ class PagedKVCache:
                                         v_scale.data_ptr() if self.fp8 else None,
                                         self.n_pages, self.page_size, self.n_kv, self.head_dim, int(self.fp8))
         self._ref = ctypes.addressof(self._desc)
-        lib = abi.load()
-        self._prep, self._read, self._attend = lib.qh_attn_prep_paged, lib.qh_kv_read_paged, lib.qh_attn_decode_paged
+        lib, host = abi.load(), _host()
+        entries = (lib.qh_attn_prep_paged, lib.qh_kv_read_paged, lib.qh_attn_decode_paged)
+        self._prep_at, self._read_at, self._attend_at = (ctypes.cast(f, ctypes.c_void_p).value for f in entries)
+        self._prep, self._read, self._attend = host.prep, host.read, host.attend
 
     @classmethod
     def alloc(cls, n_pages, page_size, n_kv, head_dim, dtype=_BF, device="cuda"):
@@ -104,18 +114,15 @@ class PagedKVCache:
             return cls(*kv)
         return cls(*(t.view(FP8) for t in kv), *(torch.zeros(shape[:3], device=device) for _ in range(2)))
 
-    def _call(self, what, fn, *args):
-        """Launch on the current stream of the cache's device."""
-        if _current_device() == self.dev:
-            rc = fn(*args, _raw_stream(self.dev))
-        else:
-            with torch.cuda.device(self.dev):
-                rc = fn(*args, _raw_stream(self.dev))
-        if rc != 0:
-            abi.check(rc, what)
+    # The native module checks a call's tensors and launches it; it hands back None where one
+    # does not fit, and only then are they gone through one by one, for the message.
 
-    # Each call checks its tensors in one expression, which costs a decode step's host a
-    # few microseconds; only where it fails are they gone through one by one, for the message.
+    def _call(self, fn, *args):
+        """Launch with the cache's device as the current one."""
+        if _current_device() == self.dev:
+            return fn(*args)
+        with torch.cuda.device(self.dev):
+            return fn(*args)
 
     def prep(self, k, v, pages, at, seq=None, q=None, q_out=None, rope=None, pos=None, q_norm=None, k_norm=None,
              eps=1e-6):
@@ -127,57 +134,14 @@ class PagedKVCache:
         default) or fp32 (what qh_attn_prefill takes).  rope: RopeAxes with pos int32
         [axes, T] (or [T] for one axis).  A token with an index out of range (padding:
         -1) is left out altogether.  Returns q_out."""
-        dev, D, n_kv = self.dev, self.head_dim, self.n_kv
-        kn = k.shape
-        T = kn[0] if kn else 0
-        H, shape, row = 0, (T, n_kv, D), (T,)
-        ks, vs, pn = k.stride(), v.stride(), pages.shape
-        good = (k.dtype is _BF and v.dtype is _BF and pages.dtype is _INT and at.dtype is _INT
-                and k.get_device() == dev and v.get_device() == dev and pages.get_device() == dev
-                and at.get_device() == dev and kn == shape and v.shape == shape and at.shape == row
-                and len(pn) == 2 and pages.is_contiguous() and at.is_contiguous()
-                and ks[2] == 1 and vs[2] == 1 and (n_kv == 1 or ks[1] == D and vs[1] == D))
-        p_seq = p_q = p_out = p_rope = p_pos = p_qn = p_kn = None
-        f32 = qs = qh = 0
-        if good and seq is not None:
-            good = seq.dtype is _INT and seq.get_device() == dev and seq.shape == row and seq.is_contiguous()
-            p_seq = seq.data_ptr()
-        if good and rope is not None:
-            good = (pos is not None and pos.dtype is _INT and pos.get_device() == dev and rope.dev == dev
-                    and (pos.shape == (rope.n_axes, T) or rope.n_axes == 1 and pos.shape == row)
-                    and pos.is_contiguous())
-            p_rope, p_pos = rope._ref, pos.data_ptr() if good else None
-        if good and q_norm is not None:
-            good = (q_norm.dtype is _F32 and q_norm.get_device() == dev and q_norm.shape == (D,)
-                    and q_norm.is_contiguous())
-            p_qn = q_norm.data_ptr()
-        if good and k_norm is not None:
-            good = (k_norm.dtype is _F32 and k_norm.get_device() == dev and k_norm.shape == (D,)
-                    and k_norm.is_contiguous())
-            p_kn = k_norm.data_ptr()
-        if good and q is not None:
-            n = q.shape
-            good = q.dtype is _BF and q.get_device() == dev and len(n) == 3 and n[0] == T and n[2] == D
-            if good:
-                H = n[1]
-                qs, qh, last = q.stride()
-                if q_out is None:
-                    q_out = torch.empty(T, H, D, dtype=_BF, device=self.device)
-                f32 = q_out.dtype is _F32
-                good = (last == 1 and (f32 or q_out.dtype is _BF) and q_out.get_device() == dev and q_out.shape == n
-                        and q_out.is_contiguous())
-                p_q, p_out = q.data_ptr(), q_out.data_ptr()
-        elif q_out is not None:
-            good = False
-        if not good:
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=_BF, device=self.device)
+        if rope is not None and rope.dev != self.dev:
+            raise ValueError(f"rope: must be on cuda:{self.dev}")
+        rc = self._call(self._prep, self._prep_at, self._ref, self.dev, 0 if rope is None else rope._ref, k, v, pages, at,
+                        seq, q, q_out, pos, q_norm, k_norm, eps, _raw_stream(self.dev))
+        if rc is None:
             self._refuse_prep(k, v, pages, at, seq, q, q_out, rope, pos, q_norm, k_norm)
-        args = (self._ref, p_rope, p_q, qs, qh, k.data_ptr(), ks[0], v.data_ptr(), vs[0], p_qn, p_kn, eps, p_pos, p_seq,
-                at.data_ptr(), T, pages.data_ptr(), pn[0], pn[1], p_out, f32, H, _raw_stream(dev))
-        if _current_device() == dev:
-            rc = self._prep(*args)
-        else:
-            with torch.cuda.device(dev):
-                rc = self._prep(*args)
         if rc != 0:
             abi.check(rc, "attn_prep_paged")
         return q_out
@@ -194,8 +158,6 @@ class PagedKVCache:
         if seq is not None:
             _need(seq, "seq", _INT, (T,), dev)
         if rope is not None:
-            if rope.dev != dev:
-                raise ValueError(f"rope: must be on cuda:{dev}")
             if pos is None:
                 raise ValueError("rope: needs pos")
             _need(pos, "pos", _INT, (T,) if pos.dim() == 1 and rope.n_axes == 1 else (rope.n_axes, T), dev)
@@ -219,21 +181,17 @@ class PagedKVCache:
     def read(self, pages, last, k_out, v_out):
         """Positions 0 .. last[b] (int32 [B]) of each sequence to k_out, v_out bf16
         [B, n_kv, max_seq, D]; rows behind them keep what they hold."""
-        dev, pn, n = self.dev, pages.shape, k_out.shape
-        if not (pages.dtype is _INT and last.dtype is _INT and k_out.dtype is _BF and v_out.dtype is _BF
-                and pages.get_device() == dev and last.get_device() == dev and k_out.get_device() == dev
-                and v_out.get_device() == dev and len(pn) == 2 and last.shape == pn[:1] and len(n) == 4
-                and n[0] == pn[0] and n[1] == self.n_kv and n[3] == self.head_dim and v_out.shape == n
-                and pages.is_contiguous() and last.is_contiguous() and k_out.is_contiguous()
-                and v_out.is_contiguous()):
-            B = pn[0]
+        rc = self._call(self._read, self._read_at, self._ref, self.dev, pages, last, k_out, v_out, _raw_stream(self.dev))
+        if rc is None:
+            dev = self.dev
             _need(pages, "pages", _INT, (None, None), dev)
+            B = len(pages)
             _need(last, "last", _INT, (B,), dev)
             _need(k_out, "k_out", _BF, (B, self.n_kv, None, self.head_dim), dev)
-            _need(v_out, "v_out", _BF, tuple(n), dev)
+            _need(v_out, "v_out", _BF, tuple(k_out.shape), dev)
             raise ValueError("read: arguments that do not fit together")
-        self._call("kv_read_paged", self._read, self._ref, pages.data_ptr(), pn[0], pn[1], last.data_ptr(),
-                   k_out.data_ptr(), v_out.data_ptr(), n[2])
+        if rc != 0:
+            abi.check(rc, "kv_read_paged")
 
     def attend(self, q, pages, last, ws, gate=None, out=None):
         """out[b, h] = softmax(q[b, h] . K^T / sqrt(D)) V over positions 0 .. last[b]
@@ -241,35 +199,23 @@ class PagedKVCache:
         empty sequence (last[b] < 0).  q, gate: bf16 [B, n_heads, D], any strides, q as
         `prep` wrote it; ws: ``attn_workspace`` (calls that share one must not overlap).
         Returns out, bf16 [B, n_heads, D]."""
-        dev, n, pn = self.dev, q.shape, pages.shape
-        qs = q.stride()
-        good = (q.dtype is _BF and pages.dtype is _INT and last.dtype is _INT and ws.dtype is _U8
-                and q.get_device() == dev and pages.get_device() == dev and last.get_device() == dev
-                and ws.get_device() == dev and len(n) == 3 and n[2] == self.head_dim and len(pn) == 2
-                and pn[0] == n[0] and last.shape == n[:1] and qs[2] == 1
-                and pages.is_contiguous() and last.is_contiguous() and ws.is_contiguous())
-        p_gate, gs = None, _NO_STRIDE
-        if good and gate is not None:
-            gs = gate.stride()
-            good = gate.dtype is _BF and gate.get_device() == dev and gate.shape == n and gs[2] == 1
-            p_gate = gate.data_ptr()
-        if good and out is not None:
-            good = out.dtype is _BF and out.get_device() == dev and out.shape == n and out.is_contiguous()
-        if not good:
-            B, H = (n[0], n[1]) if len(n) == 3 else (None, None)
-            self._need_heads(q, "q", B, None)
+        if out is None:
+            out = torch.empty(q.shape, dtype=_BF, device=self.device)
+        rc = self._call(self._attend, self._attend_at, self._ref, self.dev, q, pages, last, ws, gate, out,
+                        _raw_stream(self.dev))
+        if rc is None:
+            dev = self.dev
+            self._need_heads(q, "q", None, None)
+            B, H = q.shape[:2]
             if gate is not None:
                 self._need_heads(gate, "gate", B, H)
             _need(pages, "pages", _INT, (B, None), dev)
             _need(last, "last", _INT, (B,), dev)
             _need(ws, "ws", _U8, (None,), dev)
-            if out is not None:
-                _need(out, "out", _BF, tuple(n), dev)
+            _need(out, "out", _BF, tuple(q.shape), dev)
             raise ValueError("attend: arguments that do not fit together")
-        if out is None:
-            out = torch.empty(n, dtype=_BF, device=self.device)
-        self._call("attn_decode_paged", self._attend, self._ref, q.data_ptr(), qs[0], qs[1], p_gate, gs[0], gs[1],
-                   pages.data_ptr(), n[0], pn[1], last.data_ptr(), n[1], out.data_ptr(), ws.data_ptr(), ws.numel())
+        if rc != 0:
+            abi.check(rc, "attn_decode_paged")
         return out
 
 
