@@ -426,7 +426,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
 
   f32x4 o[DT];
   float m, l;
-  auto step = [&]() {
+  // One tile of the wave, the next one (if there is one) asked for on the way.
+  auto step = [&](auto next) {
+    constexpr bool kNext = decltype(next)::value;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -458,13 +460,15 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     }
     Place nx = A;
     Ids ni = ai;
-    load_k(C, ci);
-    if (C.k < k1 && C.u0 != A.u0) load_q(C);  // the next pair's: this one's scores are done
-    nx = C;
-    ni = ci;
-    ++C.k;
-    if (C.k < k1) C = seek(C, C.k, k1);
-    ci = ids_of(C);
+    if constexpr (kNext) {
+      load_k(C, ci);
+      if (C.u0 != A.u0) load_q(C);             // the next pair's: this one's scores are done
+      nx = C;
+      ni = ci;
+      ++C.k;
+      if (C.k < k1) C = seek(C, C.k, k1);
+      ci = ids_of(C);
+    }
     // ---- weights ----
     float top = x[0];
 #pragma unroll
@@ -532,9 +536,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         if (d & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    load_v(nx, ni);
-    A = nx;
-    ai = ni;
+    if constexpr (kNext) {
+      load_v(nx, ni);
+      A = nx;
+      ai = ni;
+    }
   };
 
   const int rec = rec_floats(G, D);
@@ -580,40 +586,49 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   };
   // ---- this wave's pairs, one after the other -------------------------------------------
   Place at = A;
-  if (A.k < k1) {
-    while (true) {
-      const int s1 = min(at.u1, k1);
+  auto begin = [&]() {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      m = -INFINITY;
-      l = 0.0f;
-      while (A.k < s1) step();
-      l += __shfl_xor(l, 16, 64);
-      l += __shfl_xor(l, 32, 64);
-      const Place done = at;
-      const bool more = A.k < k1, begun = done.u0 < k0;
-      if (more) at = A;
-      put_slot(2 * wid + (begun ? 0 : 1));
-      if (!begun && done.u1 <= k1) {                 // all of it is here
-        const float* src = slot_of(2 * wid + 1);
-        for (int i0 = lane; i0 < items; i0 += 256) {
-          u32x2 gt[4];
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    m = -INFINITY;
+    l = 0.0f;
+  };
+  auto finish = [&](const Place& done) {
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const bool begun = done.u0 < k0;
+    put_slot(2 * wid + (begun ? 0 : 1));
+    if (begun || done.u1 > k1) return;
+    // all of it is here
+    const float* src = slot_of(2 * wid + 1);
+    for (int i0 = lane; i0 < items; i0 += 256) {
+      u32x2 gt[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const Item it = item(min(i0 + 64 * u, items - 1));
-            gt[u] = gate_of(done.b, done.kvh * G + it.h, it.c);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 64 * u;
-            if (i >= items) break;
-            const Item it = item(i);
-            emit(done.b, done.kvh * G + it.h, it.c, ((const f32x4*)src)[i], src[G * D + 2 * it.h + 1], gt[u]);
-          }
-        }
+      for (int u = 0; u < 4; ++u) {
+        const Item it = item(min(i0 + 64 * u, items - 1));
+        gt[u] = gate_of(done.b, done.kvh * G + it.h, it.c);
       }
-      if (!more) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u;
+        if (i >= items) break;
+        const Item it = item(i);
+        emit(done.b, done.kvh * G + it.h, it.c, ((const f32x4*)src)[i], src[G * D + 2 * it.h + 1], gt[u]);
+      }
     }
+  };
+  if (A.k < k1) {
+    begin();
+    while (C.k < k1) {
+      const bool over = C.u0 != A.u0;                // A is the last of its pair here
+      step(std::true_type{});
+      if (over) {
+        finish(at);
+        at = A;
+        begin();
+      }
+    }
+    step(std::false_type{});                         // the wave's last tile
+    finish(at);
   }
   // ---- pairs that waves cut: every thread its items, pair by pair -------------------------
   __syncthreads();
