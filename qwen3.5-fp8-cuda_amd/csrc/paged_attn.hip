@@ -35,9 +35,9 @@
 // piece to arrive joins them.  All joins go in the order of the pieces: the result does
 // not depend on who comes last.
 //
-// Measured: 128 sequences of 500 to 6000 positions (64 / 8 heads of 128, bf16) 187 us, 6.2 TB/s;
-// one of 200001 (16 / 4 heads of 256, E4M3) 74 us, 5.7 TB/s, of 4096 12.9 us; 43 of 1 to 8000 32 us,
-// 4.2 TB/s.  With the arithmetic taken out the long ones take as long.  Short ones are a chain of
+// Measured: 128 sequences of 500 to 6000 positions (64 / 8 heads of 128, bf16) 184 us, 6.3 TB/s;
+// one of 200001 (16 / 4 heads of 256, E4M3) 73 us, 5.7 TB/s, of 4096 11.5 us; 43 of 1 to 8000 29 us,
+// 4.6 TB/s.  With the arithmetic taken out the long ones take as long.  Short ones are a chain of
 // dependent round trips: length, page ids, rows, LDS join, record, arrival, records.
 #include <algorithm>
 #include <type_traits>
