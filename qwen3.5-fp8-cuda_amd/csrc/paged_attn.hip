@@ -183,10 +183,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   using T = Tile<D, FP8>;
   constexpr int kThreads = 64 * kWaves;
   // Tiles of a pair that one workgroup takes rather than join pieces.  A wave's second tile of
-  // 256 E4M3 values takes longer than the join (1 sequence of 400 positions, 16 / 4 heads: 11.0 us
-  // in one workgroup, 9.7 in pieces; 16 of them: 11.9 and 11.4), one of 128 does not (32 / 8 heads:
-  // 8.4 and 8.6; 16 of them: 9.2 and 12.5), nor one of bf16, which has a SIMD to itself (10.4
-  // and 10.6 of 256).
+  // 256 E4M3 values takes longer than the join (1 sequence of 400 positions, 16 / 4 heads: 10.3 us
+  // in one workgroup, 8.2 in pieces; 16 of them: 11.2 and 9.9); one of 128 hardly, and pieces for all of
+  // a batch do not fit (32 / 8 heads: 7.9 and 7.6; 16 of them: 8.7 and 10.8); nor one of bf16, which has
+  // a SIMD to itself (200 positions of 256: 8.2 and 8.4; 16 of them: 9.2 and 9.7).
   constexpr int kWhole = D == 256 && kWaves == 8 ? kWaves : 2 * kWaves;
   constexpr int DT = D / 16;                         // 16-dim tiles of the output
   constexpr int KK = D / 32;                         // products of a score tile
@@ -236,8 +236,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
         share = max(4, (sum + slots - B - 1) / (slots - B));
       // Four waves have a SIMD each, eight take as long for 5 tiles as for 8; and from some length on
       // half the pieces are worth a shared SIMD (1 sequence, 32 / 8 heads of 128, E4M3: 2000 positions
-      // 10.2 us with shares of 4, 10.6 of 8, 4096 12.6 and 11.3; 16 / 4 of 256: 3000 12.3 and 13.1,
-      // 6000 15.5 and 14.5; 3 of 3000 in shares of 5: 15.6 and 14.3).
+      // 9.2 us with shares of 4, 9.4 of 8, 4096 11.3 and 10.6; 16 / 4 of 256: 3000 10.7 and 11.3,
+      // 6000 13.6 and 12.8; 3 of 3000 in shares of 5: 13.7 and 12.6).
       if (share < 8 && (share > 4 || most > D / 2)) share = 8;
     }
     if (share > 0) {
