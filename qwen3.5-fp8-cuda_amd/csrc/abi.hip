@@ -975,7 +975,7 @@ QH_EXPORT int qh_attn_prep_paged(const qh_paged_cache* cache, const qh_rope_axes
   p.q_f32 = q_f32;
   p.n_heads = n_heads;
   if (qh_launch_paged_prep(p, cache->head_dim, stream) != 0) return -1;
-  if (T == 0) return 0;
+  if (T == 0 || n_seqs == 0) return 0;
   return check_launch("qh_attn_prep_paged");
 }
 

@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(QhPagedPrepParams p, in
     src[u] += t0 * ts[u] + c0;
     next[u] = *(const u32x4*)src[u];
   }
-  // Where token t's rows go.  A row of padding, or an index outside its range: nowhere.
+  // Where token t's rows go.  A row of padding, or an index outside its range: nowhere (it looks
+  // at the table's first entry, which is there: no launch without a sequence or a page of its table).
   if (tid < nt) {
     const int t = t0 + tid, s = p.seq ? p.seq[t] : t, at = p.at[t];
     bool ok = s >= 0 && s < p.c.n_seqs && at >= 0 && at < p.c.capacity;
@@ -489,6 +490,7 @@ int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
       return -1;
     }
   }
+  if (p.c.n_seqs == 0) return 0;  // every token is left out, and there may be no table to look at
   const int rows = (p.q ? p.n_heads : 0) + 2 * p.c.n_kv, pass = 256 / (D / 8), passes = (rows + pass - 1) / pass;
   // A head a thread while that leaves no more than six workgroups a CU (16 / 4 heads of 256: 400
   // tokens, 1200 workgroups, 6.4 us against 7.1 with three heads a thread; 700 tokens, 2100, 10.7

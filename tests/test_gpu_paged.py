@@ -844,3 +844,24 @@ def test_prompts_and_next_tokens_through_the_paged_cache(fp8):
             err = (out.cpu()[b:b + 1].double() - y).abs()
             assert bool((err <= HALF_BF16 * (y.abs() + tol) + tol).all())
             assert bool(((q.cpu()[b].double() - qx[b]).abs() <= HALF_BF16 * qx[b].abs() + 2 * ARITH * ref.pair_size(qx[b], 32)).all())
+
+
+# ------------------------------------------------------------------ batches of which nothing is left
+@pytest.mark.parametrize("fp8", [False, True])
+def test_prep_of_padding_alone_without_a_sequence(fp8):
+    """A batch whose sequences have all ended: a table without rows, tokens of padding.  Nothing is written."""
+    g = gen(40)
+    T, H, kv, D, page = 5, 4, 2, 128, 8
+    parts = pool(g, 3, kv, page, D, fp8)
+    cache = on_gpu(parts)
+    none = torch.empty(0, 4, dtype=torch.int32, device=DEV)
+    q_was = randn(g, T, H, D)
+    q_out = q_was.to(DEV)
+    k, v = bf(randn(g, T, kv, D)).to(DEV), bf(randn(g, T, kv, D)).to(DEV)
+    at = torch.tensor([-1, 0, 7, 31, 2**31 - 1], dtype=torch.int32, device=DEV)
+    seq = torch.tensor([-1, 0, 1, 2**31 - 1, -2**31], dtype=torch.int32, device=DEV)
+    assert cache.prep(k, v, none, at, seq=seq, q=bf(randn(g, T, H, D)).to(DEV), q_out=q_out) is q_out
+    torch.cuda.synchronize()
+    assert torch.equal(q_out.cpu(), q_was)
+    for got, was in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), parts):
+        assert got is None or torch.equal(got.cpu().view(torch.uint8), was.view(torch.uint8))

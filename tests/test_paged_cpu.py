@@ -212,3 +212,16 @@ def test_axes_of_pairs():
     assert ref.axes_of(8, [4, 2, 2], True) == [0, 1, 2, 0, 1, 2, 0, 0]
     a = ref.axes_of(32, [11, 11, 10], True)
     assert [a.count(i) for i in range(3)] == [11, 11, 10]
+
+
+@pytest.mark.parametrize("pages", [None, P[10]])
+def test_prep_without_sequences_launches_nothing(pages):
+    """Every token of a batch without sequences is left out: there is no table to look anything up in
+    (an empty tensor's address is null)."""
+    assert prep(n_seqs=0, pages=pages) == 0, abi.last_error()
+    assert prep(c=cache(fp8=1, k_scale=P[2], v_scale=P[3]), r=rope(), n_seqs=0, pages=pages) == 0, abi.last_error()
+    # what no call may bring is refused all the same
+    for bad, said in ((dict(k=None), "null pointer"), (dict(seq=None), "one per sequence"), (dict(k_ts=1025), "multiples of 8"),
+                      (dict(r=rope(rot=24, sections=(12,))), "rot=24")):
+        assert prep(n_seqs=0, pages=pages, **bad) == -1
+        assert said in abi.last_error()
