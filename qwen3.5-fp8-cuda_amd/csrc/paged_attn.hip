@@ -178,6 +178,14 @@ __device__ __forceinline__ int small_quotient_s(int a, int b) {  // of numbers t
   return __builtin_amdgcn_readfirstlane(small_quotient(a, b));
 }
 
+// Between a wave's LDS accesses to what other lanes of it wrote, or will write: the hardware takes
+// a wave's accesses in order, this keeps the compiler from reordering them (no instruction, no wait).
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int D, bool FP8, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhPagedAttnParams p) {
   using T = Tile<D, FP8>;
@@ -597,8 +605,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     const bool begun = done.u0 < k0;
+    wave_lds_order();                                // the last pair's slot has been read
     put_slot(2 * wid + (begun ? 0 : 1));
     if (begun || done.u1 > k1) return;
+    wave_lds_order();
     // all of it is here
     const float* src = slot_of(2 * wid + 1);
     for (int i0 = lane; i0 < items; i0 += 256) {
