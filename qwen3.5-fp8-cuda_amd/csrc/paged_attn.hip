@@ -19,8 +19,10 @@
 //     16 bytes or so of each of its 8 positions' rows (whole rows of 128 to 512 bytes to a
 //     16-lane group) and gathers the same element of all 8 by byte permutes.
 // E4M3 rows widen exactly to bf16; their scales multiply the score (K) and the weight
-// (V).  Weights enter the product as the sum of two bf16 numbers (2^-17 of them is
-// lost, as against 2^-9 with one, for matrix instructions that have time to spare).
+// (V).  Weights enter the product as the sum of two bf16 numbers: what is lost is up to
+// 2^-16 of a weight over bf16 rows, whose first part is cut off, not rounded, and 2^-17 over
+// E4M3 rows (one bf16 number: 2^-8; a third part that loses nothing: 1 to 2 % of the time of
+// every call, for outputs that are rounded by 2^-8).
 // Scores, maxima, sums and outputs are fp32.  The maximum follows with a slack of 2^8:
 // weights up to 256 lose nothing in fp32, and a tile whose scores stay below that
 // needs no exchange between lanes and no rescaling.
@@ -50,6 +52,7 @@ namespace {
 constexpr int kTile = 32;    // positions per wave and step
 constexpr int kMaxWG = 256;  // workgroups that hold a share (one per CU)
 constexpr int kMaxG = 16;
+constexpr float kAbove = 1.00000011920928955f;  // 1 + 2^-23
 // Waves of a workgroup: two to a SIMD; one where a tile of bf16 rows of 256 fills the
 // registers (16 / 4 heads, 300 positions: 11.9 us with four waves, 16.6 with eight), or where
 // the LDS has no room for the partial results of eight.
@@ -504,8 +507,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     u32x4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      hi[i] = pack_bf2(w[2 * i], w[2 * i + 1]);
-      lo[i] = pack_bf2(w[2 * i] - bf_lo(hi[i]), w[2 * i + 1] - bf_hi(hi[i]));
+      if constexpr (FP8) {
+        hi[i] = pack_bf2(w[2 * i], w[2 * i + 1]);
+        lo[i] = pack_bf2(w[2 * i] - bf_lo(hi[i]), w[2 * i + 1] - bf_hi(hi[i]));
+      } else {  // both parts above zero, or an infinity of V would meet a zero or its own negative
+        hi[i] = __builtin_amdgcn_perm(__float_as_uint(w[2 * i + 1]), __float_as_uint(w[2 * i]), 0x07060302u);
+        lo[i] = pack_bf2(fmaf(w[2 * i], kAbove, -bf_lo(hi[i])), fmaf(w[2 * i + 1], kAbove, -bf_hi(hi[i])));
+      }
     }
     // ---- outputs ----
     if (__any(left < 8)) {   // what lies in a masked place may be anything: its weight of 0 must meet a 0

@@ -865,3 +865,25 @@ def test_prep_of_padding_alone_without_a_sequence(fp8):
     assert torch.equal(q_out.cpu(), q_was)
     for got, was in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), parts):
         assert got is None or torch.equal(got.cpu().view(torch.uint8), was.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ infinities that are seen
+@pytest.mark.parametrize("lens", [(1, 2, 40), (300, 33), (6000,)])     # in a wave, in a workgroup, in pieces
+@pytest.mark.parametrize("H,kv,D", [(8, 2, 256), (16, 2, 128)])
+def test_attend_hands_on_a_visible_infinity_of_v(H, kv, D, lens):
+    """An infinity in a visible row of V is the output's in its dimension, of the heads of its KV head,
+    with its sign; all else is as it was.  Scores stay within a few units, so no weight vanishes."""
+    g = gen(41 + D + lens[0])
+    page, B = 16, len(lens)
+    table, n_pages = tables(g, lens, page)
+    parts = pool(g, n_pages, kv, page, D, False)
+    q, last = bf(randn(g, B, H, D)), torch.tensor(lens, dtype=torch.int32) - 1
+    ws = paged.attn_workspace(H, kv, D)
+    clean = check_attend(parts, on_gpu(parts), q, table, last, ws=ws).cpu()
+    for b, n in enumerate(lens):
+        for j, d, x in ((0, 5, math.inf), (n // 2, D // 2 + 1, -math.inf), (n - 1, D - 1, math.inf)):
+            parts[1][int(table[b, j // page]), 1, j % page, d] = x
+    out = on_gpu(parts).attend(q.to(DEV), table.to(DEV), last.to(DEV), ws).cpu()
+    want = clean.clone()
+    want[:, H // 2:, 5], want[:, H // 2:, D // 2 + 1], want[:, H // 2:, D - 1] = math.inf, -math.inf, math.inf
+    assert torch.equal(out, want)
