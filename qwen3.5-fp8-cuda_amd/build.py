@@ -4,7 +4,9 @@ Replaces the reference's compile.bat (nvcc -> two Windows DLLs): one shared
 library exporting both the reference's ctypes symbols and the native qh_*
 entry points.  Objects are compiled in parallel; the library is written next
 to this file so it travels with the source tree, as is the extension module
-_paged_host.so (csrc/paged_host.cpp, host code against torch's headers).
+_paged_host.so (csrc/paged_host.cpp, host code against torch's headers).  The
+library needs hipcc alone: it is linked whether the module builds or not, and
+where there is no torch the module is left out.
 
     python build.py [--jobs N] [--debug]
 """
@@ -56,8 +58,12 @@ def compile_one(cc, src, obj, extra):
 
 
 def build_host(extra):
-    """The extension module that checks and launches the paged cache's calls."""
-    import torch
+    """The extension module that checks and launches the paged cache's calls: its path, or None
+    without a torch to build it against."""
+    try:
+        import torch
+    except ImportError:
+        return None
     root = os.path.dirname(torch.__file__)
     tmp = HOST_PATH + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", *extra,
@@ -66,10 +72,14 @@ def build_host(extra):
            "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "paged_host.cpp"), "-o", tmp,
            "-L", os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"paged_host.cpp failed: {e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"paged_host.cpp failed:\n{r.stderr}")
     os.replace(tmp, HOST_PATH)
+    return HOST_PATH
 
 
 def build(jobs=None, debug=False, verbose=True):
@@ -81,8 +91,8 @@ def build(jobs=None, debug=False, verbose=True):
     objs = [os.path.join(objdir, os.path.basename(s)[:-4] + ".o") for s in srcs]
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 4)))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        futs = [ex.submit(build_host, extra)]
-        futs += [ex.submit(compile_one, cc, s, o, extra) for s, o in zip(srcs, objs)]
+        host = ex.submit(build_host, extra)
+        futs = [ex.submit(compile_one, cc, s, o, extra) for s, o in zip(srcs, objs)]
         for f in futs:
             f.result()
     tmp = LIB_PATH + ".tmp"
@@ -95,6 +105,8 @@ def build(jobs=None, debug=False, verbose=True):
     os.replace(tmp, LIB_PATH)
     if verbose:
         print(f"built {LIB_PATH} ({len(srcs)} sources, {ARCH})")
+    if host.result() is None and verbose:
+        print("no torch: without _paged_host.so, which PagedKVCache needs")
     return LIB_PATH
 
 
