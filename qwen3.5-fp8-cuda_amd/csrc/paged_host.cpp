@@ -63,6 +63,10 @@ struct Args {
 constexpr int64_t kMaxInt = 0x7FFFFFFF;
 bool is_int(int64_t n) { return n <= kMaxInt; }
 
+// An axis's stride; 0 where nothing is read at it (torch gives an axis of size 1 any stride, the entry
+// points take multiples of 8).
+int64_t step(const at::Tensor& t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
+
 PyObject* status(bool good, int rc) {
   if (PyErr_Occurred()) return nullptr;
   if (!good) Py_RETURN_NONE;
@@ -120,8 +124,8 @@ PyObject* prep(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     if (v[9] != Py_None) {
       if (const at::Tensor* q = a.rows(9, T, -1, D)) {
         H = q->size(1);
-        qs = q->stride(0);
-        qh = q->stride(1);
+        qs = step(*q, 0);
+        qh = step(*q, 1);
         qp = q->data_ptr();
         f32 = THPVariable_Check(v[10]) && THPVariable_Unpack(v[10]).scalar_type() == at::kFloat;
         out = a.dense(10, f32 ? at::kFloat : at::kBFloat16, {T, H, D});
@@ -135,7 +139,7 @@ PyObject* prep(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
       const int64_t n_seqs = table.size(0), max_pages = table.size(1);
       if (!is_int(n_seqs) || !is_int(max_pages)) Py_RETURN_NONE;
       const void *kp = k->data_ptr(), *vp = vv->data_ptr();
-      const int64_t ks = k->stride(0), vs = vv->stride(0);
+      const int64_t ks = step(*k, 0), vs = step(*vv, 0);
       Py_BEGIN_ALLOW_THREADS
       rc = entry(cache, rope, qp, qs, qh, kp, ks, vp, vs, wq, wk, eps, pos, seq, where, (int)T, pages, (int)n_seqs,
                  (int)max_pages, out, f32, (int)H, stream);
@@ -200,7 +204,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
       const int64_t max_pages = THPVariable_Unpack(v[4]).size(1), ws_bytes = THPVariable_Unpack(v[6]).size(0);
       if (!is_int(max_pages)) Py_RETURN_NONE;
       const void *qp = q->data_ptr(), *gp = gate ? gate->data_ptr() : nullptr;
-      const int64_t qs = q->stride(0), qh = q->stride(1), gs = gate ? gate->stride(0) : 0, gh = gate ? gate->stride(1) : 0;
+      const int64_t qs = step(*q, 0), qh = step(*q, 1), gs = gate ? step(*gate, 0) : 0, gh = gate ? step(*gate, 1) : 0;
       Py_BEGIN_ALLOW_THREADS
       rc = entry(cache, qp, qs, qh, gp, gs, gh, pages, (int)B, (int)max_pages, last, (int)H, out, ws, (size_t)ws_bytes,
                  stream);

@@ -126,10 +126,10 @@ class PagedKVCache:
 
     def prep(self, k, v, pages, at, seq=None, q=None, q_out=None, rope=None, pos=None, q_norm=None, k_norm=None,
              eps=1e-6):
-        """Write T tokens: k, v bf16 [T, n_kv, D] (heads dense, any token stride) to
+        """Write T tokens: k, v bf16 [T, n_kv, D] (heads dense, any token stride of 8 n) to
         position at[t] (int32 [T]) of sequence seq[t] (int32 [T]; None: token t is
         sequence t's), pages int32 [n_seqs, max_pages].  q bf16 [T, n_heads, D] (any
-        strides, for instance the q half of interleaved q | gate rows) goes through the
+        strides of 8 n, for instance the q half of interleaved q | gate rows) goes through the
         same norm and rotation to q_out [T, n_heads, D], bf16 (what `attend` takes; the
         default) or fp32 (what qh_attn_prefill takes).  rope: RopeAxes with pos int32
         [axes, T] (or [T] for one axis).  A token with an index out of range (padding:
@@ -196,7 +196,7 @@ class PagedKVCache:
     def attend(self, q, pages, last, ws, gate=None, out=None):
         """out[b, h] = softmax(q[b, h] . K^T / sqrt(D)) V over positions 0 .. last[b]
         (int32 [B]) of sequence b, times sigmoid(gate[b, h]) with a gate; zeros for an
-        empty sequence (last[b] < 0).  q, gate: bf16 [B, n_heads, D], any strides, q as
+        empty sequence (last[b] < 0).  q, gate: bf16 [B, n_heads, D], any strides of 8 n, q as
         `prep` wrote it; ws: ``attn_workspace`` (calls that share one must not overlap).
         Returns out, bf16 [B, n_heads, D]."""
         if out is None:

@@ -156,3 +156,28 @@ def test_a_call_with_other_arguments_raises():
     with pytest.raises(TypeError):
         call(_paged_host.prep, "qh_attn_prep_paged", {**a, "eps": "small"}.values())
     del keep
+
+
+def odd(*shape):
+    """A bf16 tensor whose axes of size 1 have odd strides."""
+    t = torch.zeros(shape, dtype=BF)
+    return t.as_strided(shape, [s if n > 1 else 2 * s + 7 for n, s in zip(shape[:-1], t.stride()[:-1])] + [1])
+
+
+@pytest.mark.parametrize("n,heads", [(1, H), (T, 1), (1, 1)])
+def test_the_stride_of_an_axis_of_one_is_not_handed_on(n, heads):
+    """One token or one head: nothing is read at that axis's stride, whatever it is."""
+    a, keep = prep_args()
+    zi = torch.zeros(n, dtype=INT)
+    q, k, v = odd(n, heads, D), odd(n, KV, D), odd(n, KV, D)
+    a.update(k=k, v=v, q=q, at=zi, seq=zi, pos=torch.zeros(2, n, dtype=INT), q_out=torch.zeros(n, heads, D))
+    got, s = call(_paged_host.prep, "qh_attn_prep_paged", a.values())
+    assert got == 0
+    assert s[3:5] == (heads * D if n > 1 else 0, D if heads > 1 else 0)
+    assert s[6] == s[8] == (KV * D if n > 1 else 0)
+    assert s[2] == ptr(q) and s[5] == ptr(k) and s[7] == ptr(v)
+    a = attend_args()
+    a.update(q=q, gate=odd(n, heads, D), pages=torch.zeros(n, 4, dtype=INT), last=zi, out=torch.zeros(n, heads, D, dtype=BF))
+    got, s = call(_paged_host.attend, "qh_attn_decode_paged", a.values())
+    assert got == 0 and s[2:4] == s[5:7] == (heads * D if n > 1 else 0, D if heads > 1 else 0)
+    del keep
