@@ -887,3 +887,62 @@ def test_attend_hands_on_a_visible_infinity_of_v(H, kv, D, lens):
     want = clean.clone()
     want[:, H // 2:, 5], want[:, H // 2:, D // 2 + 1], want[:, H // 2:, D - 1] = math.inf, -math.inf, math.inf
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ batches, every instance of the attention
+def check_batch(g, lens, H, kv, D, page, fp8, gated, most=48):
+    """A batch against 64 bits, K and V random: its longest and shortest sequences, the first and last ones
+    and some in between (`most` of them), zeros and finite values in all."""
+    B = len(lens)
+    table, n_pages = tables(g, lens, page)
+    parts = pool(g, n_pages, kv, page, D, fp8)
+    q, last = bf(randn(g, B, H, D)), torch.tensor(lens, dtype=torch.int32) - 1
+    gate = bf(randn(g, B, H, D)) if gated else None
+    out = on_gpu(parts).attend(q.to(DEV), table.to(DEV), last.to(DEV), paged.attn_workspace(H, kv, D),
+                               gate=None if gate is None else gate.to(DEV)).cpu()
+    assert bool(torch.isfinite(out).all()) and bool((out[last < 0] == 0).all())
+    order = sorted(range(B), key=lambda b: lens[b])
+    some = list(dict.fromkeys([0, 1, B - 2, B - 1, *order[-4:], *order[:4], *torch.randperm(B, generator=g).tolist()]))
+    some = [b for b in some if 0 <= b < B][:most]
+    want, tol = ref.attend(q[some], *parts, table[some], last[some], None if gate is None else gate[some])
+    err, lim = (out[some].double() - want).abs(), HALF_BF16 * (want.abs() + tol) + tol
+    assert bool((err <= lim).all()), f"{float((err / lim.clamp(min=1e-30)).max()):.3f} of the bound"
+
+
+def ragged(g, B, positions):
+    """B lengths of about `positions` in all: some empty, some of whole tiles, one in sixteen many times the others."""
+    u = torch.rand(B, 3, generator=g)
+    n = (u[:, 0] * 2 * positions / B / (1 + 8 / 16)).long() + 1
+    n = torch.where(u[:, 1] < 1 / 16, 8 * n, n)
+    n = torch.where(u[:, 2] < 0.1, 0, torch.where(u[:, 2] > 0.8, (n // 32 + 1) * 32, n))
+    return n.tolist()
+
+
+@pytest.mark.parametrize("B,H,kv,D,page,fp8,gated", [
+    (65, 16, 4, 256, 16, True, True),                  # E4M3 of 256 with eight waves
+    (200, 16, 4, 256, 24, True, False),
+    (600, 16, 4, 256, 8, True, True),
+    (300, 10, 2, 256, 64, True, True),
+    (129, 12, 1, 256, 40, True, True),                 # ... with four: more than 8 heads to a KV head
+    (65, 16, 4, 256, 16, False, True),                 # bf16 of 256
+    (130, 8, 8, 256, 40, False, True),
+    (600, 4, 1, 256, 64, False, False),
+    (65, 64, 8, 128, 32, False, True),                 # bf16 of 128
+    (200, 32, 8, 128, 24, False, True),
+    (2048, 6, 2, 128, 16, False, True),
+    (65, 64, 8, 128, 32, True, True),                  # E4M3 of 128
+    (333, 16, 1, 128, 8, True, False),
+])
+def test_attend_over_more_sequences_than_lanes(B, H, kv, D, page, fp8, gated):
+    g = gen(B * 31 + H + D + page)
+    check_batch(g, ragged(g, B, 50000 * 1024 // (kv * D) if kv * D > 512 else 100000), H, kv, D, page, fp8, gated)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attend_over_batches_of_all_kinds(seed):
+    """Sequences, lengths, heads, width, page and type drawn each by itself."""
+    g = gen(1000 + seed)
+    pick = lambda *xs: xs[int(torch.randint(0, len(xs), (1,), generator=g))]    # noqa: E731
+    B, D, page, fp8 = pick(1, 2, 5, 16, 31, 64, 65, 128, 200, 500), pick(128, 256), pick(8, 16, 24, 64, 256), pick(False, True)
+    kv, G, gated = pick(1, 2, 3, 4, 8), pick(1, 2, 4, 5, 8, 9, 16), pick(False, True)
+    check_batch(g, ragged(g, B, pick(1000, 8000, 40000) * 512 // (kv * D)), kv * G, kv, D, page, fp8, gated, most=16)
