@@ -174,8 +174,7 @@ __device__ __forceinline__ int wave_imax(int v) {
 // a / b for quotients below 2^20 (the compiler's division of 32-bit numbers is three times
 // as long, and a wave that divides has nothing else to do).
 __device__ __forceinline__ int small_quotient(int a, int b) {
-  const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b)), rest = a - q * b;
-  return rest < 0 ? q - 1 : rest >= b ? q + 1 : q;
+  return qh_quotient_near(a, b, __builtin_amdgcn_rcpf((float)b));
 }
 __device__ __forceinline__ int small_quotient_s(int a, int b) {  // of numbers that the wave's lanes agree on
   return __builtin_amdgcn_readfirstlane(small_quotient(a, b));
@@ -584,7 +583,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
   const int items = G * D / 4;
   struct Item { int h, c; };
   auto item = [&](int i) {
-    const int k = (int)((i >> 2) * p.group_mul >> 20), ln = i - k * 4 * G, gg = (int)(ln * p.group_mul >> 20), rr = k / (DT / 4), d = k % (DT / 4) * 4;
+    const int k = qh_group_quotient(i >> 2, p.group_mul), ln = i - k * 4 * G, gg = qh_group_quotient(ln, p.group_mul);
+    const int rr = k / (DT / 4), d = k % (DT / 4) * 4;
     return Item{ln - gg * G, RUN * (4 * gg + rr) + (FP8 ? d : 128 * (d / 8) + d % 8)};
   };
   // Where the items need no more than half of the threads, these form groups (whole waves).
@@ -816,8 +816,7 @@ static int launch(QhPagedAttnParams p, hipStream_t st) {
 
 int qh_launch_paged_attn(QhPagedAttnParams p, int D, hipStream_t st) {
   p.group = p.n_heads / p.c.n_kv;
-  // i < 1024: floor(i group_mul / 2^20) = floor(i / group) (group_mul group - 2^20 < 16)
-  p.group_mul = ((1u << 20) + p.group - 1) / p.group;
+  p.group_mul = qh_group_mul(p.group);
   p.slots = kMaxWG / p.c.n_kv;
   const bool four = waves_of(p.group, D, p.c.ks != nullptr) == 4;
   if (D == 256) {

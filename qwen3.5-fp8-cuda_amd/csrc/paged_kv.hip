@@ -424,13 +424,9 @@ int qh_paged_view(const qh_paged_cache* c, const int* pages, int n_seqs, int max
   v.n_pages = c->n_pages;
   v.page_size = c->page_size;
   v.n_kv = c->n_kv;
-  // d = page_size, s = ceil(log2 d): m = floor(2^(31+s) / d) + 1 is below 2^32 and
-  // floor(x m / 2^(31+s)) = floor(x / d) for 0 <= x < 2^31 (m d - 2^(31+s) <= d <= 2^s)
-  const unsigned d = (unsigned)c->page_size;
-  int s = 3;
-  while ((1ull << s) < d) ++s;
-  v.div_mul = (uint32_t)((1ull << (31 + s)) / d + 1);
-  v.div_shift = s - 1;
+  const QhDiv by_page = qh_div_by((uint32_t)c->page_size);
+  v.div_mul = by_page.mul;
+  v.div_shift = by_page.shift;
   v.pages = pages;
   v.n_seqs = n_seqs;
   v.max_pages = max_pages;

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "../../include/qh_paged_types.h"
+#include "qh_paged_div.h"
 
 // A cache and the page tables of a batch, as the kernels see them.
 struct QhPagedView {
@@ -17,7 +18,7 @@ struct QhPagedView {
   int n_pages;
   int page_size;
   int n_kv;
-  uint32_t div_mul;       // x / page_size = umulhi(x, div_mul) >> div_shift for 0 <= x < 2^31
+  uint32_t div_mul;       // of a position by page_size (qh_quotient)
   int div_shift;
   const int* pages;       // [n_seqs][max_pages]
   int n_seqs;
@@ -67,7 +68,7 @@ struct QhPagedAttnParams {
   float* part;
   // what the launch derives for the kernel, which would spend its time on divisions
   int group;              // heads of a KV head
-  uint32_t group_mul;     // i / group = i * group_mul >> 20 for i < 1024
+  uint32_t group_mul;     // of i < 1024 by group (qh_group_quotient)
   int group_shift;        // log2 of the threads that take a pair's items together
   int slots;              // workgroups of each KV head
 };
@@ -85,8 +86,8 @@ int qh_launch_paged_attn(QhPagedAttnParams p, int D, hipStream_t st);
 void qh_set_error(const char* fmt, ...);
 
 #if defined(__HIPCC__)
-// Quotient and remainder of a position by the page size.
+// The page of a position, counted in the sequence's table.
 __device__ __forceinline__ int page_of(const QhPagedView& c, int pos) {
-  return (int)(__umulhi((unsigned)pos, c.div_mul) >> c.div_shift);
+  return qh_quotient(pos, c.div_mul, c.div_shift);
 }
 #endif
