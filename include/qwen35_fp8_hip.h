@@ -422,7 +422,8 @@ int qh_silu_mul(const void* g, const void* u, void* m, size_t n, qh_stream_t str
  * is stored as NaN.  q null: only K and V.  Token t's head h starts at
  * q + t * q_tstride + h * q_hstride, k + t * k_tstride + h * D, v likewise
  * (elements; multiples of 8; 16-byte aligned pointers).  q_out must not overlap an
- * input.  Two tokens of one call must not name the same slot. */
+ * input.  Two tokens of one call must not name the same slot.  At most 2^26 - 64
+ * tokens and 4096 heads of a kind. */
 int qh_attn_prep_paged(const qh_paged_cache* cache, const qh_rope_axes* rope, const void* q,
                        long long q_tstride, long long q_hstride, const void* k, long long k_tstride,
                        const void* v, long long v_tstride, const float* q_norm_w,

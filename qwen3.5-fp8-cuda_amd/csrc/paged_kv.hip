@@ -85,6 +85,7 @@ __device__ __forceinline__ void put(V x, void* p) {
 }
 
 constexpr int kPrepTokens = 4;  // tokens of a workgroup, at most
+constexpr int kPrepMaxT = (1 << 26) - 64;  // 256 threads of every fourth token: fewer than 2^32 of a launch
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   const uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -437,8 +438,8 @@ int qh_paged_view(const qh_paged_cache* c, const int* pages, int n_seqs, int max
 
 int qh_launch_paged_prep(const QhPagedPrepParams& p, int D, hipStream_t st) {
   const char* what = "attn_prep_paged";
-  if (p.T < 0 || (p.q && (p.n_heads < 1 || p.n_heads > 4096)) || p.c.n_kv > 4096) {
-    qh_set_error("%s: T=%d n_heads=%d n_kv=%d (at most 4096 heads)", what, p.T, p.n_heads, p.c.n_kv);
+  if (p.T < 0 || p.T > kPrepMaxT || (p.q && (p.n_heads < 1 || p.n_heads > 4096)) || p.c.n_kv > 4096) {
+    qh_set_error("%s: T=%d n_heads=%d n_kv=%d (at most 2^26 - 64 tokens, 4096 heads)", what, p.T, p.n_heads, p.c.n_kv);
     return -1;
   }
   if (!p.seq && p.T > p.c.n_seqs) {

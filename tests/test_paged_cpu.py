@@ -225,3 +225,10 @@ def test_prep_without_sequences_launches_nothing(pages):
                       (dict(r=rope(rot=24, sections=(12,))), "rot=24")):
         assert prep(n_seqs=0, pages=pages, **bad) == -1
         assert said in abi.last_error()
+
+
+@pytest.mark.parametrize("T", [2**26 - 63, 2**31 - 1])
+def test_prep_token_limit(T):
+    """More tokens than a launch can count: k and v may be expanded views, so such a call fits the memory."""
+    assert prep(T=T, q=None, q_out=None) == -1
+    assert f"T={T}" in abi.last_error()
