@@ -23,9 +23,10 @@
 // 2^-16 of a weight over bf16 rows, whose first part is cut off, not rounded, and 2^-17 over
 // E4M3 rows (one bf16 number: 2^-8; a third part that loses nothing: 1 to 2 % of the time of
 // every call, for outputs that are rounded by 2^-8).
-// Scores, maxima, sums and outputs are fp32.  The maximum follows with a slack of 2^8:
-// weights up to 256 lose nothing in fp32, and a tile whose scores stay below that
-// needs no exchange between lanes and no rescaling.
+// Scores, maxima, sums and outputs are fp32.  Weights are 2^(s - m) with an m that a score
+// above it raises to 2^8 times that score's: none is above 1, so an output overflows no
+// sooner than the sum of the values, and a tile whose scores stay below m needs no exchange
+// between lanes and no rescaling.
 //
 // Work split: the tiles (32 positions of one KV head of one sequence) of the whole
 // batch form one line, cut into equal shares of consecutive tiles, one a wave, so ragged
@@ -485,10 +486,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    if (__any(top > m + 8.0f)) {
+    if (__any(top > m)) {
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float nm = fmaxf(m, top);
+      const float nm = top > m ? top + 8.0f : m;
       const float corr = m == -INFINITY ? 0.0f : exp2_(m - nm);
       l *= corr;
 #pragma unroll

@@ -946,3 +946,28 @@ def test_attend_over_batches_of_all_kinds(seed):
     B, D, page, fp8 = pick(1, 2, 5, 16, 31, 64, 65, 128, 200, 500), pick(128, 256), pick(8, 16, 24, 64, 256), pick(False, True)
     kv, G, gated = pick(1, 2, 3, 4, 8), pick(1, 2, 4, 5, 8, 9, 16), pick(False, True)
     check_batch(g, ragged(g, B, pick(1000, 8000, 40000) * 512 // (kv * D)), kv * G, kv, D, page, fp8, gated, most=16)
+
+
+# ------------------------------------------------------------------ values near the type's largest
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n,peak", [(64, 40), (40000, 20000), (40000, 20032), (40000, 20064)])   # tiles side by side
+def test_attend_to_values_near_the_largest(fp8, n, peak):
+    """One position of V near the largest bf16 value, the rest zeros, and its score e^5 times the others':
+    a maximum that lags behind must not carry its weight past 1, or a finite output overflows."""
+    H, kv, D, page = 8, 2, 256, 16
+    g = gen(42 + n)
+    table, n_pages = tables(g, [n], page)
+    q = bf(torch.zeros(1, H, D))
+    q[..., 0] = 16.0
+    k, v = (torch.zeros(n_pages, kv, page, D) for _ in range(2))
+    pid, off = int(table[0, peak // page]), peak % page
+    k[pid, :, off, 0] = 5.0                            # a score of 16 * 5 / sqrt(256) = 5, the others' is 0
+    v[pid, :, off] = 3.25e38 * torch.sign(torch.randn(kv, D, generator=g))
+    sc = [None, None]
+    if fp8:
+        sc = [torch.ones(n_pages, kv, page), torch.full((n_pages, kv, page), ref.MIN_SCALE)]
+        sc[1][pid, :, off] = 3.25e38 / 448
+        k, v = k.to(F8), torch.sign(v).mul(448).to(F8)
+    else:
+        k, v = bf(k), bf(v)
+    check_attend((k, v, *sc), on_gpu((k, v, *sc)), q, table, torch.tensor([n - 1], dtype=torch.int32))
