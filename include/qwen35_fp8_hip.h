@@ -446,6 +446,8 @@ size_t qh_attn_decode_paged_workspace_size(int n_heads, int n_kv, int head_dim);
  * positions 0 .. last[b] (whose rows, the new token's among them, are in the
  * cache), times sigmoid(gate) with a gate; out [n_seqs][n_heads][D] bf16, zeros for
  * a sequence with no visible position, or none whose score is above -infinity.
+ * Scores, sums and outputs are fp32; a weight enters the product with V as two bf16
+ * numbers, which lose up to 2^-16 of it (E4M3: 2^-17).
  * q (bf16, normalised and rotated) has sequence b's head h at q + b * q_bstride +
  * h * q_hstride, the gate likewise (elements; multiples of 8; 16-byte aligned
  * pointers); out must not overlap them.  n_heads / n_kv <= 16, at most 2048

@@ -245,10 +245,15 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void paged_attn_kernel(QhP
       share = max(4, (sum + slots - 1) / slots);
       if (__builtin_amdgcn_readlane(wave_scan(small_quotient(tl + share - 1, share)), 63) > slots)
         share = max(4, (sum + slots - B - 1) / (slots - B));
-      // Four waves have a SIMD each, eight take as long for 5 tiles as for 8; and from some length on
-      // half the pieces are worth a shared SIMD (1 sequence, 32 / 8 heads of 128, E4M3: 2000 positions
-      // 9.2 us with shares of 4, 9.4 of 8, 4096 11.3 and 10.6; 16 / 4 of 256: 3000 10.7 and 11.3,
-      // 6000 13.6 and 12.8; 3 of 3000 in shares of 5: 13.7 and 12.6).
+      // Four waves have a SIMD each, eight take as long for 5 tiles as for 8 (2 sequences of 4096, 16 / 4
+      // heads of 256, E4M3, in shares of 5 and of 8: 13.6 and 12.7 us); and from some length on half the
+      // pieces are worth a shared SIMD, the sooner the narrower the rows.  One sequence, shares of 4 and of 8:
+      //   16 / 4 of 256, E4M3: 3000 positions 10.8 and 11.3 us, 4096 11.8 and 11.8, 5000 12.8 and 12.5
+      //   ... bf16:            3000 12.5 and 13.2, 4096 13.9 and 13.6, 5000 15.3 and 14.5
+      //   32 / 8 of 128, E4M3: 1500 8.7 and 9.4, 2000 9.2 and 9.5, 2500 9.9 and 9.7, 3000 10.3 and 10.1
+      //   ... bf16:            2000 9.2 and 9.9, 2500 9.9 and 10.1, 3000 10.4 and 10.4, 4096 11.8 and 11.1
+      // More pairs want it earlier (2 sequences of 16 / 4 of 256, E4M3: 2500 11.6 and 11.8, 3500 12.9 and
+      // 12.3), fewer later (8 / 2: 5000 11.7 and 12.1, 6000 12.4 and 12.3): up to 5 % beside the border.
       if (share < 8 && (share > 4 || most > D / 2)) share = 8;
     }
     if (share > 0) {

@@ -15,9 +15,11 @@
 // q and bf16 rows in fp32 with one rounding at the end: the intermediate bf16 roundings
 // of the dense path (which the reference's tensors have) would be rounded again to three
 // mantissa bits here, and a second rounding moves a value in 16 to another code.
-// E4M3 codes are those of the exact quotient: V's is one of bf16 numbers, rounded to
-// fp32 correctly, which keeps the ties between two codes that such quotients often are;
-// K's, in which the factor rsqrt(..) cancels, is computed in 64 bits (as fast as 32 here).
+// E4M3 codes of V are those of the exact quotient: it is one of bf16 numbers, often a tie between
+// two codes and otherwise further from one than fp32's correct rounding moves it.  K's quotient, in
+// which the factor rsqrt(..) cancels, is computed in 64 bits (as fast as 32 here) and rounded to fp32
+// then, which puts back the ties that the reciprocal moved; its code may be the exact quotient's
+// neighbour where that lies within 2^-24 of itself from the border between the two.
 #include <algorithm>
 #include <type_traits>
 
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(QhPagedReadParams p) {
       if (!ok[u]) continue;
       const size_t o = ((size_t)pair * p.max_seq + p0 + mine + u * (256 / LPR)) * D + c;
       if constexpr (FP8) {
-auto four = [](uint32_t x, float s) {
+        auto four = [](uint32_t x, float s) {
           const qh_f32x2 lo = e4m3x2_lo_f32(x), hi = e4m3x2_hi_f32(x);
           return u32x2{pack_bf2(lo.x * s, lo.y * s), pack_bf2(hi.x * s, hi.y * s)};
         };

@@ -131,7 +131,9 @@ class PagedKVCache:
         sequence t's), pages int32 [n_seqs, max_pages].  q bf16 [T, n_heads, D] (any
         strides of 8 n, for instance the q half of interleaved q | gate rows) goes through the
         same norm and rotation to q_out [T, n_heads, D], bf16 (what `attend` takes; the
-        default) or fp32 (what qh_attn_prefill takes).  rope: RopeAxes with pos int32
+        default) or fp32 (what qh_attn_prefill takes: not rounded behind the norm, so it multiplies
+        the low halves of all dimensions, 13 % longer at 3700 tokens than for the dense path's q, which is
+        bf16 in the dimensions that are not turned).  rope: RopeAxes with pos int32
         [axes, T] (or [T] for one axis).  A token with an index out of range (padding:
         -1) is left out altogether.  Returns q_out."""
         if q is not None and q_out is None:
