@@ -462,6 +462,33 @@ int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, long long q
                          const int* last, int n_heads, void* out, void* ws, size_t ws_bytes,
                          qh_stream_t stream);
 
+/* ---- a serving step of several requests ------------------------------------
+ * No counterparts in the reference, which serves one request (main.py:1509-1604). */
+
+/* The next step of a batch planned on the device.  Row b holds length[b] positions on the
+ * first ceil(length[b] / page_size) pages of its table pages [n_rows][max_pages]; the free
+ * pages are free_pages[0 .. *n_free), of which the last is taken first.
+ *   - rows with done[b] != 0 (done null: none) put their pages behind the free ones, row after
+ *     row, and hold nothing;
+ *   - row b asks for new_tokens[b] tokens (below 0: none) and the pages that they need.  Rows
+ *     are served in order while the free pages and T token rows last; from a row whose pages
+ *     are not there, rows that need pages get nothing, from one whose tokens have no room no
+ *     row does.  A row that all free pages, all T rows or its table could not serve alone gets
+ *     nothing and is not counted;
+ *   - with seq: token i of row b is flat row start[b] + i, seq its row, at its position;
+ *     seq = at = -1 behind the last token, start [n_rows + 1].  Without (null; start null,
+ *     T = n_rows): at[b] is the position of row b's token or -1, new_tokens > 0 count as 1;
+ *   - last[b] (null: not wanted): the row's newest position, -1 where it holds nothing.
+ * length_out [n_rows] and n_free_out [1] may be length and n_free themselves; other buffers
+ * must not overlap.  A length outside [0, max_pages * page_size] or a *n_free outside
+ * [0, n_pages] counts as the nearest inside; page ids are handed on unread, and none is written
+ * outside free_pages [n_pages] or its row's table.  At most 2048 rows, 2^31 - 65536 positions a
+ * row and 2^26 - 64 tokens; page_size a positive multiple of 8. */
+int qh_page_tables_step(int* pages, int n_rows, int max_pages, int page_size, const int* length,
+                        const int* new_tokens, const int* done, int* free_pages, int n_pages,
+                        const int* n_free, int* length_out, int* n_free_out, int* at, int* seq, int T,
+                        int* start, int* last, qh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

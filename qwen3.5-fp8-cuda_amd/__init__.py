@@ -11,9 +11,10 @@ Modules:
   config  model shape (config.json keys)
   synth   seeded synthetic weights, reference block quantizer
   paged   paged KV cache for several sequences: write, read back, decode attention
+  tables  page tables of a batch whose sequences come and go, planned on the GPU
   engine  decode engine: per-token launch sequence and HIP-graph replay
   build   hipcc build of the shared library
 """
-from . import abi, config, ops, paged, synth  # noqa: F401
+from . import abi, config, ops, paged, synth, tables  # noqa: F401
 
-__all__ = ["abi", "config", "ops", "paged", "synth", "engine"]
+__all__ = ["abi", "config", "ops", "paged", "synth", "tables", "engine"]

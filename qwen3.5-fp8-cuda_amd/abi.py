@@ -116,6 +116,7 @@ NATIVE_SIGNATURES = {
     "qh_kv_read_paged": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
     "qh_attn_decode_paged_workspace_size": (_sz, [_i, _i, _i]),
     "qh_attn_decode_paged": (_i, [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _vp, _i, _vp, _vp, _sz, _vp]),
+    "qh_page_tables_step": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
 }
 
 
@@ -166,6 +167,11 @@ def check(rc, what=""):
     if rc != 0:
         raise QhError(f"{what}: {last_error()}" if what else last_error())
     return rc
+
+
+def address(name):
+    """The address of an entry point, as the extension modules call it."""
+    return ctypes.cast(getattr(load(), name), _vp).value
 
 
 def ptr(t):

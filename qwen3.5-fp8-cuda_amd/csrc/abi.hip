@@ -21,6 +21,7 @@
 #include "qh_paged.h"
 #include "qh_prefill.h"
 #include "qh_sample.h"
+#include "qh_serve.h"
 #include "qh_kernels.h"
 #include "qh_norm.h"
 
@@ -1054,4 +1055,44 @@ QH_EXPORT int qh_attn_decode_paged(const qh_paged_cache* cache, const void* q, l
   p.part = (float*)((unsigned*)ws + kPagedMaxUnits);
   if (qh_launch_paged_attn(p, cache->head_dim, stream) != 0) return -1;
   return check_launch("qh_attn_decode_paged");
+}
+
+// ---- a serving step of several requests (no counterpart in the reference, which serves
+// one, main.py:1509-1604) ----------------------------------------------------------------
+// Pages given back and taken, positions and rows of a step's tokens.
+QH_EXPORT int qh_page_tables_step(int* pages, int n_rows, int max_pages, int page_size, const int* length,
+                                  const int* new_tokens, const int* done, int* free_pages, int n_pages,
+                                  const int* n_free, int* length_out, int* n_free_out, int* at, int* seq, int T,
+                                  int* start, int* last, hipStream_t stream) {
+  const char* what = "page_tables_step";
+  if (n_rows < 0 || n_rows > kTablesMaxRows) {
+    qh_set_error("%s: n_rows=%d (at most %d)", what, n_rows, kTablesMaxRows);
+    return -1;
+  }
+  if (page_size < 8 || page_size % 8 != 0 || max_pages < 1 || (long long)max_pages * page_size > 0x7FFF0000LL) {
+    qh_set_error("%s: max_pages=%d page_size=%d (page_size must be a positive multiple of 8, a row at most 2^31 - 65536 "
+                 "positions)", what, max_pages, page_size);
+    return -1;
+  }
+  if (n_pages < 0) {
+    qh_set_error("%s: n_pages=%d", what, n_pages);
+    return -1;
+  }
+  if (T < 0 || T > (1 << 26) - 64) {
+    qh_set_error("%s: T=%d (at most 2^26 - 64)", what, T);
+    return -1;
+  }
+  if (seq ? !start : (start || T != n_rows)) {
+    qh_set_error("%s: start belongs to seq; without seq there is one token a row (T=%d, n_rows=%d)", what, T, n_rows);
+    return -1;
+  }
+  if ((n_pages > 0 && !free_pages) || !n_free || !n_free_out || (T > 0 && !at) ||
+      (n_rows > 0 && (!pages || !length || !new_tokens || !length_out))) {
+    qh_set_error("%s: null pointer", what);
+    return -1;
+  }
+  const QhTablesParams p = {pages,   n_rows, max_pages,  page_size,  length, new_tokens, done,  free_pages, n_pages,
+                            n_free,  length_out, n_free_out, at,     seq,    T,          start, last};
+  if (qh_launch_tables(p, stream) != 0) return -1;
+  return check_launch(what);
 }
