@@ -489,6 +489,26 @@ int qh_page_tables_step(int* pages, int n_rows, int max_pages, int page_size, co
                         const int* n_free, int* length_out, int* n_free_out, int* at, int* seq, int T,
                         int* start, int* last, qh_stream_t stream);
 
+/* Workspace bytes of qh_adapters_add for at most max_tokens tokens and adapters of this rank, any K
+ * and N (0 for what it does not take). */
+size_t qh_adapters_workspace_size(int max_tokens, int rank);
+
+/* Low-rank adapters of many requests beside a projection that they share: out[t] = y[t] +
+ * scale[i] * b[i] (a[i] x[t]) with i = ids[t]; out[t] = y[t] where ids[t] is outside
+ * [0, n_adapters).  a [n_adapters][rank][K], b [n_adapters][N][rank], x, y (what the projection
+ * gave) and out are bf16, scale fp32; products and sums are fp32, a x enters the second product
+ * as two bf16 numbers, which lose up to 2^-16 of it, and the output is rounded once.  Tokens may
+ * come in any order; one request's adapter never reaches another's rows, whatever it holds.
+ * Token t has x + t * x_tstride, y and out likewise (elements; multiples of 8; 16-byte aligned
+ * pointers).  out may be y itself (then rows without an adapter are not touched), and must not
+ * overlap anything else.  rank (at most 128), K and N are multiples of 8; an adapter of a smaller
+ * rank has rows and columns of zeros.  At most 2^20 - 64 tokens.  ws: 256-byte aligned; calls that
+ * share one must not overlap. */
+int qh_adapters_add(const void* a, const void* b, const float* scale, int n_adapters, int rank, int K,
+                    int N, const void* x, long long x_tstride, const int* ids, int T, const void* y,
+                    long long y_tstride, void* out, long long out_tstride, void* ws, size_t ws_bytes,
+                    qh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

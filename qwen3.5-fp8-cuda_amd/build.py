@@ -107,7 +107,7 @@ def build(jobs=None, debug=False, verbose=True):
     if verbose:
         print(f"built {LIB_PATH} ({len(srcs)} sources, {ARCH})")
     if None in [h.result() for h in hosts] and verbose:
-        print("no torch: without _paged_host.so and _serve_host.so, which PagedKVCache and PageTables need")
+        print("no torch: without _paged_host.so and _serve_host.so, which PagedKVCache, PageTables and Adapters need")
     return LIB_PATH
 
 

@@ -1096,3 +1096,51 @@ QH_EXPORT int qh_page_tables_step(int* pages, int n_rows, int max_pages, int pag
   if (qh_launch_tables(p, stream) != 0) return -1;
   return check_launch(what);
 }
+
+QH_EXPORT size_t qh_adapters_workspace_size(int max_tokens, int rank) {
+  if (max_tokens < 0 || max_tokens > kAdaptersMaxTokens || rank < 8 || rank > kAdaptersMaxRank || rank % 8 != 0) return 0;
+  return qh_adapters_ws_bytes(max(max_tokens, 1), rank);
+}
+
+// out = y + scale B A x by the adapter of each token.
+QH_EXPORT int qh_adapters_add(const void* a, const void* b, const float* scale, int n_adapters, int rank, int K, int N,
+                              const void* x, long long x_tstride, const int* ids, int T, const void* y,
+                              long long y_tstride, void* out, long long out_tstride, void* ws, size_t ws_bytes,
+                              hipStream_t stream) {
+  const char* what = "adapters_add";
+  if (n_adapters < 1 || rank < 8 || rank > kAdaptersMaxRank || rank % 8 != 0 || K < 8 || K % 8 != 0 || N < 8 || N % 8 != 0) {
+    qh_set_error("%s: n_adapters=%d rank=%d K=%d N=%d (rank, K and N must be positive multiples of 8, rank at most %d)", what,
+                 n_adapters, rank, K, N, kAdaptersMaxRank);
+    return -1;
+  }
+  if (T < 0 || T > kAdaptersMaxTokens) {
+    qh_set_error("%s: T=%d (at most %d)", what, T, kAdaptersMaxTokens);
+    return -1;
+  }
+  if (T == 0) return 0;
+  if (!a || !b || !scale || !x || !ids || !y || !out || !ws) {
+    qh_set_error("%s: null pointer", what);
+    return -1;
+  }
+  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)x | (uintptr_t)y | (uintptr_t)out) % 16 != 0 || x_tstride % 8 ||
+      y_tstride % 8 || out_tstride % 8) {
+    qh_set_error("%s: pointers must be 16-byte aligned and strides multiples of 8", what);
+    return -1;
+  }
+  if (out == x || (out == y && T > 1 && out_tstride != y_tstride) || (T > 1 && llabs(out_tstride) < N)) {
+    qh_set_error("%s: out must not alias x or overlap itself; it may be y, with its stride (out %lld, y %lld, N=%d)", what,
+                 out_tstride, y_tstride, N);
+    return -1;
+  }
+  const size_t need = qh_adapters_ws_bytes(T, rank);
+  if (ws_bytes < need || (uintptr_t)ws % 256 != 0) {
+    qh_set_error("%s: workspace of %zu bytes must be 256-byte aligned and at least qh_adapters_workspace_size (%zu)", what,
+                 ws_bytes, need);
+    return -1;
+  }
+  const QhAdaptersParams p = {(const uint16_t*)a, (const uint16_t*)b, scale,          n_adapters, rank,           K,
+                              N,                  (const uint16_t*)x, x_tstride,      ids,        T,              (const uint16_t*)y,
+                              y_tstride,          (uint16_t*)out,     out_tstride,    (float*)ws};
+  if (qh_launch_adapters(p, stream) != 0) return -1;
+  return check_launch(what);
+}

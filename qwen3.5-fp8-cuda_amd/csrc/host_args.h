@@ -48,6 +48,13 @@ struct Args {
                       (t->stride(2) == 1 || t->numel() == 0);
     return fits ? t : fail();
   }
+  // bf16 [n, width] with a dense last axis (n, width -1: any).
+  const at::Tensor* matrix(int i, int64_t n, int64_t width) {
+    const at::Tensor* t = tensor(i, at::kBFloat16, 2);
+    if (!t) return nullptr;
+    const bool fits = (n < 0 || t->size(0) == n) && (width < 0 || t->size(1) == width) && (t->stride(1) == 1 || t->numel() == 0);
+    return fits ? t : fail();
+  }
   template <typename T>
   T address(int i) {
     return reinterpret_cast<T>(PyLong_AsVoidPtr(v[i]));

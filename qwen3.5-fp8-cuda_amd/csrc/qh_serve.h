@@ -1,5 +1,5 @@
 // Launch descriptors of what a serving step needs around the paged cache: its page
-// tables and slot maps (tables.hip).
+// tables and slot maps (tables.hip), the adapters of its requests (adapters.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -27,6 +27,28 @@ struct QhTablesParams {
 };
 
 constexpr int kTablesMaxRows = 2048;
+
+struct QhAdaptersParams {
+  const uint16_t* a;      // [n][R][K] bf16
+  const uint16_t* b;      // [n][N][R] bf16
+  const float* scale;     // [n]
+  int n, R, K, N;
+  const uint16_t* x;      // token t at x + t * x_ts
+  long long x_ts;
+  const int* ids;         // [T] adapter of each token; outside [0, n): none
+  int T;
+  const uint16_t* y;
+  long long y_ts;
+  uint16_t* out;          // may be y itself
+  long long out_ts;
+  float* h;               // workspace [slices][T][rank rounded up to 16]
+};
+
+constexpr int kAdaptersMaxRank = 128;
+constexpr int kAdaptersMaxTokens = (1 << 20) - 64;  // 16 to a workgroup along one axis of the grid
+
+size_t qh_adapters_ws_bytes(int max_tokens, int R);
+int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st);
 
 int qh_launch_tables(const QhTablesParams& p, hipStream_t st);
 void qh_set_error(const char* fmt, ...);

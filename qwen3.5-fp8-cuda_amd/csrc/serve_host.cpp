@@ -1,4 +1,4 @@
-// The host side of a serving step's calls (tables.py): checks the torch tensors of a call and
+// The host side of a serving step's calls (tables.py, adapters.py): checks the torch tensors of a call and
 // launches it.  Each function takes the address of the C entry point and the call's tensors; it
 // returns the entry point's status, or None where a tensor is not what the call takes: the
 // Python caller then finds out which, for the message.
@@ -51,7 +51,45 @@ PyObject* step_tables(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   });
 }
 
+// add(entry, device, a, b, scale, x, ids, y, ws, out, stream)
+PyObject* add_adapters(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  if (!takes(nargs, 11)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    Args args{v};
+    const auto entry = args.address<decltype(&qh_adapters_add)>(0);
+    args.dev = (int)PyLong_AsLong(v[1]);
+    void* stream = args.address<void*>(10);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor* at = args.tensor(2, at::kBFloat16, 3);
+    const int64_t n = at ? at->size(0) : 0, R = at ? at->size(1) : 0, K = at ? at->size(2) : 0;
+    const void* a = args.dense(2, at::kBFloat16, {-1, -1, -1});
+    const at::Tensor* bt = args.tensor(3, at::kBFloat16, 3);
+    const int64_t N = bt ? bt->size(1) : 0;
+    const void* b = args.dense(3, at::kBFloat16, {n, N, R});
+    const float* scale = (const float*)args.dense(4, at::kFloat, {n});
+    const at::Tensor* x = args.matrix(5, -1, K);
+    const int64_t T = x ? x->size(0) : 0;
+    const int* ids = (const int*)args.dense(6, at::kInt, {T});
+    const at::Tensor* y = args.matrix(7, T, N);
+    void* ws = args.dense(8, at::kByte, {-1});
+    const at::Tensor* out = args.matrix(9, T, N);
+    int rc = 0;
+    args.good = args.good && is_int(n) && is_int(R) && is_int(K) && is_int(N) && is_int(T);
+    if (args.good) {
+      const void *xp = x->data_ptr(), *yp = y->data_ptr();
+      void* op = out->data_ptr();
+      const int64_t xs = step(*x, 0), ys = step(*y, 0), os = step(*out, 0);
+      const size_t ws_bytes = (size_t)THPVariable_Unpack(v[8]).size(0);
+      Py_BEGIN_ALLOW_THREADS
+      rc = entry(a, b, scale, (int)n, (int)R, (int)K, (int)N, xp, xs, ids, (int)T, yp, ys, op, os, ws, ws_bytes, stream);
+      Py_END_ALLOW_THREADS
+    }
+    return status(args.good, rc);
+  });
+}
+
 PyMethodDef methods[] = {
+    {"add", (PyCFunction)(void (*)(void))add_adapters, METH_FASTCALL, "Check the tensors of Adapters.add and launch it."},
     {"step", (PyCFunction)(void (*)(void))step_tables, METH_FASTCALL, "Check the tensors of PageTables.step and launch it."},
     {nullptr, nullptr, 0, nullptr},
 };

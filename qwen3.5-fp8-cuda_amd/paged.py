@@ -39,6 +39,23 @@ def _host():
     return _paged_host
 
 
+def _serve_host():
+    """The extension module that checks and launches a serving step's calls (csrc/serve_host.cpp)."""
+    try:
+        from . import _serve_host
+    except ImportError as e:
+        raise ImportError("_serve_host.so does not load: build it with `python qwen3.5-fp8-cuda_amd/build.py`") from e
+    return _serve_host
+
+
+def _with_device(dev, fn, *args):
+    """Launch with `dev` as the current device."""
+    if _current_device() == dev:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _need(t, name, dtype, shape, dev, contiguous=True):
     """Raise unless t is a `dtype` tensor of `shape` (None: any size) on GPU `dev`."""
     if t.dtype != dtype:
@@ -119,10 +136,7 @@ class PagedKVCache:
 
     def _call(self, fn, *args):
         """Launch with the cache's device as the current one."""
-        if _current_device() == self.dev:
-            return fn(*args)
-        with torch.cuda.device(self.dev):
-            return fn(*args)
+        return _with_device(self.dev, fn, *args)
 
     def prep(self, k, v, pages, at, seq=None, q=None, q_out=None, rope=None, pos=None, q_norm=None, k_norm=None,
              eps=1e-6):

@@ -13,16 +13,7 @@ back, so a step can be captured in a HIP graph: what changes between replays is 
 import torch
 
 from . import abi
-from .paged import _INT, _current_device, _need, _raw_stream
-
-
-def _host():
-    """The extension module that checks and launches the calls (csrc/serve_host.cpp)."""
-    try:
-        from . import _serve_host
-    except ImportError as e:
-        raise ImportError("_serve_host.so does not load: build it with `python qwen3.5-fp8-cuda_amd/build.py`") from e
-    return _serve_host
+from .paged import _INT, _need, _raw_stream, _serve_host, _with_device
 
 
 class PageTables:
@@ -43,7 +34,7 @@ class PageTables:
         self.pages, self.length, self.free, self.n_free = pages, length, free, n_free
         self.page_size, self.n_rows, self.dev, self.device = int(page_size), len(pages), dev, pages.device
         self._entry = abi.address("qh_page_tables_step")
-        self._step = _host().step
+        self._step = _serve_host().step
 
     @classmethod
     def alloc(cls, n_rows, max_pages, n_pages, page_size, device="cuda"):
@@ -72,13 +63,8 @@ class PageTables:
         n_free_out, int32 of the same sizes, those two go there instead."""
         length_out = self.length if length_out is None else length_out
         n_free_out = self.n_free if n_free_out is None else n_free_out
-        args = (self._entry, self.dev, self.pages, self.page_size, self.length, new, done, self.free, self.n_free,
-                length_out, n_free_out, at, seq, start, last, _raw_stream(self.dev))
-        if _current_device() == self.dev:
-            rc = self._step(*args)
-        else:
-            with torch.cuda.device(self.dev):
-                rc = self._step(*args)
+        rc = _with_device(self.dev, self._step, self._entry, self.dev, self.pages, self.page_size, self.length, new, done,
+                          self.free, self.n_free, length_out, n_free_out, at, seq, start, last, _raw_stream(self.dev))
         if rc is None:
             self._refuse(new, at, seq, done, start, last, length_out, n_free_out)
         if rc != 0:
