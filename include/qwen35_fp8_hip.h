@@ -509,6 +509,31 @@ int qh_adapters_add(const void* a, const void* b, const float* scale, int n_adap
                     long long y_tstride, void* out, long long out_tstride, void* ws, size_t ws_bytes,
                     qh_stream_t stream);
 
+/* Workspace bytes of qh_sample_rows for at most so many rows of this vocabulary (0 for what it does
+ * not take).  It grows with both; a call may bring a larger one. */
+size_t qh_sample_rows_workspace_size(int rows, int vocab);
+
+/* A token for each row of logits (row b at logits + b * row_stride elements, bf16, or fp32 with
+ * logits_f32), by the row's settings and its random number u[b] of [0, 1).  With weights
+ * w_i = exp((x_i - max x) / temperature), in the order of falling logits, equal ones by index:
+ *   top_k  the first top_k are kept (0 or below, or vocab and above: all);
+ *   top_p  of those, the ones before which less than top_p of their weight lies (1 or above: all);
+ *   min_p  of those, the ones with w_i >= min_p (0 or below: all);
+ * the first is kept always.  token[b] is the first kept index whose running sum of kept weights, in
+ * index order, is above u[b] times the whole; with temperature 0 or below (or NaN) the first of the
+ * largest logits.  logprob[b] (null: not wanted): the logarithm of the token's weight over those of
+ * all logits, before any filter; at temperature 1 where that is 0 or below.  A logit that is NaN
+ * counts as -infinity; a row with nothing above -infinity has token -1 and logprob -infinity; with
+ * +infinity in it, those logits alone have weights.  temperature, top_k, top_p, min_p null: 1, all,
+ * all, all (with the last three null one launch does).  Sums are of 64 bits; a weight is exact to
+ * 2^-36 and below 2^-63.75 of the largest it is none.  The same call gives the same tokens.
+ * rows at most 65535, vocab at most 2^20.  ws: 256-byte aligned, zeroed once when it is allocated
+ * (the kernels return its counters to zero); calls that share one must not overlap. */
+int qh_sample_rows(const void* logits, long long row_stride, int logits_f32, int rows, int vocab,
+                   const float* u, const float* temperature, const int* top_k, const float* top_p,
+                   const float* min_p, int64_t* token, float* logprob, void* ws, size_t ws_bytes,
+                   qh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,9 +13,10 @@ Modules:
   paged   paged KV cache for several sequences: write, read back, decode attention
   tables  page tables of a batch whose sequences come and go, planned on the GPU
   adapters  low-rank adapters of many requests beside a shared projection
+  sampling  a token for each row of a batch's logits
   engine  decode engine: per-token launch sequence and HIP-graph replay
   build   hipcc build of the shared library
 """
-from . import abi, adapters, config, ops, paged, synth, tables  # noqa: F401
+from . import abi, adapters, config, ops, paged, sampling, synth, tables  # noqa: F401
 
-__all__ = ["abi", "adapters", "config", "ops", "paged", "synth", "tables", "engine"]
+__all__ = ["abi", "adapters", "config", "ops", "paged", "sampling", "synth", "tables", "engine"]

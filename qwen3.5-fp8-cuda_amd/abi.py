@@ -117,6 +117,8 @@ NATIVE_SIGNATURES = {
     "qh_attn_decode_paged_workspace_size": (_sz, [_i, _i, _i]),
     "qh_attn_decode_paged": (_i, [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _vp, _i, _vp, _vp, _sz, _vp]),
     "qh_page_tables_step": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
+    "qh_sample_rows_workspace_size": (_sz, [_i, _i]),
+    "qh_sample_rows": (_i, [_vp, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "qh_adapters_workspace_size": (_sz, [_i, _i]),
     "qh_adapters_add": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _ll, _vp, _i, _vp, _ll, _vp, _ll, _vp, _sz, _vp]),
 }

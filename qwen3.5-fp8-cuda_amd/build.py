@@ -107,7 +107,8 @@ def build(jobs=None, debug=False, verbose=True):
     if verbose:
         print(f"built {LIB_PATH} ({len(srcs)} sources, {ARCH})")
     if None in [h.result() for h in hosts] and verbose:
-        print("no torch: without _paged_host.so and _serve_host.so, which PagedKVCache, PageTables and Adapters need")
+        print("no torch: without _paged_host.so and _serve_host.so, which paged.py, tables.py, adapters.py and "
+              "sampling.py need")
     return LIB_PATH
 
 

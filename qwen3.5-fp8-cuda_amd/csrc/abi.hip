@@ -1144,3 +1144,39 @@ QH_EXPORT int qh_adapters_add(const void* a, const void* b, const float* scale, 
   if (qh_launch_adapters(p, stream) != 0) return -1;
   return check_launch(what);
 }
+
+QH_EXPORT size_t qh_sample_rows_workspace_size(int rows, int vocab) {
+  if (rows < 0 || rows > kSampleRowsMaxRows || vocab < 1 || vocab > kSampleRowsMaxVocab) return 0;
+  return qh_sample_rows_ws_bytes(max(rows, 1), vocab);
+}
+
+// A token for each row of logits with the row's own temperature, top-k, top-p and min-p.
+QH_EXPORT int qh_sample_rows(const void* logits, long long row_stride, int logits_f32, int rows, int vocab, const float* u,
+                             const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                             int64_t* token, float* logprob, void* ws, size_t ws_bytes, hipStream_t stream) {
+  const char* what = "sample_rows";
+  if (rows < 0 || rows > kSampleRowsMaxRows || vocab < 1 || vocab > kSampleRowsMaxVocab) {
+    qh_set_error("%s: rows=%d vocab=%d (at most %d rows of 1 to %d logits)", what, rows, vocab, kSampleRowsMaxRows,
+                 kSampleRowsMaxVocab);
+    return -1;
+  }
+  if (rows == 0) return 0;
+  if (!logits || !u || !token || !ws) {
+    qh_set_error("%s: null pointer", what);
+    return -1;
+  }
+  if ((uintptr_t)logits % (logits_f32 ? 4 : 2) != 0) {
+    qh_set_error("%s: logits must be aligned to their size", what);
+    return -1;
+  }
+  const size_t need = qh_sample_rows_ws_bytes(rows, vocab);
+  if (ws_bytes < need || (uintptr_t)ws % 256 != 0) {
+    qh_set_error("%s: workspace of %zu bytes must be 256-byte aligned and at least qh_sample_rows_workspace_size (%zu)", what,
+                 ws_bytes, need);
+    return -1;
+  }
+  const QhSampleRowsParams p = {logits, row_stride, logits_f32 != 0, rows,  vocab,   u,          temperature,
+                                top_k,  top_p,      min_p,           token, logprob, (uint8_t*)ws};
+  if (qh_launch_sample_rows(p, stream) != 0) return -1;
+  return check_launch(what);
+}

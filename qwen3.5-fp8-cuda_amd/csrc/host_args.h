@@ -48,11 +48,11 @@ struct Args {
                       (t->stride(2) == 1 || t->numel() == 0);
     return fits ? t : fail();
   }
-  // bf16 [n, width] with a dense last axis (n, width -1: any).
-  const at::Tensor* matrix(int i, int64_t n, int64_t width) {
-    const at::Tensor* t = tensor(i, at::kBFloat16, 2);
+  // [n, width] with a dense last axis (n, width -1: any).
+  const at::Tensor* matrix(int i, int64_t n, int64_t width, at::ScalarType type = at::kBFloat16) {
+    const at::Tensor* t = tensor(i, type, 2);
     if (!t) return nullptr;
-    const bool fits = (n < 0 || t->size(0) == n) && (width < 0 || t->size(1) == width) && (t->stride(1) == 1 || t->numel() == 0);
+    const bool fits = (n < 0 || t->size(0) == n) && (width < 0 || t->size(1) == width) && (t->stride(1) == 1 || t->size(1) <= 1 || t->numel() == 0);
     return fits ? t : fail();
   }
   template <typename T>

@@ -1,5 +1,6 @@
 // Launch descriptors of what a serving step needs around the paged cache: its page
-// tables and slot maps (tables.hip), the adapters of its requests (adapters.hip).
+// tables and slot maps (tables.hip), the adapters of its requests (adapters.hip), a token
+// for each row of logits (sample_rows.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -49,6 +50,27 @@ constexpr int kAdaptersMaxTokens = (1 << 20) - 64;  // 16 to a workgroup along o
 
 size_t qh_adapters_ws_bytes(int max_tokens, int R);
 int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st);
+
+struct QhSampleRowsParams {
+  const void* logits;        // row b at logits + b * stride (elements), bf16 or fp32
+  long long stride;
+  int f32;
+  int B, V;
+  const float* u;            // [B] random numbers of [0, 1)
+  const float* temperature;  // optional [B]; 0 or below: the largest
+  const int* top_k;          // optional [B]; 0 or below: all
+  const float* top_p;        // optional [B]; 1 or above: all
+  const float* min_p;        // optional [B]; 0 or below: all
+  int64_t* token;            // [B]
+  float* logprob;            // optional [B]
+  uint8_t* ws;
+};
+
+constexpr int kSampleRowsMaxVocab = 1 << 20;  // 128 workgroups a row
+constexpr int kSampleRowsMaxRows = 65535;     // the grid's second axis
+
+size_t qh_sample_rows_ws_bytes(int rows, int V);
+int qh_launch_sample_rows(const QhSampleRowsParams& p, hipStream_t st);
 
 int qh_launch_tables(const QhTablesParams& p, hipStream_t st);
 void qh_set_error(const char* fmt, ...);

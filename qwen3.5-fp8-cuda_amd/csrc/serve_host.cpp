@@ -1,5 +1,5 @@
-// The host side of a serving step's calls (tables.py, adapters.py): checks the torch tensors of a call and
-// launches it.  Each function takes the address of the C entry point and the call's tensors; it
+// The host side of a serving step's calls (tables.py, adapters.py, sampling.py): checks the torch tensors of
+// a call and launches it.  Each function takes the address of the C entry point and the call's tensors; it
 // returns the entry point's status, or None where a tensor is not what the call takes: the
 // Python caller then finds out which, for the message.
 #include "host_args.h"
@@ -88,7 +88,42 @@ PyObject* add_adapters(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   });
 }
 
+// sample(entry, device, logits, u, ws, temperature, top_k, top_p, min_p, out, logprob, stream)
+PyObject* sample_rows(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  if (!takes(nargs, 12)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    Args a{v};
+    const auto entry = a.address<decltype(&qh_sample_rows)>(0);
+    a.dev = (int)PyLong_AsLong(v[1]);
+    void* stream = a.address<void*>(11);
+    if (PyErr_Occurred()) return nullptr;
+    const bool f32 = THPVariable_Check(v[2]) && THPVariable_Unpack(v[2]).scalar_type() == at::kFloat;
+    const at::Tensor* x = a.matrix(2, -1, -1, f32 ? at::kFloat : at::kBFloat16);
+    const int64_t B = x ? x->size(0) : 0, V = x ? x->size(1) : 0;
+    const float* u = (const float*)a.dense(3, at::kFloat, {B});
+    void* ws = a.dense(4, at::kByte, {-1});
+    const float* heat = (const float*)a.dense_or_none(5, at::kFloat, {B});
+    const int* top_k = (const int*)a.dense_or_none(6, at::kInt, {B});
+    const float* top_p = (const float*)a.dense_or_none(7, at::kFloat, {B});
+    const float* min_p = (const float*)a.dense_or_none(8, at::kFloat, {B});
+    int64_t* token = (int64_t*)a.dense(9, at::kLong, {B});
+    float* logprob = (float*)a.dense_or_none(10, at::kFloat, {B});
+    int rc = 0;
+    a.good = a.good && is_int(B) && is_int(V);
+    if (a.good) {
+      const void* xp = x->data_ptr();
+      const int64_t stride = step(*x, 0);
+      const size_t ws_bytes = (size_t)THPVariable_Unpack(v[4]).size(0);
+      Py_BEGIN_ALLOW_THREADS
+      rc = entry(xp, stride, f32, (int)B, (int)V, u, heat, top_k, top_p, min_p, token, logprob, ws, ws_bytes, stream);
+      Py_END_ALLOW_THREADS
+    }
+    return status(a.good, rc);
+  });
+}
+
 PyMethodDef methods[] = {
+    {"sample", (PyCFunction)(void (*)(void))sample_rows, METH_FASTCALL, "Check the tensors of sampling.sample and launch it."},
     {"add", (PyCFunction)(void (*)(void))add_adapters, METH_FASTCALL, "Check the tensors of Adapters.add and launch it."},
     {"step", (PyCFunction)(void (*)(void))step_tables, METH_FASTCALL, "Check the tensors of PageTables.step and launch it."},
     {nullptr, nullptr, 0, nullptr},
