@@ -8,15 +8,17 @@
 // sampler (main.py:49-87) is qh_sample_top_p: one row, its bf16 roundings, its own random numbers.
 //
 // No sort: where the cuts fall is found in a histogram of the weights.
-//   1. A workgroup reads 8192 logits (once from memory, which is the bound of the whole) into 256
-//      bins of a quarter of an octave of weight below its largest, counts and weights in one 64-bit
-//      LDS atomic each.  The last workgroup of a row adds the histograms up.  Without filters it
-//      knows in whose sum the draw lies and walks through those 8192 again; with them it knows the
-//      bins (the range) in which the cuts fall.
-//   2. Launched only where a filter is given: workgroups whose chunk has logits in the range put
-//      them on the row's list; the row's last one selects the cuts on it, digit after digit of a
-//      key of value and index, adds up what is kept of each chunk and walks through one.  A list
-//      longer than its place is not written; the row itself is gone through instead.
+//   1. scan: a workgroup reads 8192 logits (once from memory, which is the bound of the whole) into
+//      256 bins of a quarter of an octave of weight below its largest, counts and weights in one
+//      64-bit LDS atomic each; only their sum where the row has no filter.
+//   2. plan: a workgroup a row adds the chunks up.  Without filters it knows in whose sum the draw
+//      lies and walks through those 8192 again; with them it knows the bins (the range) in which
+//      the cuts fall.
+//   3. list: workgroups whose chunk has logits in the range put them on the row's list.
+//   4. cut: a workgroup a row selects the cuts on its list, digit after digit of a key of value and
+//      index, adds up what is kept of each chunk and walks through one.  A list longer than its
+//      place is not written; the row itself is gone through instead.
+// The last two are launched only where a filter is given.
 //
 // Borders between tokens lie as close as the smallest weight, so weights are 64-bit: t = 4 x
 // log2(e) / T in double, floor(t) the bin, 2^((t - floor(t) - 1) / 4) from a polynomial (7.8e-14)
@@ -27,15 +29,19 @@
 
 namespace {
 
-constexpr int NT = 256;
-constexpr int kChunk = 8192;           // logits of a workgroup, 32 a thread
+constexpr int NT = 512;
+constexpr int kWaves = NT / 64;
+constexpr int kChunk = 8192;           // logits of a workgroup, 16 a thread
 constexpr int kRounds = kChunk / (8 * NT);
 constexpr int kBins = 256;
+constexpr int kCopies = 4;             // of the histogram in LDS, by lane: logits crowd in few bins
 constexpr int kList = 32768;           // places of a row's list
+constexpr int kShort = 4096;           // entries of a list that stays in LDS
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
 constexpr double kInfT = 1e300;        // t of an infinite logit: above every finite one
 constexpr uint64_t kMassMask = (1ull << 50) - 1;  // a bin: weights below bit 50, the count above
-static_assert(kMaxChunks <= NT, "a thread a chunk");
+constexpr int kNone = 0x7FFFFFFF;
+static_assert(kMaxChunks <= kBins && NT == 2 * kBins, "a thread a chunk, two a bin");
 
 struct Chunk {      // what a workgroup hands on
   double base;      // the bin of its largest logit; -infinity where there is none
@@ -44,7 +50,7 @@ struct Chunk {      // what a workgroup hands on
   int top_at;       // its first index, where the row wants it
 };
 
-struct RowPlan {    // what the first launch decides for the second
+struct RowPlan {    // what the plan says to the launches behind it
   int done;
   int lo, hi;       // the range: bins below the row's largest
   int by_k, by_p;   // which cuts fall in it
@@ -61,7 +67,7 @@ struct Ws {
   double* sure;      // [B][chunks] weights before the range
   RowPlan* plan;     // [B]
   uint64_t* list;    // [B][kList]
-  unsigned* count;   // [rows at most][4] arrivals of both launches, places taken: zero between calls
+  unsigned* taken;   // [B] places of the list that are taken
 };
 
 int n_chunks(int V) { return (V + kChunk - 1) / kChunk; }
@@ -70,13 +76,13 @@ size_t layout(int B, int V, uint8_t* base, Ws* w) {
   const size_t nc = n_chunks(V);
   size_t off = 0;
   auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) & ~(size_t)255; return base + o; };
-  uint8_t* count = take((size_t)(kSampleRowsMaxRows + 1) * 16);  // in one place for calls of any size: they stay zero
+  uint8_t* taken = take((size_t)B * 4);
   uint8_t* hist = take(B * nc * kBins * 8);
   uint8_t* chunk = take(B * nc * sizeof(Chunk));
   uint8_t* sure = take(B * nc * 8);
   uint8_t* plan = take(B * sizeof(RowPlan));
   uint8_t* list = take((size_t)B * min(kList, V) * 8);
-  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (RowPlan*)plan, (uint64_t*)list, (unsigned*)count};
+  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (RowPlan*)plan, (uint64_t*)list, (unsigned*)taken};
   return off;
 }
 
@@ -176,82 +182,109 @@ __device__ __forceinline__ void load8(const QhSampleRowsParams& p, int b, int i,
 // The first index of round r of a chunk for this thread.
 __device__ __forceinline__ int index_of(int chunk, int r) { return chunk * kChunk + (r * NT + (int)threadIdx.x) * 8; }
 
-constexpr int kIndexBits = 24;  // whole digits of 8; an index takes 20 of them
-
 // Sort key of a logit and its index: larger for a larger value, of equal ones for a smaller index.
+// The index takes `ib` bits.
 template <bool F32>
-__device__ __forceinline__ uint64_t key_of(float x, int i) {
+__device__ __forceinline__ uint64_t key_of(float x, int i, int ib) {
   const uint32_t u = __float_as_uint(x);
   uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
   if (!F32) k >>= 16;
-  return (uint64_t)k << kIndexBits | (uint64_t)((1 << kIndexBits) - 1 - i);
+  return (uint64_t)k << ib | (uint64_t)((1 << ib) - 1 - i);
 }
 template <bool F32>
-__device__ __forceinline__ float value_of(uint64_t key) {
-  uint32_t k = (uint32_t)(key >> kIndexBits);
+__device__ __forceinline__ float value_of(uint64_t key, int ib) {
+  uint32_t k = (uint32_t)(key >> ib);
   if (!F32) k = k << 16 | (k & 0x8000u ? 0u : 0xFFFFu);  // of a negative value the low bits came out inverted
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
-__device__ __forceinline__ int index_of_key(uint64_t key) {
-  return (1 << kIndexBits) - 1 - (int)(key & ((1 << kIndexBits) - 1));
-}
+__device__ __forceinline__ int index_of_key(uint64_t key, int ib) { return (1 << ib) - 1 - (int)(key & ((1 << ib) - 1)); }
 
 // ---- workgroup sums ----------------------------------------------------------------------------
-// Exclusive prefix over the threads, and the total; a fixed order of additions.
 template <typename T>
-__device__ __forceinline__ T block_excl(T v, T* s_w, T& total) {
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+__device__ __forceinline__ T wave_excl(T v, T& all) {
+  const int lane = threadIdx.x & 63;
   T x = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const T y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
-  T before = __shfl_up(x, 1, 64);
-  if (lane == 0) before = 0;
-  if (lane == 63) s_w[wid] = x;
-  __syncthreads();
-  T tot = 0, off = 0;
-#pragma unroll
-  for (int q = 0; q < NT / 64; ++q) {
-    if (q == wid) off = tot;
-    tot += s_w[q];
+  all = __shfl(x, 63, 64);
+  const T before = __shfl_up(x, 1, 64);
+  return lane == 0 ? T(0) : before;
+}
+// Exclusive prefixes over the threads of two values, and their totals; a fixed order of additions.
+template <typename A, typename B>
+__device__ __forceinline__ void block_excl(A a, B b, A* s_a, B* s_b, A& a_excl, A& a_all, B& b_excl, B& b_all) {
+  const int wid = threadIdx.x >> 6;
+  A wa;
+  B wb;
+  a_excl = wave_excl(a, wa);
+  b_excl = wave_excl(b, wb);
+  if ((threadIdx.x & 63) == 0) {
+    s_a[wid] = wa;
+    s_b[wid] = wb;
   }
   __syncthreads();
-  total = tot;
-  return off + before;
+  A at = 0, ao = 0;
+  B bt = 0, bo = 0;
+#pragma unroll
+  for (int q = 0; q < kWaves; ++q) {
+    if (q == wid) {
+      ao = at;
+      bo = bt;
+    }
+    at += s_a[q];
+    bt += s_b[q];
+  }
+  __syncthreads();
+  a_excl += ao;
+  b_excl += bo;
+  a_all = at;
+  b_all = bt;
 }
-template <typename T>
-__device__ __forceinline__ T block_total(T v, T* s_w) {
-  T total;
-  block_excl(v, s_w, total);
-  return total;
+// The total over the threads, in a fixed order.
+__device__ __forceinline__ double block_total(double v, double* s_d) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if ((threadIdx.x & 63) == 0) s_d[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int q = 0; q < kWaves; ++q) t += s_d[q];
+  __syncthreads();
+  return t;
 }
-// The least over the threads of v, the same in all.
+// The least over the threads, the same in all.
 __device__ __forceinline__ int block_min(int v, int* s_i) {
-  if (threadIdx.x == 0) *s_i = 0x7FFFFFFF;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) s_i[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (v != 0x7FFFFFFF) atomicMin(s_i, v);
+  int r = s_i[0];
+#pragma unroll
+  for (int q = 1; q < kWaves; ++q) r = min(r, s_i[q]);
   __syncthreads();
-  const int r = *s_i;
+  return r;
+}
+__device__ __forceinline__ float block_max(float v, float* s_f) {
+  v = wave_max(v);
+  if ((threadIdx.x & 63) == 0) s_f[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = s_f[0];
+#pragma unroll
+  for (int q = 1; q < kWaves; ++q) r = fmaxf(r, s_f[q]);
   __syncthreads();
   return r;
 }
 
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint64_t published(const uint64_t* p) {
-  return __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint64_t bits(double d) { return (uint64_t)__double_as_longlong(d); }
-__device__ __forceinline__ double from_bits(uint64_t u) { return __longlong_as_double((long long)u); }
-
-struct Shared {
-  uint64_t hist[kBins];
-  double d[NT / 64];
-  uint64_t u[NT / 64];
-  int i[4];
+struct Sums {  // LDS of the sums above
+  double d[2][kWaves];
+  uint64_t u[kWaves];
+  float f[kWaves];
+  int i[kWaves];
+  double at[2];
+  uint64_t n[2];
 };
 
 // ---- the draw ----------------------------------------------------------------------------------
@@ -259,43 +292,44 @@ struct Shared {
 // first index whose running sum of kept weights is above u times the whole.  kept(x, i) is a logit's
 // weight, 0 where it is not kept.
 template <bool F32, typename Kept>
-__device__ __forceinline__ int draw(const QhSampleRowsParams& p, int b, double mass, int chunks, Shared& s, Kept kept) {
-  double total;
-  const double before = block_excl(mass, s.d, total);
-  const float u = p.u[b];
+__device__ __forceinline__ int draw(const QhSampleRowsParams& p, int b, float u, double mass, int chunks, Sums& s, Kept kept,
+                                    double& total) {
+  double before, none, none_all;
+  block_excl(mass, 0.0, s.d[0], s.d[1], before, total, none, none_all);
   const double target = (u > 0.0f ? min((double)u, 1.0) : 0.0) * total;
   const bool some = (int)threadIdx.x < chunks && mass > 0.0;
-  int c = block_min(some && before + mass > target ? (int)threadIdx.x : 0x7FFFFFFF, s.i);
-  if (c == 0x7FFFFFFF) c = -block_min(some ? -(int)threadIdx.x : 0x7FFFFFFF, s.i);  // u = 1: the last
+  int c = block_min(some && before + mass > target ? (int)threadIdx.x : kNone, s.i);
+  if (c == kNone) c = -block_min(some ? -(int)threadIdx.x : kNone, s.i);  // u = 1: the last
   if (c < 0 || c >= chunks) return -1;
-  if ((int)threadIdx.x == c) s.d[0] = before;
-  __syncthreads();
-  double run = s.d[0];
-  __syncthreads();
-  int last = 0x7FFFFFFF;
+  if ((int)threadIdx.x == c) s.at[0] = before;
+  float x[kRounds][8];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
+  double w[kRounds][8], sum[kRounds] = {};
+  int last = kNone;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[r][e] = kept(x[r][e], index_of(c, r) + e);
+      sum[r] += w[r][e];
+      if (w[r][e] > 0.0) last = -(index_of(c, r) + e);
+    }
+  static_assert(kRounds == 2, "two prefixes at once");
+  double excl[2], all[2];
+  block_excl(sum[0], sum[1], s.d[0], s.d[1], excl[0], all[0], excl[1], all[1]);
+  int found = kNone;
+#pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    float x[8];
-    double w[8], sum = 0.0;
-    const int i0 = index_of(c, r);
-    load8<F32>(p, b, i0, x);
+    double at = (s.at[0] + (r ? all[0] : 0.0)) + excl[r];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = kept(x[e], i0 + e);
-      sum += w[e];
-      if (w[e] > 0.0) last = -(i0 + e);
+      at += w[r][e];
+      if (found == kNone && w[r][e] > 0.0 && at > target) found = index_of(c, r) + e;
     }
-    double all;
-    double at = run + block_excl(sum, s.d, all);
-    int found = 0x7FFFFFFF;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      at += w[e];
-      if (found == 0x7FFFFFFF && w[e] > 0.0 && at > target) found = i0 + e;
-    }
-    found = block_min(found, s.i);
-    if (found != 0x7FFFFFFF) return found;
-    run += all;
   }
+  found = block_min(found, s.i);
+  if (found != kNone) return found;
   // the sums in another order fell short of the target: the last kept
   last = block_min(last, s.i);
   return last <= 0 ? -last : -1;
@@ -313,82 +347,83 @@ __device__ __forceinline__ void finish(const QhSampleRowsParams& p, int b, int t
   p.logprob[b] = some ? (float)log((double)fx * quarter(bin) / total) : -INFINITY;
 }
 
-// ---- first launch ------------------------------------------------------------------------------
+// ---- scan ------------------------------------------------------------------------------
 template <bool F32>
 __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams p, Ws w, int chunks) {
-  __shared__ Shared s;
+  __shared__ Sums s;
+  __shared__ uint64_t s_hist[kBins * kCopies];
   const int tid = threadIdx.x, b = blockIdx.y, c = blockIdx.x;
-  const Settings set(p, b);
-  const bool filtered = set.filtered();
   const size_t row = (size_t)b * chunks;
 
   float x[kRounds][8];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
+  const Settings set(p, b);
+  const bool filtered = set.filtered();
+  for (int i = tid; i < kBins * kCopies; i += NT) s_hist[i] = 0;
   float top = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    load8<F32>(p, b, index_of(c, r), x[r]);
+  for (int r = 0; r < kRounds; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = fmaxf(top, x[r][e]);
-  }
-  s.hist[tid] = 0;
-  top = wave_max(top);
-  if ((tid & 63) == 0) s.d[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf((float)s.d[0], (float)s.d[1]), fmaxf((float)s.d[2], (float)s.d[3]));
+  top = block_max(top, s.f);
   const double base = top == INFINITY ? kInfT : floor((double)top * set.c4);
-  int top_at = 0x7FFFFFFF;
+  int top_at = kNone;
   if (set.first) {
 #pragma unroll
     for (int r = kRounds - 1; r >= 0; --r)
 #pragma unroll
       for (int e = 7; e >= 0; --e)
         if (x[r][e] == top) top_at = index_of(c, r) + e;
-    top_at = block_min(top_at, &s.i[0]);
+    top_at = block_min(top_at, s.i);
   }
   double mass = 0.0;
-  if (!set.first || p.logprob) {
+  if (filtered) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         int bin;
         uint64_t fx;
-        if (weigh(x[r][e], set.c4, base, bin, fx)) atomicAdd((unsigned long long*)&s.hist[bin], fx | 1ull << 50);
+        if (weigh(x[r][e], set.c4, base, bin, fx))
+          atomicAdd((unsigned long long*)&s_hist[bin * kCopies + (tid & (kCopies - 1))], fx | 1ull << 50);
       }
     __syncthreads();
-    const uint64_t mine = s.hist[tid];
-    if (filtered) publish(&w.hist[(row + c) * kBins + tid], mine);
-    mass = block_total((double)(mine & kMassMask) * quarter(tid), s.d);
+    if (tid < kBins) {
+      uint64_t mine = 0;
+#pragma unroll
+      for (int q = 0; q < kCopies; ++q) mine += s_hist[tid * kCopies + q];
+      w.hist[(row + c) * kBins + tid] = mine;
+      mass = (double)(mine & kMassMask) * quarter(tid);
+    }
+  } else if (!set.first || p.logprob) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        int bin;
+        uint64_t fx;
+        if (weigh(x[r][e], set.c4, base, bin, fx)) mass += (double)fx * quarter(bin);
+      }
   }
-  if (tid == 0) {
-    uint64_t* o = (uint64_t*)&w.chunk[row + c];
-    publish(o, bits(base));
-    publish(o + 1, bits(mass));
-    publish(o + 2, (uint64_t)(uint32_t)top_at << 32 | __float_as_uint(top));
-  }
-  if (!arrive_last(&w.count[4 * b], chunks, &s.i[0])) return;
-  if (tid == 0) reset_counter(&w.count[4 * b]);
+  mass = block_total(mass, s.d[0]);
+  if (tid == 0) w.chunk[row + c] = Chunk{base, mass, top, top_at};
+}
 
-  // the row's last workgroup
-  double my_base = -INFINITY, my_mass = 0.0;
-  float my_top = -INFINITY;
-  int my_at = 0x7FFFFFFF;
-  if (tid < chunks) {
-    const uint64_t* o = (const uint64_t*)&w.chunk[row + tid];
-    my_base = from_bits(published(o));
-    my_mass = from_bits(published(o + 1));
-    const uint64_t v = published(o + 2);
-    my_top = __uint_as_float((uint32_t)v);
-    my_at = (int)(v >> 32);
-  }
-  __syncthreads();
-  const float wave_top = wave_max(my_top);
-  if ((tid & 63) == 0) s.d[tid >> 6] = wave_top;
-  __syncthreads();
-  const float row_top = fmaxf(fmaxf((float)s.d[0], (float)s.d[1]), fmaxf((float)s.d[2], (float)s.d[3]));
-  __syncthreads();
-  RowPlan plan = {};
-  plan.done = 1;
+// ---- plan ----------------------------------------------------------------------------------------
+template <bool F32>
+__global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams p, Ws w, int chunks) {
+  __shared__ Sums s;
+  __shared__ uint64_t s_other[2 * kBins];
+  __shared__ double s_base[kMaxChunks];
+  const int tid = threadIdx.x, b = blockIdx.x;
+  const size_t row = (size_t)b * chunks;
+  const float u = p.u[b];
+  const Settings set(p, b);
+  const bool filtered = set.filtered();
+  Chunk mine = {-INFINITY, 0.0, -INFINITY, kNone};
+  if (tid < chunks) mine = w.chunk[row + tid];
+  const float row_top = block_max(mine.top, s.f);
   if (row_top == -INFINITY) {
     if (tid == 0) {
       p.token[b] = -1;
@@ -398,20 +433,20 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
     return;
   }
   const double row_base = row_top == INFINITY ? kInfT : floor((double)row_top * set.c4);
-  const double scaled = my_mass > 0.0 ? my_mass * quarter_far(row_base - my_base) : 0.0;
+  const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(row_base - mine.base) : 0.0;
+  auto every = [&](float v, int) {
+    int bin;
+    uint64_t fx;
+    return weigh(v, set.c4, row_base, bin, fx) ? (double)fx * quarter(bin) : 0.0;
+  };
+  double total;
   if (!filtered) {
     int token;
-    double total;
     if (set.first) {
-      token = block_min(my_top == row_top ? my_at : 0x7FFFFFFF, &s.i[0]);
-      total = block_total(scaled, s.d);
+      token = block_min(mine.top == row_top ? mine.top_at : kNone, s.i);
+      total = block_total(scaled, s.d[0]);
     } else {
-      total = block_total(scaled, s.d);
-      token = draw<F32>(p, b, scaled, chunks, s, [&](float v, int) {
-        int bin;
-        uint64_t fx;
-        return weigh(v, set.c4, row_base, bin, fx) ? (double)fx * quarter(bin) : 0.0;
-      });
+      token = draw<F32>(p, b, u, scaled, chunks, s, every, total);
     }
     if (tid == 0) {
       finish<F32>(p, b, token, set.c4, row_base, total);
@@ -420,42 +455,59 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
     return;
   }
 
-  // the row's histogram, a bin a thread
+  // the row's histogram: two threads a bin, every other chunk each, eight loads on their way at once
   uint64_t mass_fx = 0;
   int count = 0;
   {
-    double* bases = (double*)s.hist;  // of up to 128 chunks
-    if (tid < chunks) bases[tid] = my_base;
+    if (tid < chunks) s_base[tid] = mine.base;
     __syncthreads();
-    for (int q = 0; q < chunks; ++q) {
-      const double off = row_base - bases[q];  // infinite for a chunk without logits
-      if (!(off <= (double)tid)) continue;
-      const uint64_t v = published(&w.hist[(row + q) * kBins + (tid - (int)off)]);
-      mass_fx += v & kMassMask;
-      count += (int)(v >> 50);
+    const int j = tid & (kBins - 1);
+    for (int q0 = tid / kBins; q0 < chunks; q0 += 16) {
+      uint64_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int q = q0 + 2 * e;
+        const double off = q < chunks ? row_base - s_base[q] : INFINITY;  // infinite for a chunk without logits
+        const bool in = off <= (double)j;
+        v[e] = w.hist[in ? (row + q) * kBins + (j - (int)off) : row * kBins];
+        if (!in) v[e] = 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mass_fx += v[e] & kMassMask;
+        count += (int)(v[e] >> 50);
+      }
+    }
+    if (tid >= kBins) {
+      s_other[2 * j] = mass_fx;
+      s_other[2 * j + 1] = (uint64_t)count;
+      mass_fx = 0;
+      count = 0;
     }
     __syncthreads();
+    if (tid < kBins) {
+      mass_fx += s_other[2 * j];
+      count += (int)s_other[2 * j + 1];
+    }
   }
-  const double weight = (double)mass_fx * quarter(tid);
-  double total;
-  const double excl = block_excl(weight, s.d, total);
-  uint64_t n_all;
-  const uint64_t n_excl = block_excl((uint64_t)count, s.u, n_all);
-  const int none = 0x7FFFFFFF;
-  int lo = none, hi = none;
+  const double weight = tid < kBins ? (double)mass_fx * quarter(tid) : 0.0;
+  double excl;
+  uint64_t n_excl, n_all;
+  block_excl(weight, (uint64_t)count, s.d[0], s.u, excl, total, n_excl, n_all);
+  RowPlan plan = {};
+  int lo = kNone, hi = kNone;
   plan.by_k = set.k > 0 && (uint64_t)set.k < n_all;
   plan.by_p = set.by_p;
   double p_of = total;
   if (plan.by_k) {
-    lo = hi = block_min(n_excl + count >= (uint64_t)set.k ? tid : none, &s.i[0]);
-    if (tid == hi) s.d[0] = excl;
+    lo = hi = block_min(n_excl + count >= (uint64_t)set.k ? tid : kNone, s.i);
+    if (tid == hi) s.at[0] = excl;
     __syncthreads();
-    p_of = s.d[0];  // top-p's share is of these at least
-    __syncthreads();
+    p_of = s.at[0];  // top-p's share is of these at least
   }
   if (plan.by_p) {
-    lo = block_min(count > 0 && excl + weight >= set.p * p_of ? tid : none, &s.i[0]);
-    if (lo == none) lo = -block_min(count > 0 ? -tid : none, &s.i[0]);
+    lo = block_min(count > 0 && excl + weight >= set.p * p_of ? tid : kNone, s.i);
+    if (lo == kNone) lo = -block_min(count > 0 ? -tid : kNone, s.i);
     if (!plan.by_k) hi = lo;
     else lo = min(lo, hi);
   }
@@ -473,11 +525,7 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
     }
   }
   if (lo >= kBins) {  // nothing is cut
-    const int token = draw<F32>(p, b, scaled, chunks, s, [&](float v, int) {
-      int bin;
-      uint64_t fx;
-      return weigh(v, set.c4, row_base, bin, fx) ? (double)fx * quarter(bin) : 0.0;
-    });
+    const int token = draw<F32>(p, b, u, scaled, chunks, s, every, total);
     if (tid == 0) {
       finish<F32>(p, b, token, set.c4, row_base, total);
       w.plan[b].done = 1;
@@ -485,177 +533,242 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
     return;
   }
   hi = min(hi, kBins - 1);
-  plan.above = block_total(tid < lo ? weight : 0.0, s.d);
-  plan.below = block_total(tid > hi ? weight : 0.0, s.d);
-  plan.n_list = (int)block_total((uint64_t)(tid >= lo && tid <= hi ? count : 0), s.u);
-  const int n_above = (int)block_total((uint64_t)(tid < lo ? count : 0), s.u);
+  if (tid == lo) {
+    s.d[0][0] = excl;
+    s.n[0] = n_excl;
+  }
+  if (tid == hi) {
+    s.d[0][1] = excl + weight;
+    s.n[1] = n_excl + count;
+  }
+  __syncthreads();
   if (tid == 0) {
     plan.done = 0;
     plan.lo = lo;
     plan.hi = hi;
-    plan.k = set.k - n_above;
+    plan.above = s.d[0][0];
+    plan.below = total - s.d[0][1];
+    plan.n_list = (int)(s.n[1] - s.n[0]);
+    plan.k = set.k - (int)s.n[0];
     plan.top = row_top;
     plan.base = row_base;
     plan.total = total;
     w.plan[b] = plan;
+    w.taken[b] = 0;
   }
 }
 
-// ---- second launch -----------------------------------------------------------------------------
+// ---- list ----------------------------------------------------------------------------------------
 template <bool F32>
-__global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams p, Ws w, int chunks, int places) {
-  __shared__ Shared s;
-  __shared__ unsigned s_count[256];
-  __shared__ uint64_t s_kept[kMaxChunks];
+__global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams p, Ws w, int chunks, int places, int ib) {
+  __shared__ Sums s;
+  __shared__ unsigned s_n;
   const int tid = threadIdx.x, b = blockIdx.y, c = blockIdx.x;
+  const RowPlan plan = w.plan[b];
+  if (plan.done) return;
+  const size_t row = (size_t)b * chunks;
+  uint64_t* list = w.list + (size_t)b * places;
+
+  // this chunk's weight before the range, and how many of its logits are in the range
+  const double off = plan.base - w.chunk[row + c].base;
+  double sure = 0.0;
+  uint64_t n = 0;
+  if (off < (double)kBins && tid < kBins) {
+    const uint64_t v = w.hist[(row + c) * kBins + tid];
+    const int j = tid + (int)off;
+    if (j < plan.lo) sure = (double)(v & kMassMask) * quarter(j);
+    else if (j <= plan.hi) n = v >> 50;
+  }
+  double sure_excl, sure_all;
+  uint64_t n_excl, n_all;
+  block_excl(sure, n, s.d[0], s.u, sure_excl, sure_all, n_excl, n_all);
+  if (tid == 0) w.sure[row + c] = sure_all;
+  if (n_all == 0 || plan.n_list > places) return;
+  float x[kRounds][8];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
+  const Settings set(p, b);
+  if (tid == 0) s_n = atomicAdd(&w.taken[b], (unsigned)n_all);
+  __syncthreads();
+  // the range's ends as logits, a little wide: most logits need no more
+  const float x_lo = (float)((plan.base - plan.hi) / set.c4), x_hi = (float)((plan.base - plan.lo + 1.0) / set.c4);
+  const float slack = 1e-6f * fmaxf(fabsf(x_lo), fabsf(x_hi));
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (x[r][e] < x_lo - slack || x[r][e] > x_hi + slack) continue;
+      int bin;
+      uint64_t fx;
+      if (weigh(x[r][e], set.c4, plan.base, bin, fx) && bin >= plan.lo && bin <= plan.hi) {
+        const unsigned at = atomicAdd(&s_n, 1u);
+        if (at < (unsigned)places) list[at] = key_of<F32>(x[r][e], index_of(c, r) + e, ib);
+      }
+    }
+}
+
+// ---- cut -----------------------------------------------------------------------------------------
+template <bool F32>
+__global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams p, Ws w, int chunks, int places, int ib) {
+  __shared__ Sums s;
+  __shared__ uint64_t s_list[kShort];
+  __shared__ uint64_t s_mass[NT], s_kept[kMaxChunks];
+  __shared__ unsigned s_count[NT];
+  const int tid = threadIdx.x, b = blockIdx.x;
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
   const Settings set(p, b);
   const size_t row = (size_t)b * chunks;
-  uint64_t* list = w.list + (size_t)b * places;
+  const uint64_t* list = w.list + (size_t)b * places;
   const bool listed = plan.n_list <= places;
 
-  {  // this chunk's weight before the range, and its logits in the range
-    const double off = plan.base - w.chunk[row + c].base;
-    double sure = 0.0;
-    int n = 0;
-    if (off < (double)kBins) {
-      const uint64_t v = w.hist[(row + c) * kBins + tid];
-      const int j = tid + (int)off;
-      if (j < plan.lo) sure = (double)(v & kMassMask) * quarter(j);
-      else if (j <= plan.hi) n = (int)(v >> 50);
-    }
-    sure = block_total(sure, s.d);
-    n = (int)block_total((uint64_t)n, s.u);
-    if (n > 0 && listed) {
-      if (tid == 0) {
-        s.i[1] = (int)__hip_atomic_fetch_add(&w.count[4 * b + 2], (unsigned)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s.i[2] = 0;
-      }
-      __syncthreads();
-      const int first = s.i[1];
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        float x[8];
-        load8<F32>(p, b, index_of(c, r), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          int bin;
-          uint64_t fx;
-          if (weigh(x[e], set.c4, plan.base, bin, fx) && bin >= plan.lo && bin <= plan.hi) {
-            const int at = first + atomicAdd(&s.i[2], 1);
-            if (at < places) publish(&list[at], key_of<F32>(x[e], index_of(c, r) + e));
-          }
-        }
-      }
-    }
-    if (tid == 0) publish((uint64_t*)&w.sure[row + c], bits(sure));
-  }
-  if (!arrive_last(&w.count[4 * b + 1], chunks, &s.i[0])) return;
-  if (tid == 0) {
-    reset_counter(&w.count[4 * b + 1]);
-    reset_counter(&w.count[4 * b + 2]);
-  }
-
-  // The row's last workgroup.  Weights of the range in units of its first bin's, 2^-unit: whole
-  // numbers whose sum stays below 2^53.
-  int unit = 53;
-  while ((1ll << (53 - unit)) < plan.n_list) --unit;
-  const double to_units = ldexp(1.0 / quarter(plan.lo & 3), unit - 35 + (plan.lo >> 2));
+  // Weights of the range in units of its first bin's, 2^-unit: whole numbers whose sum stays below 2^53.
+  const float u = p.u[b];
+  const double sure = tid < chunks ? w.sure[row + tid] : 0.0;
+  const int n_list = plan.n_list;
+  const int unit = 53 - (n_list > 1 ? 32 - __clz(n_list - 1) : 0);
+  const double to_units = ldexp(1.0 / quarter(plan.lo & 3), unit - 35 + (plan.lo >> 2)), from_units = 1.0 / to_units;
   auto in_range = [&](float x, uint64_t& fx) {
     int bin;
     if (!weigh(x, set.c4, plan.base, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
     fx = (uint64_t)rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo));
     return true;
   };
-  // fn(key, weight) for every logit of the range
-  auto each = [&](auto fn) {
-    uint64_t fx;
-    if (listed) {
-      for (int i = tid; i < plan.n_list; i += NT) {
-        const uint64_t key = published(&list[i]);
-        if (in_range(value_of<F32>(key), fx)) fn(key, fx);
+  if (tid < chunks) s_kept[tid] = 0;
+  const bool brief = listed && n_list <= kShort;
+  if (brief) {
+    uint64_t v[kShort / NT];
+#pragma unroll
+    for (int i = 0; i < kShort / NT; ++i) v[i] = i * NT + tid < n_list ? list[i * NT + tid] : 0;
+#pragma unroll
+    for (int i = 0; i < kShort / NT; ++i)
+      if (i * NT + tid < n_list) s_list[i * NT + tid] = v[i];
+  }
+  __syncthreads();
+  // fn(key, weight) for every logit of the range (weight 0 where it is not wanted)
+  auto each = [&](bool weights, auto fn) {
+    uint64_t fx = 0;
+    if (brief) {
+      for (int i = tid; i < n_list; i += NT) {
+        const uint64_t key = s_list[i];
+        if (!weights || in_range(value_of<F32>(key, ib), fx)) fn(key, fx);
+      }
+    } else if (listed) {
+      for (int i0 = tid; i0 < n_list; i0 += 8 * NT) {
+        uint64_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = list[min(i0 + e * NT, n_list - 1)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i0 + e * NT < n_list && (!weights || in_range(value_of<F32>(v[e], ib), fx))) fn(v[e], fx);
       }
     } else {
-      for (int q = 0; q < chunks; ++q)
-        for (int r = 0; r < kRounds; ++r) {
-          float x[8];
-          load8<F32>(p, b, index_of(q, r), x);
+      for (int q = 0; q < chunks; ++q) {
+        float x[kRounds][8];
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(q, r), x[r]);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (in_range(x[e], fx)) fn(key_of<F32>(x[e], index_of(q, r) + e), fx);
-        }
-    }
-  };
-  // The least key such that the keys from it up, of those from `least` up, are `want` (a number of
-  // them, or of weight): digit after digit from the top, until one key is left.
-  auto select = [&](bool by_weight, uint64_t least, uint64_t want) {
-    uint64_t prefix = 0;
-    for (int shift = F32 ? 48 : 32;; shift -= 8) {
-      s_count[tid] = 0;
-      s.hist[tid] = 0;
-      __syncthreads();
-      each([&](uint64_t key, uint64_t fx) {
-        if (key < least || key >> (shift + 8) != prefix) return;
-        const int digit = (int)(key >> shift) & 255;
-        atomicAdd(&s_count[digit], 1u);
-        if (by_weight) atomicAdd((unsigned long long*)&s.hist[digit], fx);
-      });
-      __syncthreads();
-      const int digit = 255 - tid;
-      const uint64_t mine = by_weight ? s.hist[digit] : s_count[digit];
-      uint64_t all;
-      const uint64_t before = block_excl(mine, s.u, all);
-      const int at = block_min(s_count[digit] > 0 && before + mine >= want ? tid : 0x7FFFFFFF, &s.i[0]);
-      if (at == 0x7FFFFFFF) return least;  // all of them
-      if (tid == at) {
-        s.u[0] = before;
-        s.i[1] = (int)s_count[digit];
+            if (in_range(x[r][e], fx)) fn(key_of<F32>(x[r][e], index_of(q, r) + e, ib), fx);
       }
-      __syncthreads();
-      want -= s.u[0];
-      const int n = s.i[1];
-      __syncthreads();
-      prefix = prefix << 8 | (uint64_t)(255 - at);
-      const uint64_t cut = prefix << shift;
-      if (n == 1 || shift == 0) return cut > least ? cut : least;
     }
-  };
-  auto sum_from = [&](uint64_t least) {
-    uint64_t mine = 0;
-    each([&](uint64_t key, uint64_t fx) { mine += key >= least ? fx : 0; });
-    return block_total(mine, s.u);
   };
 
   uint64_t cut = 0;
-  if (plan.by_k) cut = select(false, 0, (uint64_t)plan.k);
-  if (plan.by_p) {
-    const double above = plan.above * to_units;
-    const double share = set.p * (above + (double)sum_from(cut) + (plan.by_k ? 0.0 : plan.below * to_units));
-    const double want = ceil(share - above);
-    cut = select(true, cut, want >= 1.0 ? (uint64_t)want : 1);
+  if (plan.by_k || plan.by_p) {
+    // what all keys have in common tells nothing: digits are of the distance from the least
+    uint64_t least = ~0ull, most = 0;
+    each(false, [&](uint64_t key, uint64_t) {
+      least = key < least ? key : least;
+      most = key > most ? key : most;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t l = __shfl_xor(least, o, 64), m = __shfl_xor(most, o, 64);
+      least = l < least ? l : least;
+      most = m > most ? m : most;
+    }
+    if ((tid & 63) == 0) {
+      s_mass[tid >> 6] = least;
+      s_mass[kWaves + (tid >> 6)] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) {
+      least = s_mass[q] < least ? s_mass[q] : least;
+      most = s_mass[kWaves + q] > most ? s_mass[kWaves + q] : most;
+    }
+    __syncthreads();
+    const int key_bits = most > least ? 64 - __clzll((long long)(most - least)) : 0;
+    // The least key such that those from it up, of the ones from `cut` up, are as many (or weigh as
+    // much) as wanted(their sum), digit after digit of nine bits, until one key is left.
+    auto select = [&](bool by_weight, auto wanted) {
+      uint64_t prefix = 0, want = 0;
+      int high = key_bits;  // the digits above are settled
+      for (int round = 0;; ++round) {
+        const int shift = max(high - 9, 0);
+        s_count[tid] = 0;
+        s_mass[tid] = 0;
+        __syncthreads();
+        each(by_weight, [&](uint64_t key, uint64_t fx) {
+          const uint64_t d = key - least;
+          if (key < cut || d >> high != prefix) return;
+          const int digit = (int)(d >> shift) & ((1 << (high - shift)) - 1);
+          atomicAdd(&s_count[digit], 1u);
+          if (by_weight) atomicAdd((unsigned long long*)&s_mass[digit], fx);
+        });
+        __syncthreads();
+        const int digit = NT - 1 - tid;
+        const uint64_t n = s_count[digit], mine = by_weight ? s_mass[digit] : n;
+        uint64_t before, all;
+        double none, none_all;
+        block_excl(mine, 0.0, s.u, s.d[0], before, all, none, none_all);
+        if (round == 0) want = wanted(all);
+        const int at = block_min(n > 0 && before + mine >= want ? tid : kNone, s.i);
+        if (at == kNone) return;  // all of them
+        if (tid == at) {
+          s.n[0] = before;
+          s.n[1] = n;
+        }
+        __syncthreads();
+        want -= s.n[0];
+        const uint64_t left = s.n[1];
+        prefix = prefix << (high - shift) | (uint64_t)(NT - 1 - at);
+        high = shift;
+        if (left == 1 || shift == 0) break;
+      }
+      const uint64_t found = least + (prefix << high);
+      cut = found > cut ? found : cut;
+    };
+    if (plan.by_k) select(false, [&](uint64_t) { return (uint64_t)plan.k; });
+    if (plan.by_p)
+      select(true, [&](uint64_t all) {
+        const double above = plan.above * to_units;
+        const double share = set.p * (above + (double)all + (plan.by_k ? 0.0 : plan.below * to_units));
+        const double want = ceil(share - above);
+        return want >= 1.0 ? (uint64_t)want : (uint64_t)1;
+      });
   }
-  auto kept = [&](uint64_t key) {
-    return key >= cut && (!set.by_m || plan.top == INFINITY ||
-                          exp(((double)value_of<F32>(key) - (double)plan.top) / set.heat) >= set.m);
+
+  auto kept = [&](float x, uint64_t key) {
+    return key >= cut && (!set.by_m || plan.top == INFINITY || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
   };
-  if (tid < chunks) s_kept[tid] = 0;
-  __syncthreads();
-  each([&](uint64_t key, uint64_t fx) {
-    if (kept(key)) atomicAdd((unsigned long long*)&s_kept[index_of_key(key) / kChunk], fx);
+  each(true, [&](uint64_t key, uint64_t fx) {
+    if (kept(value_of<F32>(key, ib), key)) atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], fx);
   });
   __syncthreads();
-  double mass = 0.0;
   // back in the units of the row's first bin: whole numbers too, of that bin's weights
-  const double from_units = 1.0 / to_units;
-  if (tid < chunks) mass = from_bits(published((const uint64_t*)&w.sure[row + tid])) + (double)s_kept[tid] * from_units;
-  const int token = draw<F32>(p, b, mass, chunks, s, [&](float x, int i) {
+  const double mass = tid < chunks ? sure + (double)s_kept[tid] * from_units : 0.0;
+  double kept_all;
+  const int token = draw<F32>(p, b, u, mass, chunks, s, [&](float x, int i) {
     int bin;
     uint64_t fx;
     if (!weigh(x, set.c4, plan.base, bin, fx) || bin > plan.hi) return 0.0;
     if (bin < plan.lo) return (double)fx * quarter(bin);
-    return kept(key_of<F32>(x, i)) ? rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo)) * from_units : 0.0;
-  });
+    return kept(x, key_of<F32>(x, i, ib)) ? rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo)) * from_units : 0.0;
+  }, kept_all);
   if (tid == 0) finish<F32>(p, b, token, set.c4, plan.base, plan.total);
 }
 
@@ -664,7 +777,12 @@ void launch(const QhSampleRowsParams& p, const Ws& w, hipStream_t st) {
   const int chunks = n_chunks(p.V);
   const dim3 grid(chunks, p.B);
   sample_rows_scan_kernel<F32><<<grid, NT, 0, st>>>(p, w, chunks);
-  if (p.top_k || p.top_p || p.min_p) sample_rows_cut_kernel<F32><<<grid, NT, 0, st>>>(p, w, chunks, min(kList, p.V));
+  sample_rows_plan_kernel<F32><<<p.B, NT, 0, st>>>(p, w, chunks);
+  if (!p.top_k && !p.top_p && !p.min_p) return;
+  int ib = 1;  // bits of an index
+  while ((1 << ib) < p.V) ++ib;
+  sample_rows_list_kernel<F32><<<grid, NT, 0, st>>>(p, w, chunks, min(kList, p.V), ib);
+  sample_rows_cut_kernel<F32><<<p.B, NT, 0, st>>>(p, w, chunks, min(kList, p.V), ib);
 }
 
 }  // namespace

@@ -31,7 +31,7 @@ def sample(logits, u, ws, temperature=None, top_k=None, top_p=None, min_p=None, 
     those of all logits, before any filter, goes (at temperature 1 for the largest logit).
 
     ws: ``sample_workspace`` for B rows and V logits or more (calls that share one must not overlap).
-    Without top_k, top_p and min_p (None, not tensors of what switches them off) one launch does."""
+    Without top_k, top_p and min_p (None, not tensors of what switches them off) two launches of four do."""
     global _entry, _sample
     if _entry is None:
         _entry, _sample = abi.address("qh_sample_rows"), _serve_host().sample
@@ -61,8 +61,8 @@ def sample(logits, u, ws, temperature=None, top_k=None, top_p=None, min_p=None, 
 
 
 def sample_workspace(rows, vocab, device="cuda"):
-    """A zeroed workspace for `sample` of up to so many rows and logits a row."""
+    """A workspace for `sample` of up to so many rows and logits a row."""
     n = int(abi.load().qh_sample_rows_workspace_size(rows, vocab))
     if n == 0:
         raise ValueError(f"sample_workspace: rows={rows} vocab={vocab} unsupported")
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device)

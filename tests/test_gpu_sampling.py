@@ -34,7 +34,8 @@ def run(x, u, settings, ws=None, **kw):
     """(tokens, logprobs) of rows x (CPU, or a GPU view) with a list of settings."""
     x = x.to(DEV) if x.device.type == "cpu" else x
     B, V = x.shape
-    ws = sampling.sample_workspace(B, V, device=DEV) if ws is None else ws
+    if ws is None:
+        ws = sampling.sample_workspace(B, V, device=DEV).fill_(0xFF)     # nothing of it is read before it is written
     lp = torch.full((B,), 7.0, device=DEV)
     tok = sampling.sample(x, torch.tensor(u, dtype=F32, device=DEV), ws, logprob=lp, **(cols(settings) if settings else {}), **kw)
     return tok.tolist(), lp.tolist()

@@ -24,7 +24,7 @@ def call(**kw):
     (dict(B=-1), "rows=-1"), (dict(B=65536), "65535"), (dict(V=0), "vocab=0"), (dict(V=2**20 + 1), "1048576"),
     (dict(x=None), "null"), (dict(u=None), "null"), (dict(token=None), "null"), (dict(ws=None), "null"),
     (dict(x=ctypes.c_void_p(4097)), "aligned"), (dict(x=ctypes.c_void_p(4098), f32=1), "aligned"),
-    (dict(ws=ctypes.c_void_p(4096 + 64)), "256-byte"), (dict(ws_bytes=1 << 20), "workspace")])
+    (dict(ws=ctypes.c_void_p(4096 + 64)), "256-byte"), (dict(ws_bytes=1000), "workspace")])
 def test_refusals(bad, said):
     assert call(**bad) == -1
     assert "sample_rows" in abi.last_error() and said in abi.last_error()
