@@ -21,9 +21,10 @@
 // The last two are launched only where a filter is given.
 //
 // Borders between tokens lie as close as the smallest weight, so weights are 64-bit: t = 4 x
-// log2(e) / T in double, floor(t) the bin, 2^((t - floor(t) - 1) / 4) from a polynomial (7.8e-14)
-// as an integer of 35 bits, which any order of atomics adds up to the same sum.  A weight is
-// 2^-36 off its value, alike wherever it is used.  Weights below 2^-63.75 of the largest are none.
+// log2(e) / T in double, its nearest integer the bin, 2^(g / 4) of what is left (|g| <= 1/2) from a
+// polynomial (1.1e-13) as an integer of 35 bits, which any order of atomics adds up to the same
+// sum.  A weight is 2^-36 off its value, alike wherever it is used.  Weights below 2^-63.75 of the
+// largest are none.
 #include "qh_common.h"
 #include "qh_serve.h"
 
@@ -38,14 +39,13 @@ constexpr int kCopies = 4;             // of the histogram in LDS, by lane: logi
 constexpr int kList = 32768;           // places of a row's list
 constexpr int kShort = 4096;           // entries of a list that stays in LDS
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
-constexpr double kInfT = 1e300;        // t of an infinite logit: above every finite one
 constexpr uint64_t kMassMask = (1ull << 50) - 1;  // a bin: weights below bit 50, the count above
 constexpr int kNone = 0x7FFFFFFF;
 static_assert(kMaxChunks <= kBins && NT == 2 * kBins, "a thread a chunk, two a bin");
 
 struct Chunk {      // what a workgroup hands on
   double base;      // the bin of its largest logit; -infinity where there is none
-  double mass;      // its weights, as multiples of a weight 2^((base + 1) / 4) / 2^35
+  double mass;      // its weights in units of that bin
   float top;        // the largest
   int top_at;       // its first index, where the row wants it
 };
@@ -56,8 +56,7 @@ struct RowPlan {    // what the plan says to the launches behind it
   int by_k, by_p;   // which cuts fall in it
   int n_list;       // logits in it
   int k;            // of which top-k keeps so many
-  float top;
-  double base;      // the row's first bin
+  float top;        // the row's largest
   double total, above, below;  // weights of all bins, of those before and behind the range
 };
 
@@ -86,6 +85,8 @@ size_t layout(int B, int V, uint8_t* base, Ws* w) {
   return off;
 }
 
+__device__ __forceinline__ uint64_t bits(double d) { return (uint64_t)__double_as_longlong(d); }
+
 // ---- a row's settings ------------------------------------------------------------------------
 struct Settings {
   double c4;       // t = x c4
@@ -111,29 +112,50 @@ struct Settings {
 };
 
 // ---- weights -----------------------------------------------------------------------------------
-constexpr double kL = 0.17328679513998632;  // ln(2) / 4
-constexpr double kA0 = 34359738368.0 * 0.9170040432046712;  // 2^35 2^(-1/8)
+// 2^(g / 4) by the polynomial through its seven Chebyshev points of [-1/2, 1/2], scaled so that g = 0
+// gives a whole number: weights of equal logits add up without a rounding.
+constexpr uint64_t kOne = 31508019007;        // about 2^35 2^(-1/8)
+constexpr double kP1 = 5459923634.982943, kP2 = 473066334.20437115, kP3 = 27325381.376510937, kP4 = 1183781.9759320344,
+                 kP5 = 41039.59278978226, kP6 = 1185.1772411226116;
+constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: added to |t| < 2^50, the sum's low bits are the nearest integer
+constexpr double kWhole = 4503599627370496.0;  // 2^52
 
-// The bin of a logit below `base` and its weight in the bin's own units (2^35: a whole quarter of an
-// octave up); false where it has none.
-__device__ __forceinline__ bool weigh(float x, double c4, double base, int& bin, uint64_t& fx) {
-  const double t = x == INFINITY ? kInfT : (double)x * c4;
-  const double q = floor(t), d = base - q;
-  if (!(d < (double)kBins)) return false;
-  const double g = (t - q) - 0.5;
-  // 2^(g / 4) by its series in g ln(2) / 4, |.| <= 0.0867
-  double e = kL * kL * kL * kL * kL * kL * kL / 5040.0 * kA0;
-  e = fma(e, g, kL * kL * kL * kL * kL * kL / 720.0 * kA0);
-  e = fma(e, g, kL * kL * kL * kL * kL / 120.0 * kA0);
-  e = fma(e, g, kL * kL * kL * kL / 24.0 * kA0);
-  e = fma(e, g, kL * kL * kL / 6.0 * kA0);
-  e = fma(e, g, kL * kL / 2.0 * kA0);
-  e = fma(e, g, kL * kA0);
-  e = fma(e, g, kA0);
-  bin = (int)d;
-  fx = (uint64_t)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFull;  // + 2^52: rounded to an integer
-  return true;
+// e + 2^52 of a weight e in its bin's units, rounded to an integer by the last addition.
+__device__ __forceinline__ double power(double g) {
+  double e = fma(kP6, g, kP5);
+  e = fma(e, g, kP4);
+  e = fma(e, g, kP3);
+  e = fma(e, g, kP2);
+  e = fma(e, g, kP1);
+  return fma(e, g, (double)kOne + kWhole);
 }
+
+// The weights below a largest logit.
+struct Scale {
+  double c4, base;  // the largest's bin
+  float top;        // the largest
+  bool far;         // |t| of it is 2^50 or more (or it is infinite): no other logit is near enough to have a weight
+  __device__ __forceinline__ Scale(double c4_, float top_) : c4(c4_), top(top_) {
+    const double t = (double)top * c4;
+    far = !(fabs(t) < 1125899906842624.0);
+    base = fabsf(top) == INFINITY ? (double)top : far ? t : (t + kRound) - kRound;
+  }
+  // The bin of a logit below `base` and its weight in the bin's units; false where it has none.
+  __device__ __forceinline__ bool weigh(float x, int& bin, uint64_t& fx) const {
+    if (far) {
+      bin = 0;
+      fx = kOne;
+      return x == top && top > -INFINITY;
+    }
+    const double tm = fma((double)x, c4, kRound), d = (kRound + base) - tm;
+    if (!(d < (double)kBins)) return false;
+    bin = (int)d;
+    fx = bits(power(fma((double)x, c4, -(tm - kRound)))) & 0xFFFFFFFFFull;
+    return true;
+  }
+};
+// Bins from a to b below it (they may be far apart, or infinite).
+__device__ __forceinline__ double below(double a, double b) { return a == b ? 0.0 : a - b; }
 // 2^(-j / 4)
 __device__ __forceinline__ double quarter(int j) {
   const double s = (j & 2 ? 0.7071067811865476 : 1.0) * (j & 1 ? 0.8408964152537145 : 1.0);
@@ -143,12 +165,10 @@ __device__ __forceinline__ double quarter(int j) {
 __device__ __forceinline__ double quarter_far(double j) { return j < 4096.0 ? quarter((int)j) : 0.0; }
 
 // ---- logits ------------------------------------------------------------------------------------
-// NaN counts as -infinity, -0 as 0.
-__device__ __forceinline__ float tidy(float x) { return x == x ? x + 0.0f : -INFINITY; }
-
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-// Eight logits from index i on (-infinity behind the row's end).
+// Eight logits from index i on (-infinity behind the row's end).  A NaN among them fails every
+// comparison on its way: it has no weight and is no maximum.
 template <bool F32>
 __device__ __forceinline__ void load8(const QhSampleRowsParams& p, int b, int i, float (&x)[8]) {
   if constexpr (F32) {
@@ -157,26 +177,26 @@ __device__ __forceinline__ void load8(const QhSampleRowsParams& p, int b, int i,
       const u32x4 v = *(const u32x4_any*)r, w = *(const u32x4_any*)(r + 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = tidy(__uint_as_float(v[e]));
-        x[4 + e] = tidy(__uint_as_float(w[e]));
+        x[e] = __uint_as_float(v[e]);
+        x[4 + e] = __uint_as_float(w[e]);
       }
       return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = i + e < p.V ? tidy(r[e]) : -INFINITY;
+    for (int e = 0; e < 8; ++e) x[e] = i + e < p.V ? r[e] : -INFINITY;
   } else {
     const uint16_t* r = (const uint16_t*)p.logits + b * p.stride + i;
     if (i + 8 <= p.V) {
       const u32x4 v = *(const u32x4_any*)r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[2 * e] = tidy(bf_lo(v[e]));
-        x[2 * e + 1] = tidy(bf_hi(v[e]));
+        x[2 * e] = bf_lo(v[e]);
+        x[2 * e + 1] = bf_hi(v[e]);
       }
       return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = i + e < p.V ? tidy(bf2f(r[e])) : -INFINITY;
+    for (int e = 0; e < 8; ++e) x[e] = i + e < p.V ? bf2f(r[e]) : -INFINITY;
   }
 }
 // The first index of round r of a chunk for this thread.
@@ -186,7 +206,7 @@ __device__ __forceinline__ int index_of(int chunk, int r) { return chunk * kChun
 // The index takes `ib` bits.
 template <bool F32>
 __device__ __forceinline__ uint64_t key_of(float x, int i, int ib) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);  // -0 is 0
   uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
   if (!F32) k >>= 16;
   return (uint64_t)k << ib | (uint64_t)((1 << ib) - 1 - i);
@@ -200,18 +220,64 @@ __device__ __forceinline__ float value_of(uint64_t key, int ib) {
 __device__ __forceinline__ int index_of_key(uint64_t key, int ib) { return (1 << ib) - 1 - (int)(key & ((1 << ib) - 1)); }
 
 // ---- workgroup sums ----------------------------------------------------------------------------
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v) {
+  static_assert(sizeof(T) == 8, "two registers");
+  const u32x2 u = __builtin_bit_cast(u32x2, v);
+  const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, false),
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, false)};
+  return __builtin_bit_cast(T, r);
+}
+template <typename T>
+__device__ __forceinline__ T lane63(T v) {
+  const u32x2 u = __builtin_bit_cast(u32x2, v);
+  const u32x2 r = {(uint32_t)__builtin_amdgcn_readlane((int)u.x, 63), (uint32_t)__builtin_amdgcn_readlane((int)u.y, 63)};
+  return __builtin_bit_cast(T, r);
+}
+// Exclusive prefix over the wave and its total (64-bit values), by moves between lanes within the
+// registers: shifts within rows of 16, then the rows' last lanes handed on.
 template <typename T>
 __device__ __forceinline__ T wave_excl(T v, T& all) {
-  const int lane = threadIdx.x & 63;
   T x = v;
+  x += dpp_or_zero<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x += dpp_or_zero<0x112, 0xF>(x);
+  x += dpp_or_zero<0x114, 0xF>(x);
+  x += dpp_or_zero<0x118, 0xF>(x);
+  x += dpp_or_zero<0x142, 0xA>(x);  // row_bcast 15 into rows 1 and 3
+  x += dpp_or_zero<0x143, 0xC>(x);  // row_bcast 31 into rows 2 and 3
+  all = lane63(x);
+  return dpp_or_zero<0x138, 0xF>(x);  // wave_shr 1
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_min(int v) {
+  return min(v, __builtin_amdgcn_update_dpp(kNone, v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ int wave_min(int v) {
+  v = dpp_min<0x111, 0xF>(v);
+  v = dpp_min<0x112, 0xF>(v);
+  v = dpp_min<0x114, 0xF>(v);
+  v = dpp_min<0x118, 0xF>(v);
+  v = dpp_min<0x142, 0xA>(v);
+  v = dpp_min<0x143, 0xC>(v);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+// Exclusive prefix over the threads, and the total; a fixed order of additions.
+template <typename T>
+__device__ __forceinline__ T block_excl(T v, T* s_v, T& all) {
+  const int wid = threadIdx.x >> 6;
+  T w;
+  T excl = wave_excl(v, w);
+  if ((threadIdx.x & 63) == 0) s_v[wid] = w;
+  __syncthreads();
+  T at = 0, off = 0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
+  for (int q = 0; q < kWaves; ++q) {
+    if (q == wid) off = at;
+    at += s_v[q];
   }
-  all = __shfl(x, 63, 64);
-  const T before = __shfl_up(x, 1, 64);
-  return lane == 0 ? T(0) : before;
+  __syncthreads();
+  all = at;
+  return off + excl;
 }
 // Exclusive prefixes over the threads of two values, and their totals; a fixed order of additions.
 template <typename A, typename B>
@@ -245,9 +311,9 @@ __device__ __forceinline__ void block_excl(A a, B b, A* s_a, B* s_b, A& a_excl, 
 }
 // The total over the threads, in a fixed order.
 __device__ __forceinline__ double block_total(double v, double* s_d) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  if ((threadIdx.x & 63) == 0) s_d[threadIdx.x >> 6] = v;
+  double w;
+  wave_excl(v, w);
+  if ((threadIdx.x & 63) == 0) s_d[threadIdx.x >> 6] = w;
   __syncthreads();
   double t = 0.0;
 #pragma unroll
@@ -257,8 +323,7 @@ __device__ __forceinline__ double block_total(double v, double* s_d) {
 }
 // The least over the threads, the same in all.
 __device__ __forceinline__ int block_min(int v, int* s_i) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  v = wave_min(v);
   if ((threadIdx.x & 63) == 0) s_i[threadIdx.x >> 6] = v;
   __syncthreads();
   int r = s_i[0];
@@ -288,70 +353,79 @@ struct Sums {  // LDS of the sums above
 };
 
 // ---- the draw ----------------------------------------------------------------------------------
+// Token and log-probability, by the thread that has the logit; `total` is the weight of all logits.
+__device__ __forceinline__ void emit(const QhSampleRowsParams& p, int b, int token, float x, const Scale& scale, double total) {
+  p.token[b] = token;
+  if (!p.logprob) return;
+  int bin;
+  uint64_t fx;
+  p.logprob[b] = scale.weigh(x, bin, fx) ? (float)log((double)fx * quarter(bin) / total) : -INFINITY;
+}
+
 // Among the chunks, thread c's weighing `mass`, and then in the one that the draw falls into: the
 // first index whose running sum of kept weights is above u times the whole.  kept(x, i) is a logit's
-// weight, 0 where it is not kept.
+// weight, 0 where it is not kept; `total` below 0: all are.
 template <bool F32, typename Kept>
-__device__ __forceinline__ int draw(const QhSampleRowsParams& p, int b, float u, double mass, int chunks, Sums& s, Kept kept,
-                                    double& total) {
-  double before, none, none_all;
-  block_excl(mass, 0.0, s.d[0], s.d[1], before, total, none, none_all);
-  const double target = (u > 0.0f ? min((double)u, 1.0) : 0.0) * total;
+__device__ __forceinline__ void draw(const QhSampleRowsParams& p, int b, float u, double mass, int chunks, Sums& s,
+                                     const Scale& scale, double total, Kept kept) {
+  double all_mass;
+  const double before = block_excl(mass, s.d[0], all_mass);
+  if (total < 0.0) total = all_mass;
+  const double target = (u > 0.0f ? min((double)u, 1.0) : 0.0) * all_mass;
   const bool some = (int)threadIdx.x < chunks && mass > 0.0;
   int c = block_min(some && before + mass > target ? (int)threadIdx.x : kNone, s.i);
   if (c == kNone) c = -block_min(some ? -(int)threadIdx.x : kNone, s.i);  // u = 1: the last
-  if (c < 0 || c >= chunks) return -1;
+  c = min(max(c, 0), chunks - 1);
   if ((int)threadIdx.x == c) s.at[0] = before;
   float x[kRounds][8];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
   double w[kRounds][8], sum[kRounds] = {};
   int last = kNone;
+  float x_last = 0.0f;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       w[r][e] = kept(x[r][e], index_of(c, r) + e);
       sum[r] += w[r][e];
-      if (w[r][e] > 0.0) last = -(index_of(c, r) + e);
+      if (w[r][e] > 0.0) {
+        last = -(index_of(c, r) + e);
+        x_last = x[r][e];
+      }
     }
   static_assert(kRounds == 2, "two prefixes at once");
   double excl[2], all[2];
   block_excl(sum[0], sum[1], s.d[0], s.d[1], excl[0], all[0], excl[1], all[1]);
   int found = kNone;
+  float x_found = 0.0f;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     double at = (s.at[0] + (r ? all[0] : 0.0)) + excl[r];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       at += w[r][e];
-      if (found == kNone && w[r][e] > 0.0 && at > target) found = index_of(c, r) + e;
+      if (found == kNone && w[r][e] > 0.0 && at > target) {
+        found = index_of(c, r) + e;
+        x_found = x[r][e];
+      }
     }
   }
-  found = block_min(found, s.i);
-  if (found != kNone) return found;
+  int token = block_min(found, s.i);
+  if (token != kNone) {
+    if (found == token) emit(p, b, token, x_found, scale, total);
+    return;
+  }
   // the sums in another order fell short of the target: the last kept
-  last = block_min(last, s.i);
-  return last <= 0 ? -last : -1;
-}
-
-template <bool F32>
-__device__ __forceinline__ void finish(const QhSampleRowsParams& p, int b, int token, double c4, double base, double total) {
-  p.token[b] = token;
-  if (!p.logprob) return;
-  int bin;
-  uint64_t fx;
-  float x = -INFINITY;
-  if (token >= 0) x = tidy(F32 ? ((const float*)p.logits)[b * p.stride + token] : bf2f(((const uint16_t*)p.logits)[b * p.stride + token]));
-  const bool some = token >= 0 && weigh(x, c4, base, bin, fx);
-  p.logprob[b] = some ? (float)log((double)fx * quarter(bin) / total) : -INFINITY;
+  token = block_min(last, s.i);
+  if (token != kNone && last == token) emit(p, b, -token, x_last, scale, total);
 }
 
 // ---- scan ------------------------------------------------------------------------------
 template <bool F32>
 __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams p, Ws w, int chunks) {
   __shared__ Sums s;
-  __shared__ uint64_t s_hist[kBins * kCopies];
+  __shared__ uint64_t s_hist[(kBins + 1) * kCopies];
   const int tid = threadIdx.x, b = blockIdx.y, c = blockIdx.x;
   const size_t row = (size_t)b * chunks;
 
@@ -367,7 +441,6 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = fmaxf(top, x[r][e]);
   top = block_max(top, s.f);
-  const double base = top == INFINITY ? kInfT : floor((double)top * set.c4);
   int top_at = kNone;
   if (set.first) {
 #pragma unroll
@@ -377,37 +450,47 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
         if (x[r][e] == top) top_at = index_of(c, r) + e;
     top_at = block_min(top_at, s.i);
   }
+  const Scale scale(set.c4, top);
   double mass = 0.0;
-  if (filtered) {
+  if (!set.first || p.logprob) {
+    unsigned long long* mine = (unsigned long long*)&s_hist[tid & (kCopies - 1)];
+    // Logits far below the largest are lifted to 400 bins below it, whose bin is one that nobody reads: no
+    // branch a logit, and no number that its bin's 32 bits do not hold.  Where that is not a number, or
+    // 24 bits of a logit do not tell bins apart, each is looked at.
+    const float least = (float)((scale.base - 400.0) / set.c4);
+    if (!scale.far && fabs(scale.base) < 67108864.0 && least > -INFINITY) {
+      const uint32_t first = (uint32_t)bits(kRound + scale.base);
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r)
+      for (int r = 0; r < kRounds; ++r)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        int bin;
-        uint64_t fx;
-        if (weigh(x[r][e], set.c4, base, bin, fx))
-          atomicAdd((unsigned long long*)&s_hist[bin * kCopies + (tid & (kCopies - 1))], fx | 1ull << 50);
-      }
+        for (int e = 0; e < 8; ++e) {
+          const double v = x[r][e] > least ? x[r][e] : least;
+          const double tm = fma(v, set.c4, kRound);
+          const uint32_t bin = min(first - (uint32_t)bits(tm), (uint32_t)kBins);
+          const uint64_t fx = bits(power(fma(v, set.c4, -(tm - kRound))));
+          atomicAdd(mine + bin * kCopies, fx + ((1ull << 50) - 0x4330000000000000ull));  // its exponent away, a count in
+        }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          int bin;
+          uint64_t fx;
+          if (scale.weigh(x[r][e], bin, fx)) atomicAdd(mine + bin * kCopies, fx | 1ull << 50);
+        }
+    }
     __syncthreads();
     if (tid < kBins) {
-      uint64_t mine = 0;
+      uint64_t v = 0;
 #pragma unroll
-      for (int q = 0; q < kCopies; ++q) mine += s_hist[tid * kCopies + q];
-      w.hist[(row + c) * kBins + tid] = mine;
-      mass = (double)(mine & kMassMask) * quarter(tid);
+      for (int q = 0; q < kCopies; ++q) v += s_hist[tid * kCopies + q];
+      if (filtered) w.hist[(row + c) * kBins + tid] = v;
+      mass = (double)(v & kMassMask) * quarter(tid);
     }
-  } else if (!set.first || p.logprob) {
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        int bin;
-        uint64_t fx;
-        if (weigh(x[r][e], set.c4, base, bin, fx)) mass += (double)fx * quarter(bin);
-      }
+    mass = block_total(mass, s.d[0]);
   }
-  mass = block_total(mass, s.d[0]);
-  if (tid == 0) w.chunk[row + c] = Chunk{base, mass, top, top_at};
+  if (tid == 0) w.chunk[row + c] = Chunk{scale.base, mass, top, top_at};
 }
 
 // ---- plan ----------------------------------------------------------------------------------------
@@ -432,26 +515,22 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
     return;
   }
-  const double row_base = row_top == INFINITY ? kInfT : floor((double)row_top * set.c4);
-  const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(row_base - mine.base) : 0.0;
+  const Scale scale(set.c4, row_top);
+  const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(below(scale.base, mine.base)) : 0.0;
   auto every = [&](float v, int) {
     int bin;
     uint64_t fx;
-    return weigh(v, set.c4, row_base, bin, fx) ? (double)fx * quarter(bin) : 0.0;
+    return scale.weigh(v, bin, fx) ? (double)fx * quarter(bin) : 0.0;
   };
-  double total;
   if (!filtered) {
-    int token;
     if (set.first) {
-      token = block_min(mine.top == row_top ? mine.top_at : kNone, s.i);
-      total = block_total(scaled, s.d[0]);
+      const int token = block_min(mine.top == row_top ? mine.top_at : kNone, s.i);
+      const double all = block_total(scaled, s.d[0]);
+      if (tid == 0) emit(p, b, token, row_top, scale, all);
     } else {
-      token = draw<F32>(p, b, u, scaled, chunks, s, every, total);
+      draw<F32>(p, b, u, scaled, chunks, s, scale, -1.0, every);
     }
-    if (tid == 0) {
-      finish<F32>(p, b, token, set.c4, row_base, total);
-      w.plan[b].done = 1;
-    }
+    if (tid == 0) w.plan[b].done = 1;
     return;
   }
 
@@ -467,7 +546,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int q = q0 + 2 * e;
-        const double off = q < chunks ? row_base - s_base[q] : INFINITY;  // infinite for a chunk without logits
+        const double off = q < chunks ? below(scale.base, s_base[q]) : INFINITY;  // infinite for a chunk without logits
         const bool in = off <= (double)j;
         v[e] = w.hist[in ? (row + q) * kBins + (j - (int)off) : row * kBins];
         if (!in) v[e] = 0;
@@ -491,7 +570,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
   }
   const double weight = tid < kBins ? (double)mass_fx * quarter(tid) : 0.0;
-  double excl;
+  double excl, total;
   uint64_t n_excl, n_all;
   block_excl(weight, (uint64_t)count, s.d[0], s.u, excl, total, n_excl, n_all);
   RowPlan plan = {};
@@ -511,9 +590,9 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     if (!plan.by_k) hi = lo;
     else lo = min(lo, hi);
   }
-  if (set.by_m && row_top != INFINITY) {
+  if (set.by_m && !scale.far) {
     // the bin of the least weight that is kept, and one on both sides
-    const double least = row_base - floor((double)row_top * set.c4 + 4.0 * log2(set.m));
+    const double least = scale.base - rint((double)row_top * set.c4 + 4.0 * log2(set.m));
     const int jm = least < (double)kBins ? (int)least : kBins;
     const int m_lo = max(jm - 1, 0), m_hi = jm + 1;
     if (m_hi < lo) {  // above the other cuts
@@ -525,11 +604,8 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
   }
   if (lo >= kBins) {  // nothing is cut
-    const int token = draw<F32>(p, b, u, scaled, chunks, s, every, total);
-    if (tid == 0) {
-      finish<F32>(p, b, token, set.c4, row_base, total);
-      w.plan[b].done = 1;
-    }
+    draw<F32>(p, b, u, scaled, chunks, s, scale, -1.0, every);
+    if (tid == 0) w.plan[b].done = 1;
     return;
   }
   hi = min(hi, kBins - 1);
@@ -551,7 +627,6 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     plan.n_list = (int)(s.n[1] - s.n[0]);
     plan.k = set.k - (int)s.n[0];
     plan.top = row_top;
-    plan.base = row_base;
     plan.total = total;
     w.plan[b] = plan;
     w.taken[b] = 0;
@@ -570,7 +645,9 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
   uint64_t* list = w.list + (size_t)b * places;
 
   // this chunk's weight before the range, and how many of its logits are in the range
-  const double off = plan.base - w.chunk[row + c].base;
+  const Settings set(p, b);
+  const Scale scale(set.c4, plan.top);
+  const double off = below(scale.base, w.chunk[row + c].base);
   double sure = 0.0;
   uint64_t n = 0;
   if (off < (double)kBins && tid < kBins) {
@@ -587,11 +664,10 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
   float x[kRounds][8];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
-  const Settings set(p, b);
   if (tid == 0) s_n = atomicAdd(&w.taken[b], (unsigned)n_all);
   __syncthreads();
   // the range's ends as logits, a little wide: most logits need no more
-  const float x_lo = (float)((plan.base - plan.hi) / set.c4), x_hi = (float)((plan.base - plan.lo + 1.0) / set.c4);
+  const float x_lo = (float)((scale.base - plan.hi - 0.75) / set.c4), x_hi = (float)((scale.base - plan.lo + 0.75) / set.c4);
   const float slack = 1e-6f * fmaxf(fabsf(x_lo), fabsf(x_hi));
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
@@ -600,7 +676,7 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
       if (x[r][e] < x_lo - slack || x[r][e] > x_hi + slack) continue;
       int bin;
       uint64_t fx;
-      if (weigh(x[r][e], set.c4, plan.base, bin, fx) && bin >= plan.lo && bin <= plan.hi) {
+      if (scale.weigh(x[r][e], bin, fx) && bin >= plan.lo && bin <= plan.hi) {
         const unsigned at = atomicAdd(&s_n, 1u);
         if (at < (unsigned)places) list[at] = key_of<F32>(x[r][e], index_of(c, r) + e, ib);
       }
@@ -618,6 +694,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
   const Settings set(p, b);
+  const Scale scale(set.c4, plan.top);
   const size_t row = (size_t)b * chunks;
   const uint64_t* list = w.list + (size_t)b * places;
   const bool listed = plan.n_list <= places;
@@ -630,7 +707,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const double to_units = ldexp(1.0 / quarter(plan.lo & 3), unit - 35 + (plan.lo >> 2)), from_units = 1.0 / to_units;
   auto in_range = [&](float x, uint64_t& fx) {
     int bin;
-    if (!weigh(x, set.c4, plan.base, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
+    if (!scale.weigh(x, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
     fx = (uint64_t)rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo));
     return true;
   };
@@ -722,9 +799,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
         __syncthreads();
         const int digit = NT - 1 - tid;
         const uint64_t n = s_count[digit], mine = by_weight ? s_mass[digit] : n;
-        uint64_t before, all;
-        double none, none_all;
-        block_excl(mine, 0.0, s.u, s.d[0], before, all, none, none_all);
+        uint64_t all;
+        const uint64_t before = block_excl(mine, s.u, all);
         if (round == 0) want = wanted(all);
         const int at = block_min(n > 0 && before + mine >= want ? tid : kNone, s.i);
         if (at == kNone) return;  // all of them
@@ -753,7 +829,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   }
 
   auto kept = [&](float x, uint64_t key) {
-    return key >= cut && (!set.by_m || plan.top == INFINITY || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
+    return key >= cut && (!set.by_m || scale.far || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
   };
   each(true, [&](uint64_t key, uint64_t fx) {
     if (kept(value_of<F32>(key, ib), key)) atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], fx);
@@ -761,15 +837,13 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   __syncthreads();
   // back in the units of the row's first bin: whole numbers too, of that bin's weights
   const double mass = tid < chunks ? sure + (double)s_kept[tid] * from_units : 0.0;
-  double kept_all;
-  const int token = draw<F32>(p, b, u, mass, chunks, s, [&](float x, int i) {
+  draw<F32>(p, b, u, mass, chunks, s, scale, plan.total, [&](float x, int i) {
     int bin;
     uint64_t fx;
-    if (!weigh(x, set.c4, plan.base, bin, fx) || bin > plan.hi) return 0.0;
+    if (!scale.weigh(x, bin, fx) || bin > plan.hi) return 0.0;
     if (bin < plan.lo) return (double)fx * quarter(bin);
     return kept(x, key_of<F32>(x, i, ib)) ? rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo)) * from_units : 0.0;
-  }, kept_all);
-  if (tid == 0) finish<F32>(p, b, token, set.c4, plan.base, plan.total);
+  });
 }
 
 template <bool F32>

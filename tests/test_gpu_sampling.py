@@ -169,6 +169,23 @@ def test_masked_logits_hold_nothing_back():
         assert tw == [t[0] + 20001] and lpw == lp
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_every_nan_is_masked(dtype):
+    """NaN of either sign and any payload, quiet and signaling."""
+    x = logits(gen(18), 16, 9000, dtype)
+    u, s = draws(random.Random(18), 16), SETTINGS
+    inner = x[:, 1000:].contiguous()
+    codes = torch.arange(0x7F81, 0x7F81 + 127).repeat(8)[:1000] | torch.where(torch.arange(1000) % 3 == 0, 0x8000, 0)
+    if dtype == BF:
+        x.view(torch.int16)[:, :1000] = codes.to(torch.int32).to(torch.int16)
+    else:
+        x.view(torch.int32)[:, :1000] = ((codes << 16) - torch.where(codes >= 0x8000, 1 << 32, 0) + torch.arange(1000)).to(torch.int32)
+    assert bool(x[:, :1000].isnan().all())
+    t, lp = run(x, u, s)
+    tw, lpw = run(inner, u, s)
+    assert t == [v + 1000 for v in tw] and lp == lpw
+
+
 def test_infinite_logits():
     """+infinity takes all the weight, shared by those that have it."""
     x = torch.randn(6, 9000, generator=gen(1))
