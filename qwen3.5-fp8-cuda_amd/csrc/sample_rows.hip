@@ -36,8 +36,8 @@ constexpr int kChunk = 8192;           // logits of a workgroup, 16 a thread
 constexpr int kRounds = kChunk / (8 * NT);
 constexpr int kBins = 256;
 constexpr int kCopies = 4;             // of the histogram in LDS, by lane: logits crowd in few bins
-constexpr int kList = 32768;           // places of a row's list
-constexpr int kShort = 4096;           // entries of a list that stays in LDS
+constexpr int kList = 65536;           // places of a row's list
+constexpr int kHeld = 20480;           // 32-bit words of LDS for it
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
 constexpr uint64_t kMassMask = (1ull << 50) - 1;  // a bin: weights below bit 50, the count above
 constexpr int kNone = 0x7FFFFFFF;
@@ -153,6 +153,20 @@ struct Scale {
     fx = bits(power(fma((double)x, c4, -(tm - kRound)))) & 0xFFFFFFFFFull;
     return true;
   }
+};
+// The logits of bins `hi` to `lo` below the largest lie between these two (a little wide): a test that
+// most logits fail without their weight.  Where all have to be looked at, all pass.
+struct Ends {
+  float lo, hi;
+  __device__ __forceinline__ Ends(const Scale& s, int bin_lo, int bin_hi) {
+    lo = (float)((s.base - bin_hi - 0.75) / s.c4);
+    hi = (float)((s.base - bin_lo + 0.75) / s.c4);
+    const float slack = 1e-6f * fmaxf(fabsf(lo), fabsf(hi));
+    lo -= slack;
+    hi += slack;
+  }
+  __device__ __forceinline__ bool below(float x) const { return x < lo; }
+  __device__ __forceinline__ bool out(float x) const { return x < lo || x > hi; }
 };
 // Bins from a to b below it (they may be far apart, or infinite).
 __device__ __forceinline__ double below(double a, double b) { return a == b ? 0.0 : a - b; }
@@ -666,14 +680,12 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
   for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
   if (tid == 0) s_n = atomicAdd(&w.taken[b], (unsigned)n_all);
   __syncthreads();
-  // the range's ends as logits, a little wide: most logits need no more
-  const float x_lo = (float)((scale.base - plan.hi - 0.75) / set.c4), x_hi = (float)((scale.base - plan.lo + 0.75) / set.c4);
-  const float slack = 1e-6f * fmaxf(fabsf(x_lo), fabsf(x_hi));
+  const Ends ends(scale, plan.lo, plan.hi);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (x[r][e] < x_lo - slack || x[r][e] > x_hi + slack) continue;
+      if (ends.out(x[r][e])) continue;
       int bin;
       uint64_t fx;
       if (scale.weigh(x[r][e], bin, fx) && bin >= plan.lo && bin <= plan.hi) {
@@ -687,59 +699,55 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
 template <bool F32>
 __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams p, Ws w, int chunks, int places, int ib) {
   __shared__ Sums s;
-  __shared__ uint64_t s_list[kShort];
-  __shared__ uint64_t s_mass[NT], s_kept[kMaxChunks];
+  __shared__ uint64_t s_held[kHeld / 2];
+  __shared__ uint64_t s_mass[NT], s_weight[NT], s_kept[kMaxChunks];
   __shared__ unsigned s_count[NT];
   const int tid = threadIdx.x, b = blockIdx.x;
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
   const Settings set(p, b);
   const Scale scale(set.c4, plan.top);
+  const Ends ends(scale, plan.lo, plan.hi);
   const size_t row = (size_t)b * chunks;
   const uint64_t* list = w.list + (size_t)b * places;
-  const bool listed = plan.n_list <= places;
-
-  // Weights of the range in units of its first bin's, 2^-unit: whole numbers whose sum stays below 2^53.
+  const int n_list = plan.n_list;
+  const bool listed = n_list <= places;
   const float u = p.u[b];
   const double sure = tid < chunks ? w.sure[row + tid] : 0.0;
-  const int n_list = plan.n_list;
+  if (tid < chunks) s_kept[tid] = 0;
+
+  // Weights of the range in units of its first bin's, 2^-unit: whole numbers whose sum stays below 2^53.
   const int unit = 53 - (n_list > 1 ? 32 - __clz(n_list - 1) : 0);
   const double to_units = ldexp(1.0 / quarter(plan.lo & 3), unit - 35 + (plan.lo >> 2)), from_units = 1.0 / to_units;
   auto in_range = [&](float x, uint64_t& fx) {
     int bin;
-    if (!scale.weigh(x, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
+    if (ends.out(x) || !scale.weigh(x, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
     fx = (uint64_t)rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo));
     return true;
   };
-  if (tid < chunks) s_kept[tid] = 0;
-  const bool brief = listed && n_list <= kShort;
-  if (brief) {
-    uint64_t v[kShort / NT];
+
+  // fn(key) for every logit of the range, from memory
+  uint64_t first[8] = {};
+  if (listed) {
 #pragma unroll
-    for (int i = 0; i < kShort / NT; ++i) v[i] = i * NT + tid < n_list ? list[i * NT + tid] : 0;
-#pragma unroll
-    for (int i = 0; i < kShort / NT; ++i)
-      if (i * NT + tid < n_list) s_list[i * NT + tid] = v[i];
+    for (int e = 0; e < 8; ++e)
+      if (tid + e * NT < n_list) first[e] = list[tid + e * NT];
   }
-  __syncthreads();
-  // fn(key, weight) for every logit of the range (weight 0 where it is not wanted)
-  auto each = [&](bool weights, auto fn) {
-    uint64_t fx = 0;
-    if (brief) {
-      for (int i = tid; i < n_list; i += NT) {
-        const uint64_t key = s_list[i];
-        if (!weights || in_range(value_of<F32>(key, ib), fx)) fn(key, fx);
-      }
-    } else if (listed) {
-      for (int i0 = tid; i0 < n_list; i0 += 8 * NT) {
+  auto each_far = [&](auto fn) {
+    if (listed) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (tid + e * NT < n_list) fn(first[e], tid + e * NT);
+      for (int i0 = tid + 8 * NT; i0 < n_list; i0 += 8 * NT) {
         uint64_t v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = list[min(i0 + e * NT, n_list - 1)];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (i0 + e * NT < n_list && (!weights || in_range(value_of<F32>(v[e], ib), fx))) fn(v[e], fx);
+          if (i0 + e * NT < n_list) fn(v[e], i0 + e * NT);
       }
     } else {
+      uint64_t fx;
       for (int q = 0; q < chunks; ++q) {
         float x[kRounds][8];
 #pragma unroll
@@ -748,91 +756,167 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
         for (int r = 0; r < kRounds; ++r)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (in_range(x[r][e], fx)) fn(key_of<F32>(x[r][e], index_of(q, r) + e, ib), fx);
+            if (in_range(x[r][e], fx)) fn(key_of<F32>(x[r][e], index_of(q, r) + e, ib), 0);
       }
     }
   };
 
-  uint64_t cut = 0;
-  if (plan.by_k || plan.by_p) {
-    // what all keys have in common tells nothing: digits are of the distance from the least
-    uint64_t least = ~0ull, most = 0;
-    each(false, [&](uint64_t key, uint64_t) {
-      least = key < least ? key : least;
-      most = key > most ? key : most;
-    });
+  // What all keys have in common tells nothing: digits are of the distance from the least.
+  uint64_t least = ~0ull, most = 0;
+  each_far([&](uint64_t key, int) {
+    least = key < least ? key : least;
+    most = key > most ? key : most;
+  });
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t l = __shfl_xor(least, o, 64), m = __shfl_xor(most, o, 64);
-      least = l < least ? l : least;
-      most = m > most ? m : most;
-    }
-    if ((tid & 63) == 0) {
-      s_mass[tid >> 6] = least;
-      s_mass[kWaves + (tid >> 6)] = most;
-    }
-    __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t l = __shfl_xor(least, o, 64), m = __shfl_xor(most, o, 64);
+    least = l < least ? l : least;
+    most = m > most ? m : most;
+  }
+  if ((tid & 63) == 0) {
+    s_mass[tid >> 6] = least;
+    s_mass[kWaves + (tid >> 6)] = most;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kWaves; ++q) {
-      least = s_mass[q] < least ? s_mass[q] : least;
-      most = s_mass[kWaves + q] > most ? s_mass[kWaves + q] : most;
+  for (int q = 0; q < kWaves; ++q) {
+    least = s_mass[q] < least ? s_mass[q] : least;
+    most = s_mass[kWaves + q] > most ? s_mass[kWaves + q] : most;
+  }
+  if (most < least) most = least = 0;  // an empty range
+  __syncthreads();
+  const int key_bits = most > least ? 64 - __clzll((long long)(most - least)) : 0;
+  // Few values (of bf16 logits nearly always): a digit is a value, all its logits weigh the same, and
+  // weights come from a table.
+  const uint64_t least_value = least >> ib;
+  const bool few = (most >> ib) - least_value < NT;
+  if (few) {
+    uint64_t fx = 0;
+    if (!in_range(value_of<F32>((least_value + tid) << ib, ib), fx)) fx = 0;
+    s_weight[tid] = fx;
+  }
+  // the list stays in LDS where it fits: as distances of 32 bits (few values: 29 at most), or whole
+  uint32_t* held32 = (uint32_t*)s_held;
+  const bool in32 = listed && key_bits <= 32 && n_list <= kHeld, in64 = listed && !in32 && n_list <= kHeld / 2;
+  if (in32) each_far([&](uint64_t key, int i) { held32[i] = (uint32_t)(key - least); });
+  else if (in64) each_far([&](uint64_t key, int i) { s_held[i] = key; });
+  __syncthreads();
+  auto each = [&](auto fn) {
+    if (in32) {
+      for (int i = tid; i < n_list; i += NT) fn(least + held32[i]);
+    } else if (in64) {
+      for (int i = tid; i < n_list; i += NT) fn(s_held[i]);
+    } else {
+      each_far([&](uint64_t key, int) { fn(key); });
     }
-    __syncthreads();
-    const int key_bits = most > least ? 64 - __clzll((long long)(most - least)) : 0;
-    // The least key such that those from it up, of the ones from `cut` up, are as many (or weigh as
-    // much) as wanted(their sum), digit after digit of nine bits, until one key is left.
-    auto select = [&](bool by_weight, auto wanted) {
-      uint64_t prefix = 0, want = 0;
-      int high = key_bits;  // the digits above are settled
-      for (int round = 0;; ++round) {
-        const int shift = max(high - 9, 0);
-        s_count[tid] = 0;
-        s_mass[tid] = 0;
-        __syncthreads();
-        each(by_weight, [&](uint64_t key, uint64_t fx) {
-          const uint64_t d = key - least;
-          if (key < cut || d >> high != prefix) return;
-          const int digit = (int)(d >> shift) & ((1 << (high - shift)) - 1);
-          atomicAdd(&s_count[digit], 1u);
-          if (by_weight) atomicAdd((unsigned long long*)&s_mass[digit], fx);
-        });
-        __syncthreads();
-        const int digit = NT - 1 - tid;
-        const uint64_t n = s_count[digit], mine = by_weight ? s_mass[digit] : n;
-        uint64_t all;
-        const uint64_t before = block_excl(mine, s.u, all);
-        if (round == 0) want = wanted(all);
-        const int at = block_min(n > 0 && before + mine >= want ? tid : kNone, s.i);
-        if (at == kNone) return;  // all of them
-        if (tid == at) {
-          s.n[0] = before;
-          s.n[1] = n;
-        }
-        __syncthreads();
-        want -= s.n[0];
-        const uint64_t left = s.n[1];
-        prefix = prefix << (high - shift) | (uint64_t)(NT - 1 - at);
-        high = shift;
-        if (left == 1 || shift == 0) break;
-      }
-      const uint64_t found = least + (prefix << high);
-      cut = found > cut ? found : cut;
-    };
-    if (plan.by_k) select(false, [&](uint64_t) { return (uint64_t)plan.k; });
-    if (plan.by_p)
-      select(true, [&](uint64_t all) {
-        const double above = plan.above * to_units;
-        const double share = set.p * (above + (double)all + (plan.by_k ? 0.0 : plan.below * to_units));
-        const double want = ceil(share - above);
-        return want >= 1.0 ? (uint64_t)want : (uint64_t)1;
+  };
+  auto weight_of = [&](uint64_t key) {
+    uint64_t fx = 0;
+    if (few) return s_weight[(key >> ib) - least_value];
+    return in_range(value_of<F32>(key, ib), fx) ? fx : (uint64_t)0;
+  };
+  // The share of top-p as a weight of the range, where what top-k leaves of the range weighs `all`.
+  auto p_want = [&](uint64_t all) {
+    const double above = plan.above * to_units;
+    const double share = set.p * (above + (double)all + (plan.by_k ? 0.0 : plan.below * to_units));
+    const double want = ceil(share - above);
+    return want >= 1.0 ? (uint64_t)want : (uint64_t)1;
+  };
+
+  uint64_t cut = 0;  // the least key that is kept
+  // The least key such that those from it up, of the ones from `cut` up that are below `from` + 2^high,
+  // are as many (or weigh as much) as wanted(their sum): digit after digit of nine bits of the distance
+  // from `from`, until one key is left.
+  auto select = [&](bool by_weight, uint64_t from, int high, auto wanted) {
+    uint64_t want = 0, prefix = 0;
+    for (int round = 0;; ++round) {
+      const int shift = max(high - 9, 0);
+      s_count[tid] = 0;
+      s_mass[tid] = 0;
+      __syncthreads();
+      each([&](uint64_t key) {
+        const uint64_t d = key - from;
+        if (key < cut || d >> high != prefix) return;
+        const int digit = (int)(d >> shift) & ((1 << (high - shift)) - 1);
+        atomicAdd(&s_count[digit], 1u);
+        if (by_weight) atomicAdd((unsigned long long*)&s_mass[digit], weight_of(key));
       });
+      __syncthreads();
+      const int digit = NT - 1 - tid;
+      const uint64_t n = s_count[digit], mine = by_weight ? s_mass[digit] : n;
+      uint64_t all;
+      const uint64_t before = block_excl(mine, s.u, all);
+      if (round == 0) want = wanted(all);
+      const int at = block_min(n > 0 && before + mine >= want ? tid : kNone, s.i);
+      if (at == kNone) return;  // all of them
+      if (tid == at) {
+        s.n[0] = before;
+        s.n[1] = n;
+      }
+      __syncthreads();
+      want -= s.n[0];
+      const uint64_t left = s.n[1];
+      prefix = prefix << (high - shift) | (uint64_t)(NT - 1 - at);
+      high = shift;
+      if (left == 1 || shift == 0) break;
+    }
+    const uint64_t found = from + (prefix << high);
+    cut = found > cut ? found : cut;
+  };
+  if (few && (plan.by_k || plan.by_p)) {
+    // how many logits each value has: both cuts as a value and how many of its logits are kept
+    s_count[tid] = 0;
+    __syncthreads();
+    each([&](uint64_t key) { atomicAdd(&s_count[(key >> ib) - least_value], 1u); });
+    __syncthreads();
+    const int value = NT - 1 - tid;
+    const uint64_t n = s_count[value], fx = s_weight[value];
+    uint64_t n_before, n_all, before, all;
+    block_excl(n, n * fx, s.u, (uint64_t*)s.d[0], n_before, n_all, before, all);
+    int cut_at = kNone, cut_n = 0;  // the value, by its thread
+    if (plan.by_k) {
+      cut_at = block_min(n > 0 && n_before + n >= (uint64_t)plan.k ? tid : kNone, s.i);
+      if (tid == cut_at) {
+        s.n[0] = plan.k - n_before;
+        s.n[1] = before + s.n[0] * fx;
+      }
+      __syncthreads();
+      if (cut_at != kNone) {
+        cut_n = (int)s.n[0];
+        all = s.n[1];
+      }
+      __syncthreads();
+    }
+    if (plan.by_p) {
+      const uint64_t want = p_want(all);
+      const int at = block_min(n > 0 && before + n * fx >= want ? tid : kNone, s.i);
+      if (tid == at) s.n[0] = (want - before + fx - 1) / fx;
+      __syncthreads();
+      if (at != kNone && (at < cut_at || (at == cut_at && (int)s.n[0] < cut_n))) {
+        cut_at = at;
+        cut_n = (int)s.n[0];
+      }
+      __syncthreads();
+    }
+    if (cut_at != kNone) {
+      const uint64_t at = least_value + (uint64_t)(NT - 1 - cut_at);
+      cut = at << ib;
+      if (cut_n < (int)s_count[NT - 1 - cut_at]) {  // of equal ones the first: by the index's digits
+        __syncthreads();
+        select(false, cut, ib, [&](uint64_t) { return (uint64_t)cut_n; });
+      }
+    }
+  } else {
+    if (plan.by_k) select(false, least, key_bits, [&](uint64_t) { return (uint64_t)plan.k; });
+    if (plan.by_p) select(true, least, key_bits, p_want);
   }
 
   auto kept = [&](float x, uint64_t key) {
     return key >= cut && (!set.by_m || scale.far || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
   };
-  each(true, [&](uint64_t key, uint64_t fx) {
-    if (kept(value_of<F32>(key, ib), key)) atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], fx);
+  each([&](uint64_t key) {
+    if (kept(value_of<F32>(key, ib), key))
+      atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], weight_of(key));
   });
   __syncthreads();
   // back in the units of the row's first bin: whole numbers too, of that bin's weights
@@ -840,7 +924,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   draw<F32>(p, b, u, mass, chunks, s, scale, plan.total, [&](float x, int i) {
     int bin;
     uint64_t fx;
-    if (!scale.weigh(x, bin, fx) || bin > plan.hi) return 0.0;
+    if (ends.below(x) || !scale.weigh(x, bin, fx) || bin > plan.hi) return 0.0;
     if (bin < plan.lo) return (double)fx * quarter(bin);
     return kept(x, key_of<F32>(x, i, ib)) ? rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo)) * from_units : 0.0;
   });
