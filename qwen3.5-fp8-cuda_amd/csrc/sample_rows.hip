@@ -64,6 +64,7 @@ struct Ws {
   uint64_t* hist;    // [B][chunks][kBins]
   Chunk* chunk;      // [B][chunks]
   double* sure;      // [B][chunks] weights before the range
+  int2* span;        // [B][chunks] a chunk's logits on the list: where they begin, how many
   RowPlan* plan;     // [B]
   uint64_t* list;    // [B][kList]
   unsigned* taken;   // [B] places of the list that are taken
@@ -79,9 +80,10 @@ size_t layout(int B, int V, uint8_t* base, Ws* w) {
   uint8_t* hist = take(B * nc * kBins * 8);
   uint8_t* chunk = take(B * nc * sizeof(Chunk));
   uint8_t* sure = take(B * nc * 8);
+  uint8_t* span = take(B * nc * 8);
   uint8_t* plan = take(B * sizeof(RowPlan));
   uint8_t* list = take((size_t)B * min(kList, V) * 8);
-  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (RowPlan*)plan, (uint64_t*)list, (unsigned*)taken};
+  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (int2*)span, (RowPlan*)plan, (uint64_t*)list, (unsigned*)taken};
   return off;
 }
 
@@ -132,13 +134,22 @@ __device__ __forceinline__ double power(double g) {
 
 // The weights below a largest logit.
 struct Scale {
-  double c4, base;  // the largest's bin
+  double c4, base;  // base: the largest's bin
   float top;        // the largest
   bool far;         // |t| of it is 2^50 or more (or it is infinite): no other logit is near enough to have a weight
+  // Logits far below the largest are lifted to `least`, 400 bins below it, and go to a bin that nobody reads:
+  // no branch a logit, and no number that its bin's 32 bits do not hold.  Not `quick`, where that is not a
+  // number, or 24 bits of a logit do not tell bins apart: then each is looked at.
+  bool quick;
+  float least;
+  uint32_t first;
   __device__ __forceinline__ Scale(double c4_, float top_) : c4(c4_), top(top_) {
     const double t = (double)top * c4;
     far = !(fabs(t) < 1125899906842624.0);
     base = fabsf(top) == INFINITY ? (double)top : far ? t : (t + kRound) - kRound;
+    least = (float)((base - 400.0) / c4);
+    quick = !far && fabs(base) < 67108864.0 && least > -INFINITY;
+    first = (uint32_t)bits(kRound + base);
   }
   // The bin of a logit below `base` and its weight in the bin's units; false where it has none.
   __device__ __forceinline__ bool weigh(float x, int& bin, uint64_t& fx) const {
@@ -153,7 +164,15 @@ struct Scale {
     fx = bits(power(fma((double)x, c4, -(tm - kRound)))) & 0xFFFFFFFFFull;
     return true;
   }
+  // The same where `quick`: bin kBins without a weight, the weight with 2^52 added.
+  __device__ __forceinline__ double weigh_quick(float x, int& bin) const {
+    const double v = x > least ? x : least;
+    const double tm = fma(v, c4, kRound);
+    bin = (int)min(first - (uint32_t)bits(tm), (uint32_t)kBins);
+    return power(fma(v, c4, -(tm - kRound)));
+  }
 };
+
 // The logits of bins `hi` to `lo` below the largest lie between these two (a little wide): a test that
 // most logits fail without their weight.  Where all have to be looked at, all pass.
 struct Ends {
@@ -165,16 +184,19 @@ struct Ends {
     lo -= slack;
     hi += slack;
   }
-  __device__ __forceinline__ bool below(float x) const { return x < lo; }
   __device__ __forceinline__ bool out(float x) const { return x < lo || x > hi; }
 };
-// Bins from a to b below it (they may be far apart, or infinite).
-__device__ __forceinline__ double below(double a, double b) { return a == b ? 0.0 : a - b; }
 // 2^(-j / 4)
 __device__ __forceinline__ double quarter(int j) {
   const double s = (j & 2 ? 0.7071067811865476 : 1.0) * (j & 1 ? 0.8408964152537145 : 1.0);
   return ldexp(s, -(j >> 2));
 }
+// ... of every bin, and 0 for what has none
+__device__ __forceinline__ void fill_quarters(double* s_quarter) {
+  if ((int)threadIdx.x <= kBins) s_quarter[threadIdx.x] = (int)threadIdx.x < kBins ? quarter(threadIdx.x) : 0.0;
+}
+// Bins from a to b below it (they may be far apart, or infinite).
+__device__ __forceinline__ double below(double a, double b) { return a == b ? 0.0 : a - b; }
 // 2^(-j / 4) of a difference of bins that may be far (or infinite)
 __device__ __forceinline__ double quarter_far(double j) { return j < 4096.0 ? quarter((int)j) : 0.0; }
 
@@ -377,11 +399,12 @@ __device__ __forceinline__ void emit(const QhSampleRowsParams& p, int b, int tok
 }
 
 // Among the chunks, thread c's weighing `mass`, and then in the one that the draw falls into: the
-// first index whose running sum of kept weights is above u times the whole.  kept(x, i) is a logit's
-// weight, 0 where it is not kept; `total` below 0: all are.
-template <bool F32, typename Kept>
+// first index whose running sum of kept weights is above u times the whole.  keep(x, i, bin) says of a
+// logit with a weight whether it is kept, of those below `least` none is; `total` below 0: all are.
+// s_quarter[j] is 2^(-j / 4).
+template <bool F32, typename Keep>
 __device__ __forceinline__ void draw(const QhSampleRowsParams& p, int b, float u, double mass, int chunks, Sums& s,
-                                     const Scale& scale, double total, Kept kept) {
+                                     const double* s_quarter, const Scale& scale, double total, float least, Keep keep) {
   double all_mass;
   const double before = block_excl(mass, s.d[0], all_mass);
   if (total < 0.0) total = all_mass;
@@ -394,14 +417,37 @@ __device__ __forceinline__ void draw(const QhSampleRowsParams& p, int b, float u
   float x[kRounds][8];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
-  double w[kRounds][8], sum[kRounds] = {};
+  double w[kRounds][8] = {}, sum[kRounds] = {};
+  if (scale.quick) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      float most = x[r][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, x[r][e]);
+      if (!__any(most >= least)) continue;  // a wave of logits that are all too small
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        int bin;
+        const double v = (scale.weigh_quick(x[r][e], bin) - kWhole) * s_quarter[bin];
+        w[r][e] = keep(x[r][e], index_of(c, r) + e, bin) ? v : 0.0;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        int bin;
+        uint64_t fx;
+        w[r][e] = scale.weigh(x[r][e], bin, fx) && keep(x[r][e], index_of(c, r) + e, bin) ? (double)fx * s_quarter[bin] : 0.0;
+      }
+  }
   int last = kNone;
   float x_last = 0.0f;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[r][e] = kept(x[r][e], index_of(c, r) + e);
       sum[r] += w[r][e];
       if (w[r][e] > 0.0) {
         last = -(index_of(c, r) + e);
@@ -468,21 +514,14 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
   double mass = 0.0;
   if (!set.first || p.logprob) {
     unsigned long long* mine = (unsigned long long*)&s_hist[tid & (kCopies - 1)];
-    // Logits far below the largest are lifted to 400 bins below it, whose bin is one that nobody reads: no
-    // branch a logit, and no number that its bin's 32 bits do not hold.  Where that is not a number, or
-    // 24 bits of a logit do not tell bins apart, each is looked at.
-    const float least = (float)((scale.base - 400.0) / set.c4);
-    if (!scale.far && fabs(scale.base) < 67108864.0 && least > -INFINITY) {
-      const uint32_t first = (uint32_t)bits(kRound + scale.base);
+    if (scale.quick) {
 #pragma unroll
       for (int r = 0; r < kRounds; ++r)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const double v = x[r][e] > least ? x[r][e] : least;
-          const double tm = fma(v, set.c4, kRound);
-          const uint32_t bin = min(first - (uint32_t)bits(tm), (uint32_t)kBins);
-          const uint64_t fx = bits(power(fma(v, set.c4, -(tm - kRound))));
-          atomicAdd(mine + bin * kCopies, fx + ((1ull << 50) - 0x4330000000000000ull));  // its exponent away, a count in
+          int bin;
+          const uint64_t fx = bits(scale.weigh_quick(x[r][e], bin));
+          atomicAdd(mine + bin * kCopies, fx + ((1ull << 50) - 0x4330000000000000ull));  // the exponent away, a count in
         }
     } else {
 #pragma unroll
@@ -512,12 +551,13 @@ template <bool F32>
 __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams p, Ws w, int chunks) {
   __shared__ Sums s;
   __shared__ uint64_t s_other[2 * kBins];
-  __shared__ double s_base[kMaxChunks];
+  __shared__ double s_base[kMaxChunks], s_quarter[kBins + 1];
   const int tid = threadIdx.x, b = blockIdx.x;
   const size_t row = (size_t)b * chunks;
   const float u = p.u[b];
   const Settings set(p, b);
   const bool filtered = set.filtered();
+  fill_quarters(s_quarter);
   Chunk mine = {-INFINITY, 0.0, -INFINITY, kNone};
   if (tid < chunks) mine = w.chunk[row + tid];
   const float row_top = block_max(mine.top, s.f);
@@ -531,18 +571,14 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
   }
   const Scale scale(set.c4, row_top);
   const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(below(scale.base, mine.base)) : 0.0;
-  auto every = [&](float v, int) {
-    int bin;
-    uint64_t fx;
-    return scale.weigh(v, bin, fx) ? (double)fx * quarter(bin) : 0.0;
-  };
+  auto every = [](float, int, int) { return true; };
   if (!filtered) {
     if (set.first) {
       const int token = block_min(mine.top == row_top ? mine.top_at : kNone, s.i);
       const double all = block_total(scaled, s.d[0]);
       if (tid == 0) emit(p, b, token, row_top, scale, all);
     } else {
-      draw<F32>(p, b, u, scaled, chunks, s, scale, -1.0, every);
+      draw<F32>(p, b, u, scaled, chunks, s, s_quarter, scale, -1.0, -INFINITY, every);
     }
     if (tid == 0) w.plan[b].done = 1;
     return;
@@ -618,7 +654,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
   }
   if (lo >= kBins) {  // nothing is cut
-    draw<F32>(p, b, u, scaled, chunks, s, scale, -1.0, every);
+    draw<F32>(p, b, u, scaled, chunks, s, s_quarter, scale, -1.0, -INFINITY, every);
     if (tid == 0) w.plan[b].done = 1;
     return;
   }
@@ -673,12 +709,18 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
   double sure_excl, sure_all;
   uint64_t n_excl, n_all;
   block_excl(sure, n, s.d[0], s.u, sure_excl, sure_all, n_excl, n_all);
-  if (tid == 0) w.sure[row + c] = sure_all;
+  if (tid == 0) {
+    w.sure[row + c] = sure_all;
+    if (n_all == 0) w.span[row + c] = int2{0, 0};
+  }
   if (n_all == 0 || plan.n_list > places) return;
   float x[kRounds][8];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) load8<F32>(p, b, index_of(c, r), x[r]);
-  if (tid == 0) s_n = atomicAdd(&w.taken[b], (unsigned)n_all);
+  if (tid == 0) {
+    s_n = atomicAdd(&w.taken[b], (unsigned)n_all);
+    w.span[row + c] = int2{(int)s_n, (int)n_all};
+  }
   __syncthreads();
   const Ends ends(scale, plan.lo, plan.hi);
 #pragma unroll
@@ -702,6 +744,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   __shared__ uint64_t s_held[kHeld / 2];
   __shared__ uint64_t s_mass[NT], s_weight[NT], s_kept[kMaxChunks];
   __shared__ unsigned s_count[NT];
+  __shared__ double s_quarter[kBins + 1];
+  __shared__ int2 s_span[kMaxChunks];
   const int tid = threadIdx.x, b = blockIdx.x;
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
@@ -714,7 +758,11 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const bool listed = n_list <= places;
   const float u = p.u[b];
   const double sure = tid < chunks ? w.sure[row + tid] : 0.0;
-  if (tid < chunks) s_kept[tid] = 0;
+  if (tid < chunks) {
+    s_kept[tid] = 0;
+    s_span[tid] = w.span[row + tid];
+  }
+  fill_quarters(s_quarter);
 
   // Weights of the range in units of its first bin's, 2^-unit: whole numbers whose sum stays below 2^53.
   const int unit = 53 - (n_list > 1 ? 32 - __clz(n_list - 1) : 0);
@@ -761,35 +809,16 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     }
   };
 
-  // What all keys have in common tells nothing: digits are of the distance from the least.
-  uint64_t least = ~0ull, most = 0;
-  each_far([&](uint64_t key, int) {
-    least = key < least ? key : least;
-    most = key > most ? key : most;
-  });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t l = __shfl_xor(least, o, 64), m = __shfl_xor(most, o, 64);
-    least = l < least ? l : least;
-    most = m > most ? m : most;
-  }
-  if ((tid & 63) == 0) {
-    s_mass[tid >> 6] = least;
-    s_mass[kWaves + (tid >> 6)] = most;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kWaves; ++q) {
-    least = s_mass[q] < least ? s_mass[q] : least;
-    most = s_mass[kWaves + q] > most ? s_mass[kWaves + q] : most;
-  }
-  if (most < least) most = least = 0;  // an empty range
-  __syncthreads();
-  const int key_bits = most > least ? 64 - __clzll((long long)(most - least)) : 0;
+  // What all keys have in common tells nothing: digits are of the distance from the least that the
+  // range may have.
+  const bool whole = !(ends.lo <= ends.hi);  // ends that are no numbers: the largest alone has a weight
+  const uint64_t least_value = key_of<F32>(whole ? plan.top : ends.lo, 0, ib) >> ib;
+  const uint64_t values = (key_of<F32>(whole ? plan.top : ends.hi, 0, ib) >> ib) - least_value + 1;
+  const uint64_t least = least_value << ib;
+  const int key_bits = 64 - __clzll((long long)((values << ib) - 1));
   // Few values (of bf16 logits nearly always): a digit is a value, all its logits weigh the same, and
   // weights come from a table.
-  const uint64_t least_value = least >> ib;
-  const bool few = (most >> ib) - least_value < NT;
+  const bool few = values <= NT;
   if (few) {
     uint64_t fx = 0;
     if (!in_range(value_of<F32>((least_value + tid) << ib, ib), fx)) fx = 0;
@@ -803,7 +832,14 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   __syncthreads();
   auto each = [&](auto fn) {
     if (in32) {
-      for (int i = tid; i < n_list; i += NT) fn(least + held32[i]);
+      for (int i0 = tid; i0 < n_list; i0 += 4 * NT) {  // four reads on their way at once
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = held32[min(i0 + e * NT, n_list - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + e * NT < n_list) fn(least + v[e]);
+      }
     } else if (in64) {
       for (int i = tid; i < n_list; i += NT) fn(s_held[i]);
     } else {
@@ -911,23 +947,50 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     if (plan.by_p) select(true, least, key_bits, p_want);
   }
 
-  auto kept = [&](float x, uint64_t key) {
-    return key >= cut && (!set.by_m || scale.far || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
+  // a key from the cut up, as a comparison of logits
+  const float x_cut = cut > 0 ? value_of<F32>(cut, ib) : -INFINITY;
+  const int i_cut = index_of_key(cut, ib);
+  auto kept = [&](float x, int i) {
+    return (x > x_cut || (x == x_cut && i <= i_cut)) &&
+           (!set.by_m || scale.far || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
   };
-  each([&](uint64_t key) {
-    if (kept(value_of<F32>(key, ib), key))
-      atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], weight_of(key));
-  });
+  // what is kept of each chunk: its logits lie together on the list, a wave adds them up
+  auto weight_kept = [&](uint64_t key) { return kept(value_of<F32>(key, ib), index_of_key(key, ib)) ? weight_of(key) : 0; };
+  if (listed) {
+    for (int c = tid >> 6; c < chunks; c += kWaves) {
+      const int2 span = s_span[c];
+      uint64_t mine = 0, all;
+      const int end = span.x + span.y;
+      if (in32 && few && !set.by_m) {
+        const uint32_t cut32 = cut > least ? (uint32_t)(cut - least) : 0;  // the cut is not above the largest key
+        for (int i0 = span.x + (tid & 63); i0 < end; i0 += 256) {
+          uint32_t v[4];
+          uint64_t fx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = held32[min(i0 + 64 * e, end - 1)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) fx[e] = s_weight[v[e] >> ib];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine += i0 + 64 * e < end && v[e] >= cut32 ? fx[e] : 0;
+        }
+      } else {
+        for (int i = span.x + (tid & 63); i < end; i += 64)
+          mine += weight_kept(in32 ? least + held32[i] : in64 ? s_held[i] : list[i]);
+      }
+      wave_excl(mine, all);
+      if ((tid & 63) == 0) s_kept[c] = all;
+    }
+  } else {
+    each([&](uint64_t key) {
+      const uint64_t fx = weight_kept(key);
+      if (fx) atomicAdd((unsigned long long*)&s_kept[index_of_key(key, ib) / kChunk], fx);
+    });
+  }
   __syncthreads();
   // back in the units of the row's first bin: whole numbers too, of that bin's weights
   const double mass = tid < chunks ? sure + (double)s_kept[tid] * from_units : 0.0;
-  draw<F32>(p, b, u, mass, chunks, s, scale, plan.total, [&](float x, int i) {
-    int bin;
-    uint64_t fx;
-    if (ends.below(x) || !scale.weigh(x, bin, fx) || bin > plan.hi) return 0.0;
-    if (bin < plan.lo) return (double)fx * quarter(bin);
-    return kept(x, key_of<F32>(x, i, ib)) ? rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo)) * from_units : 0.0;
-  });
+  draw<F32>(p, b, u, mass, chunks, s, s_quarter, scale, plan.total, ends.lo,
+            [&](float x, int i, int bin) { return bin < plan.lo || (bin <= plan.hi && kept(x, i)); });
 }
 
 template <bool F32>
