@@ -53,17 +53,20 @@ struct TileIds {
 };
 
 // ---- h = A x -----------------------------------------------------------------------------
-// A workgroup: 16 tokens, one slice of K, the tile's adapters z, z + gridDim.z, ...  Its four
-// waves take the slice's blocks of 64 in turn and add up through LDS.  Per block a lane loads
-// 32 bytes of its row of x and of A (128 bytes a row and wave: whole cache lines); which 8 of
-// a block's 64 go into which product is the same for both operands, and free.
-template <int RT>  // tiles of 16 ranks
-__global__ __launch_bounds__(256) void adapters_shrink_kernel(QhAdaptersParams p, int slice) {
-  __shared__ f32x4 s_part[4][RT][64];
+// A workgroup: 16 MT tokens, one slice of K, the tile's adapters z, z + gridDim.z, ...  Its eight
+// waves take the slice's blocks of 64 in turn, BLOCKS of them with all loads on their way at once,
+// and add up through LDS.
+constexpr int kShrinkWaves = 8;
+
+template <int MT, int RT, int BLOCKS>  // RT: tiles of 16 ranks
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapters_shrink_kernel(QhAdaptersParams p, int slice) {
+  __shared__ f32x4 s_part[kShrinkWaves][MT * RT][64];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-  const int t0 = blockIdx.y * 16, k0 = blockIdx.x * slice, k1 = min(p.K, k0 + slice);
-  TileIds tile(p, t0, 16);
-  const uint16_t* xr = p.x + (long long)min(t0 + row, p.T - 1) * p.x_ts;
+  const int t0 = blockIdx.y * 16 * MT, k0 = blockIdx.x * slice, k1 = min(p.K, k0 + slice);
+  TileIds tile(p, t0, 16 * MT);
+  const uint16_t* xr[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xr[m] = p.x + (long long)min(t0 + 16 * m + row, p.T - 1) * p.x_ts;
   const int Rp = 16 * ((p.R + 15) / 16);
   const u32x4 zero = {0, 0, 0, 0};
   for (int j = 0; tile.left != 0; ++j) {
@@ -73,38 +76,54 @@ __global__ __launch_bounds__(256) void adapters_shrink_kernel(QhAdaptersParams p
     const uint16_t* ar[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) ar[r] = p.a + ((size_t)a * p.R + min(16 * r + row, p.R - 1)) * p.K;
-    f32x4 acc[RT];
+    f32x4 acc[MT][RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[r] = f32x4{0, 0, 0, 0};
-    for (int k = k0 + 64 * wid; k < k1; k += 256) {
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int c = k + 16 * g + 8 * half;
+      for (int r = 0; r < RT; ++r) acc[m][r] = f32x4{0, 0, 0, 0};
+    for (int k = k0 + 64 * wid; k < k1; k += 64 * kShrinkWaves * BLOCKS) {
+      u32x4 x[2 * BLOCKS][MT], w[2 * BLOCKS][RT];
+#pragma unroll
+      for (int i = 0; i < 2 * BLOCKS; ++i) {
+        const int c = k + 64 * kShrinkWaves * (i / 2) + 32 * (i % 2) + 8 * g;
         const bool in = c < k1;
-        const u32x4 x = in ? load16(xr + c) : zero;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) acc[r] = mfma(in ? load16(ar[r] + c) : zero, x, acc[r]);
+        for (int r = 0; r < RT; ++r) w[i][r] = in ? load16(ar[r] + c) : zero;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x[i][m] = in ? load16(xr[m] + c) : zero;
       }
+#pragma unroll
+      for (int i = 0; i < 2 * BLOCKS; ++i)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m][r] = mfma(w[i][r], x[i][m], acc[m][r]);
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) s_part[wid][r][lane] = acc[r];
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s_part[wid][m * RT + r][lane] = acc[m][r];
     __syncthreads();
-    // lane: token row, ranks 16 r + 4 g .. + 3
-    for (int r = wid; r < RT; r += 4) {
-      const f32x4 s = (s_part[0][r][lane] + s_part[1][r][lane]) + (s_part[2][r][lane] + s_part[3][r][lane]);
-      if ((mine >> row) & 1 && 16 * r < Rp)
-        *(f32x4*)(p.h + ((size_t)blockIdx.x * p.T + t0 + row) * Rp + 16 * r + 4 * g) = s;
+    // lane: token row of its tile of 16, ranks 16 r + 4 g .. + 3
+    for (int q = wid; q < MT * RT; q += kShrinkWaves) {
+      const int m = q / RT, r = q % RT;
+      f32x4 s = s_part[0][q][lane];
+#pragma unroll
+      for (int v = 1; v < kShrinkWaves; ++v) s += s_part[v][q][lane];
+      if ((mine >> (16 * m + row)) & 1 && 16 * r < Rp)
+        *(f32x4*)(p.h + ((size_t)blockIdx.x * p.T + t0 + 16 * m + row) * Rp + 16 * r + 4 * g) = s;
     }
     __syncthreads();
   }
 }
 
 // ---- out = y + scale B h -------------------------------------------------------------------
-// A wave: 16 MT tokens, 32 columns at a time.  The rows of B are the first operand, in an order
+// A wave: 16 MT tokens, 32 CG columns at a time.  The rows of B are the first operand, in an order
 // that leaves each lane 8 consecutive columns of one token: of a pair of products, the first has
 // columns 8 m + 0 .. 3 and the second 8 m + 4 .. 7 of each eight.  Ranks go 32 to a product, high
-// and low parts one after the other; rank 16 (and 8) has both parts in one, side by side.
-template <int MT, int RC, bool SMALL>
+// and low parts one after the other; rank 16 (and 8) has both parts in one, side by side.  The rows
+// of B of AT adapters are on their way at once, those of y behind them.
+template <int MT, int RC, bool SMALL, int CG, int AT>
 __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p, int slices, int cols) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
   const int t0 = blockIdx.y * 16 * MT;
@@ -124,9 +143,20 @@ __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p
       f32x4 u = {0, 0, 0, 0}, v = u;
       if (mine[m] >= 0 && r0 < p.R) {
         const float* h = p.h + (size_t)t * Rp + r0;
-        for (int i = 0; i < slices; ++i) {
-          u += *(const f32x4*)(h + (size_t)i * p.T * Rp);
-          v += *(const f32x4*)(h + (size_t)i * p.T * Rp + 4);
+        for (int i0 = 0; i0 < slices; i0 += 4) {
+          f32x4 a[4], b[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* part = h + (size_t)min(i0 + i, slices - 1) * p.T * Rp;
+            a[i] = *(const f32x4*)part;
+            b[i] = *(const f32x4*)(part + 4);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = i0 + i < slices;
+            u += in ? a[i] : f32x4{0, 0, 0, 0};
+            v += in ? b[i] : f32x4{0, 0, 0, 0};
+          }
         }
       }
       u *= s;
@@ -142,91 +172,134 @@ __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p
   }
   const u32x4 zero = {0, 0, 0, 0};
   for (int i = 0; i < cols; ++i) {
-    const int c0 = ((blockIdx.x * cols + i) * 4 + wid) * 32;
+    const int c0 = ((blockIdx.x * cols + i) * 4 + wid) * 32 * CG;
     if (c0 >= p.N) break;
-    f32x4 acc[MT][2];
+    f32x4 acc[MT][2 * CG];
+    u32x4 y[MT][CG];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = f32x4{0, 0, 0, 0};
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < 2 * CG; ++q) acc[m][q] = f32x4{0, 0, 0, 0};
     TileIds tile = ids;
-    while (tile.left != 0) {
-      uint64_t tokens;
-      const int a = tile.next(tokens);
-      f32x4 d[MT][2];
+    bool asked = false;
+    do {
+      int a[AT], count = 0;
+      u32x4 b[AT][RC][2 * CG];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) d[m][0] = d[m][1] = f32x4{0, 0, 0, 0};
+      for (int n = 0; n < AT; ++n) {
+        if (n > 0 && tile.left == 0) continue;
+        uint64_t tokens;
+        a[n] = tile.left != 0 ? tile.next(tokens) : 0;
+        count = n + 1;
 #pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
+        for (int c = 0; c < RC; ++c) {
+          const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int col = min(c0 + 8 * (row >> 2) + 4 * half + (row & 3), p.N - 1);
-          const u32x4 b = r0 < p.R ? load16(p.b + ((size_t)a * p.N + col) * p.R + r0) : zero;
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            d[m][half] = mfma(b, hi[m][c], d[m][half]);
-            if (!SMALL) d[m][half] = mfma(b, lo[m][c], d[m][half]);
+          for (int q = 0; q < 2 * CG; ++q) {
+            const int col = min(c0 + 32 * (q / 2) + 8 * (row >> 2) + 4 * (q % 2) + (row & 3), p.N - 1);
+            b[n][c][q] = r0 < p.R ? load16(p.b + ((size_t)a[n] * p.N + col) * p.R + r0) : zero;
           }
         }
       }
+      if (!asked) {
+        asked = true;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (mine[m] == a) {
-          acc[m][0] = d[m][0];
-          acc[m][1] = d[m][1];
-        }
-    }
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int t = t0 + 16 * m + row, c = c0 + 8 * g;
-      if (t >= p.T || c >= p.N || (mine[m] < 0 && p.out == p.y)) continue;
-      u32x4 y = load16(p.y + t * p.y_ts + c);
-      if (mine[m] >= 0) {  // a row without an adapter is copied as it is
-        const f32x4 u = acc[m][0], v = acc[m][1];
-        y = u32x4{pack_bf2(bf_lo(y.x) + u.x, bf_hi(y.x) + u.y), pack_bf2(bf_lo(y.y) + u.z, bf_hi(y.y) + u.w),
-                  pack_bf2(bf_lo(y.z) + v.x, bf_hi(y.z) + v.y), pack_bf2(bf_lo(y.w) + v.z, bf_hi(y.w) + v.w)};
+          for (int q = 0; q < CG; ++q) {
+            const int t = min(t0 + 16 * m + row, p.T - 1), c = c0 + 32 * q + 8 * g;
+            y[m][q] = c < p.N ? load16(p.y + t * p.y_ts + c) : zero;
+          }
       }
-      *(u32x4*)(p.out + t * p.out_ts + c) = y;
-    }
+#pragma unroll
+      for (int n = 0; n < AT; ++n) {
+        if (n >= count) continue;
+        f32x4 d[MT][2 * CG];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int q = 0; q < 2 * CG; ++q) {
+            d[m][q] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < RC; ++c) {
+              d[m][q] = mfma(b[n][c][q], hi[m][c], d[m][q]);
+              if (!SMALL) d[m][q] = mfma(b[n][c][q], lo[m][c], d[m][q]);
+            }
+            if (mine[m] == a[n]) acc[m][q] = d[m][q];
+          }
+      }
+    } while (tile.left != 0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < CG; ++q) {
+        const int t = t0 + 16 * m + row, c = c0 + 32 * q + 8 * g;
+        if (t >= p.T || c >= p.N || (mine[m] < 0 && p.out == p.y)) continue;
+        u32x4 z = y[m][q];
+        if (mine[m] >= 0) {  // a row without an adapter is copied as it is
+          const f32x4 u = acc[m][2 * q], v = acc[m][2 * q + 1];
+          z = u32x4{pack_bf2(bf_lo(z.x) + u.x, bf_hi(z.x) + u.y), pack_bf2(bf_lo(z.y) + u.z, bf_hi(z.y) + u.w),
+                    pack_bf2(bf_lo(z.z) + v.x, bf_hi(z.z) + v.y), pack_bf2(bf_lo(z.w) + v.z, bf_hi(z.w) + v.w)};
+        }
+        *(u32x4*)(p.out + t * p.out_ts + c) = z;
+      }
   }
 }
 
 // Slices of K whose partial sums the workspace holds.
-int max_slices(int T) { return T <= 1024 ? 8 : T <= 8192 ? 8192 / T : 1; }
+int max_slices(int T) { return T <= 2048 ? 8 : T <= 16384 ? 16384 / T : 1; }
+
+template <int MT, int RT, int BLOCKS>
+void shrink(const QhAdaptersParams& p, int slices, int slice, int z, hipStream_t st) {
+  const dim3 grid(slices, (p.T + 16 * MT - 1) / (16 * MT), z);
+  adapters_shrink_kernel<MT, RT, BLOCKS><<<grid, 64 * kShrinkWaves, 0, st>>>(p, slice);
+}
 
 }  // namespace
 
 size_t qh_adapters_ws_bytes(int max_tokens, int R) {
   // the most that max_slices(T) * T is for any T up to max_tokens
-  const size_t rows = max_tokens <= 1024 ? 8 * (size_t)max_tokens : max_tokens <= 8192 ? 8192 : (size_t)max_tokens;
+  const size_t rows = max_tokens <= 2048 ? 8 * (size_t)max_tokens : max_tokens <= 16384 ? 16384 : (size_t)max_tokens;
   return rows * (16 * ((R + 15) / 16)) * sizeof(float);
 }
 
 int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
-  const int tiles = (p.T + 15) / 16;
-  // K in slices until there are 512 workgroups, of 512 columns at least: two blocks a wave
-  int slices = min(max_slices(p.T), max(1, min(512 / tiles, (p.K + 511) / 512)));
-  const int slice = ((p.K + slices - 1) / slices + 255) / 256 * 256;
+  const bool few = p.T <= 256;
+  const int tiles = (p.T + 15) / 16, wide_tiles = (p.T + 31) / 32;
+  // K in slices until there are 512 workgroups, of a block a wave at least
+  const int step = 64 * kShrinkWaves, steps = (p.K + step - 1) / step;
+  const bool two = !few && p.R <= 64;
+  int slices = min(max_slices(p.T), max(1, min(512 / (two ? wide_tiles : tiles), steps)));
+  const int slice = (steps + slices - 1) / slices * step;
   slices = (p.K + slice - 1) / slice;
-  // few tokens name an adapter each: one a workgroup
-  const int z = p.T <= 256 ? min(16, p.T) : 1;
-  const dim3 grid(slices, tiles, z);
-  if (p.R <= 16) adapters_shrink_kernel<1><<<grid, 256, 0, st>>>(p, slice);
-  else if (p.R <= 32) adapters_shrink_kernel<2><<<grid, 256, 0, st>>>(p, slice);
-  else if (p.R <= 64) adapters_shrink_kernel<4><<<grid, 256, 0, st>>>(p, slice);
-  else adapters_shrink_kernel<8><<<grid, 256, 0, st>>>(p, slice);
-
-  const int cols = p.T <= 256 ? 1 : 4;
-  const dim3 wide((p.N + 128 * cols - 1) / (128 * cols), p.T <= 256 ? tiles : (p.T + 63) / 64);
-  if (p.T <= 256) {
-    if (p.R <= 16) adapters_expand_kernel<1, 1, true><<<wide, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 32) adapters_expand_kernel<1, 1, false><<<wide, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 64) adapters_expand_kernel<1, 2, false><<<wide, 256, 0, st>>>(p, slices, cols);
-    else adapters_expand_kernel<1, 4, false><<<wide, 256, 0, st>>>(p, slices, cols);
+  // few tokens name an adapter each: one a workgroup; of prompts a tile has one, seldom more
+  const int z = few ? min(16, p.T) : 4;
+  if (two) {
+    if (p.R <= 16) shrink<2, 1, 3>(p, slices, slice, z, st);
+    else if (p.R <= 32) shrink<2, 2, 2>(p, slices, slice, z, st);
+    else shrink<2, 4, 1>(p, slices, slice, z, st);
   } else {
-    if (p.R <= 16) adapters_expand_kernel<4, 1, true><<<wide, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 32) adapters_expand_kernel<4, 1, false><<<wide, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 64) adapters_expand_kernel<4, 2, false><<<wide, 256, 0, st>>>(p, slices, cols);
-    else adapters_expand_kernel<4, 4, false><<<wide, 256, 0, st>>>(p, slices, cols);
+    if (p.R <= 16) shrink<1, 1, 3>(p, slices, slice, z, st);
+    else if (p.R <= 32) shrink<1, 2, 2>(p, slices, slice, z, st);
+    else if (p.R <= 64) shrink<1, 4, 1>(p, slices, slice, z, st);
+    else shrink<1, 8, 1>(p, slices, slice, z, st);
+  }
+
+  // 32 tokens and 256 columns a workgroup at a time where that leaves four workgroups a CU, and then
+  // up to four times; otherwise 16 and 128
+  const int wide1 = (p.N + 255) / 256, cols = min(4, wide_tiles * wide1 / 1024);
+  if (cols == 0) {
+    const dim3 grid((p.N + 127) / 128, tiles);
+    if (p.R <= 16) adapters_expand_kernel<1, 1, true, 1, 8><<<grid, 256, 0, st>>>(p, slices, 1);
+    else if (p.R <= 32) adapters_expand_kernel<1, 1, false, 1, 8><<<grid, 256, 0, st>>>(p, slices, 1);
+    else if (p.R <= 64) adapters_expand_kernel<1, 2, false, 1, 4><<<grid, 256, 0, st>>>(p, slices, 1);
+    else adapters_expand_kernel<1, 4, false, 1, 2><<<grid, 256, 0, st>>>(p, slices, 1);
+  } else {
+    const dim3 grid((wide1 + cols - 1) / cols, wide_tiles);
+    if (p.R <= 16) adapters_expand_kernel<2, 1, true, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
+    else if (p.R <= 32) adapters_expand_kernel<2, 1, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
+    else if (p.R <= 64) adapters_expand_kernel<2, 2, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
+    else adapters_expand_kernel<2, 4, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
   }
   return 0;
 }
