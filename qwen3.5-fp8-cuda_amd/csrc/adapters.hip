@@ -129,45 +129,42 @@ __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p
   const int t0 = blockIdx.y * 16 * MT;
   const int Rp = 16 * ((p.R + 15) / 16);
   const TileIds ids(p, t0, 16 * MT);
-  // the tokens' h, scaled: the lane's token and its 8 ranks of each product
+  // The tile's h, summed over the slices of K, scaled and in two parts, once a workgroup: 4 ranks a
+  // thread.  A row's 16 bytes of padding spread the reads below over the banks.
+  constexpr int kRow = (SMALL ? 16 : 32 * RC) + 8;
+  __shared__ uint16_t s_hi[16 * MT][kRow], s_lo[16 * MT][kRow];
+  constexpr int kQuads = SMALL ? 4 : 8 * RC;
+  for (int i = threadIdx.x; i < 16 * MT * kQuads; i += 256) {
+    const int row = i / kQuads, r = 4 * (i % kQuads), t = t0 + row, a = __shfl(ids.id, row, 64);
+    f32x4 u = {0, 0, 0, 0};
+    if (a >= 0 && r < p.R) {
+      const float* h = p.h + (size_t)t * Rp + r;
+      for (int q0 = 0; q0 < slices; q0 += 4) {
+        f32x4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = *(const f32x4*)(h + (size_t)min(q0 + q, slices - 1) * p.T * Rp);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) u += q0 + q < slices ? v[q] : f32x4{0, 0, 0, 0};
+      }
+      u *= p.scale[a];
+    }
+    const u32x2 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w)};
+    *(u32x2*)&s_hi[row][r] = top;
+    *(u32x2*)&s_lo[row][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
+                                   pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
+  }
+  __syncthreads();
+  // the lane's token and its 8 ranks of each product
   u32x4 hi[MT][RC], lo[MT][RC];
   int mine[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     mine[m] = __shfl(ids.id, 16 * m + row, 64);
-    const int t = t0 + 16 * m + row;
-    const float s = mine[m] >= 0 ? p.scale[mine[m]] : 0.0f;
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
       const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
-      f32x4 u = {0, 0, 0, 0}, v = u;
-      if (mine[m] >= 0 && r0 < p.R) {
-        const float* h = p.h + (size_t)t * Rp + r0;
-        for (int i0 = 0; i0 < slices; i0 += 4) {
-          f32x4 a[4], b[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* part = h + (size_t)min(i0 + i, slices - 1) * p.T * Rp;
-            a[i] = *(const f32x4*)part;
-            b[i] = *(const f32x4*)(part + 4);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool in = i0 + i < slices;
-            u += in ? a[i] : f32x4{0, 0, 0, 0};
-            v += in ? b[i] : f32x4{0, 0, 0, 0};
-          }
-        }
-      }
-      u *= s;
-      v *= s;
-      const u32x4 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w), pack_bf2(v.x, v.y), pack_bf2(v.z, v.w)};
-      const u32x4 rest = {pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
-                          pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y))),
-                          pack_bf2(low_part(v.x, bf_lo(top.z)), low_part(v.y, bf_hi(top.z))),
-                          pack_bf2(low_part(v.z, bf_lo(top.w)), low_part(v.w, bf_hi(top.w)))};
-      hi[m][c] = SMALL && g >= 2 ? rest : top;
-      lo[m][c] = rest;
+      lo[m][c] = *(const u32x4*)&s_lo[16 * m + row][r0];
+      hi[m][c] = SMALL && g >= 2 ? lo[m][c] : *(const u32x4*)&s_hi[16 * m + row][r0];
     }
   }
   const u32x4 zero = {0, 0, 0, 0};
