@@ -118,26 +118,69 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapters_shrink_kernel(QhAd
 }
 
 // ---- out = y + scale B h -------------------------------------------------------------------
-// A wave: 16 MT tokens, 32 CG columns at a time.  The rows of B are the first operand, in an order
-// that leaves each lane 8 consecutive columns of one token: of a pair of products, the first has
-// columns 8 m + 0 .. 3 and the second 8 m + 4 .. 7 of each eight.  Ranks go 32 to a product, high
-// and low parts one after the other; rank 16 (and 8) has both parts in one, side by side.  The rows
-// of B of AT adapters are on their way at once, those of y behind them.
-template <int MT, int RC, bool SMALL, int CG, int AT>
-__global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p, int slices, int cols) {
+// A wave: 16 MT tokens and 32 CG columns; WAVES of them side by side share the tile's h.  The rows of B
+// are the first operand, in an order that leaves each lane 8 consecutive columns of one token: of a
+// pair of products, the first has columns 8 m + 0 .. 3 and the second 8 m + 4 .. 7 of each eight.
+// Ranks go 32 to a product, high and low parts one after the other; rank 16 (and 8) has both parts in
+// one, side by side.  The rows of B of AT adapters are on their way at once.
+// Of eight waves two workgroups fit a CU where a wave takes 128 registers at most.
+template <int WAVES, int MT, int RC, bool SMALL, int CG, int AT>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 1) void adapters_expand_kernel(QhAdaptersParams p, int slices) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-  const int t0 = blockIdx.y * 16 * MT;
+  const int t0 = blockIdx.y * 16 * MT, c0 = (blockIdx.x * WAVES + wid) * 32 * CG;
   const int Rp = 16 * ((p.R + 15) / 16);
-  const TileIds ids(p, t0, 16 * MT);
+  const u32x4 zero = {0, 0, 0, 0};
+  TileIds tile(p, t0, 16 * MT);
+  const int token_id = tile.id;
+
+  int a[AT], count;
+  u32x4 b[AT][RC][2 * CG];
+  auto load_b = [&]() {
+    count = 0;
+#pragma unroll
+    for (int n = 0; n < AT; ++n) {
+      if (tile.left == 0) continue;
+      uint64_t tokens;
+      a[n] = tile.next(tokens);
+      count = n + 1;
+#pragma unroll
+      for (int c = 0; c < RC; ++c) {
+        const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
+#pragma unroll
+        for (int q = 0; q < 2 * CG; ++q) {
+          const int col = min(c0 + 32 * (q / 2) + 8 * (row >> 2) + 4 * (q % 2) + (row & 3), p.N - 1);
+          b[n][c][q] = r0 < p.R ? load16(p.b + ((size_t)a[n] * p.N + col) * p.R + r0) : zero;
+        }
+      }
+    }
+  };
+  u32x4 y[MT][CG];
+  auto load_y = [&]() {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int q = 0; q < CG; ++q) {
+        const int t = min(t0 + 16 * m + row, p.T - 1), c = c0 + 32 * q + 8 * g;
+        y[m][q] = c < p.N ? load16(p.y + t * p.y_ts + c) : zero;
+      }
+  };
+  // Few tokens wait for B most: it goes first, y behind it.  Of a prompt y is most of the bytes, and h
+  // would wait behind it (loads come back in order): 3700 tokens 44 us against 35.
+  constexpr bool kEarly = AT > 1;
+  if (kEarly) {
+    load_b();
+    load_y();
+  }
+
   // The tile's h, summed over the slices of K, scaled and in two parts, once a workgroup: 4 ranks a
   // thread.  A row's 16 bytes of padding spread the reads below over the banks.
   constexpr int kRow = (SMALL ? 16 : 32 * RC) + 8;
   __shared__ uint16_t s_hi[16 * MT][kRow], s_lo[16 * MT][kRow];
   constexpr int kQuads = SMALL ? 4 : 8 * RC;
-  for (int i = threadIdx.x; i < 16 * MT * kQuads; i += 256) {
-    const int row = i / kQuads, r = 4 * (i % kQuads), t = t0 + row, a = __shfl(ids.id, row, 64);
+  for (int i = threadIdx.x; i < 16 * MT * kQuads; i += 64 * WAVES) {
+    const int tr = i / kQuads, r = 4 * (i % kQuads), t = t0 + tr, id = __shfl(token_id, tr, 64);
     f32x4 u = {0, 0, 0, 0};
-    if (a >= 0 && r < p.R) {
+    if (id >= 0 && r < p.R) {
       const float* h = p.h + (size_t)t * Rp + r;
       for (int q0 = 0; q0 < slices; q0 += 4) {
         f32x4 v[4];
@@ -146,20 +189,26 @@ __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p
 #pragma unroll
         for (int q = 0; q < 4; ++q) u += q0 + q < slices ? v[q] : f32x4{0, 0, 0, 0};
       }
-      u *= p.scale[a];
+      u *= p.scale[id];
     }
     const u32x2 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w)};
-    *(u32x2*)&s_hi[row][r] = top;
-    *(u32x2*)&s_lo[row][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
-                                   pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
+    *(u32x2*)&s_hi[tr][r] = top;
+    *(u32x2*)&s_lo[tr][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
+                                  pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
   }
   __syncthreads();
+  if (c0 >= p.N) return;
+  if (!kEarly) {
+    load_b();
+    load_y();
+  }
   // the lane's token and its 8 ranks of each product
   u32x4 hi[MT][RC], lo[MT][RC];
   int mine[MT];
+  f32x4 acc[MT][2 * CG];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    mine[m] = __shfl(ids.id, 16 * m + row, 64);
+    mine[m] = __shfl(token_id, 16 * m + row, 64);
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
       const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
@@ -167,80 +216,53 @@ __global__ __launch_bounds__(256) void adapters_expand_kernel(QhAdaptersParams p
       hi[m][c] = SMALL && g >= 2 ? lo[m][c] : *(const u32x4*)&s_hi[16 * m + row][r0];
     }
   }
-  const u32x4 zero = {0, 0, 0, 0};
-  for (int i = 0; i < cols; ++i) {
-    const int c0 = ((blockIdx.x * cols + i) * 4 + wid) * 32 * CG;
-    if (c0 >= p.N) break;
-    f32x4 acc[MT][2 * CG];
-    u32x4 y[MT][CG];
+  auto product = [&](int n, int m, int q) {
+    f32x4 d = {0, 0, 0, 0};
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int c = 0; c < RC; ++c) {
+      d = mfma(b[n][c][q], hi[m][c], d);
+      if (!SMALL) d = mfma(b[n][c][q], lo[m][c], d);
+    }
+    return d;
+  };
+  // The first adapter's product is everybody's at first (and nobody's who has none: such rows are copied).
+  bool others = false;
+  while (count > 0) {
 #pragma unroll
-      for (int q = 0; q < 2 * CG; ++q) acc[m][q] = f32x4{0, 0, 0, 0};
-    TileIds tile = ids;
-    bool asked = false;
-    do {
-      int a[AT], count = 0;
-      u32x4 b[AT][RC][2 * CG];
-#pragma unroll
-      for (int n = 0; n < AT; ++n) {
-        if (n > 0 && tile.left == 0) continue;
-        uint64_t tokens;
-        a[n] = tile.left != 0 ? tile.next(tokens) : 0;
-        count = n + 1;
-#pragma unroll
-        for (int c = 0; c < RC; ++c) {
-          const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
-#pragma unroll
-          for (int q = 0; q < 2 * CG; ++q) {
-            const int col = min(c0 + 32 * (q / 2) + 8 * (row >> 2) + 4 * (q % 2) + (row & 3), p.N - 1);
-            b[n][c][q] = r0 < p.R ? load16(p.b + ((size_t)a[n] * p.N + col) * p.R + r0) : zero;
-          }
-        }
-      }
-      if (!asked) {
-        asked = true;
+    for (int n = 0; n < AT; ++n) {
+      if (n >= count) continue;
+      if (n == 0 && !others) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int q = 0; q < CG; ++q) {
-            const int t = min(t0 + 16 * m + row, p.T - 1), c = c0 + 32 * q + 8 * g;
-            y[m][q] = c < p.N ? load16(p.y + t * p.y_ts + c) : zero;
-          }
+          for (int q = 0; q < 2 * CG; ++q) acc[m][q] = product(n, m, q);
+        others = true;
+        continue;
       }
 #pragma unroll
-      for (int n = 0; n < AT; ++n) {
-        if (n >= count) continue;
-        f32x4 d[MT][2 * CG];
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int q = 0; q < 2 * CG; ++q) {
-            d[m][q] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < RC; ++c) {
-              d[m][q] = mfma(b[n][c][q], hi[m][c], d[m][q]);
-              if (!SMALL) d[m][q] = mfma(b[n][c][q], lo[m][c], d[m][q]);
-            }
-            if (mine[m] == a[n]) acc[m][q] = d[m][q];
-          }
-      }
-    } while (tile.left != 0);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < CG; ++q) {
-        const int t = t0 + 16 * m + row, c = c0 + 32 * q + 8 * g;
-        if (t >= p.T || c >= p.N || (mine[m] < 0 && p.out == p.y)) continue;
-        u32x4 z = y[m][q];
-        if (mine[m] >= 0) {  // a row without an adapter is copied as it is
-          const f32x4 u = acc[m][2 * q], v = acc[m][2 * q + 1];
-          z = u32x4{pack_bf2(bf_lo(z.x) + u.x, bf_hi(z.x) + u.y), pack_bf2(bf_lo(z.y) + u.z, bf_hi(z.y) + u.w),
-                    pack_bf2(bf_lo(z.z) + v.x, bf_hi(z.z) + v.y), pack_bf2(bf_lo(z.w) + v.z, bf_hi(z.w) + v.w)};
+        for (int q = 0; q < 2 * CG; ++q) {
+          const f32x4 d = product(n, m, q);
+          if (mine[m] == a[n]) acc[m][q] = d;
         }
-        *(u32x4*)(p.out + t * p.out_ts + c) = z;
-      }
+    }
+    load_b();
   }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int q = 0; q < CG; ++q) {
+      const int t = t0 + 16 * m + row, c = c0 + 32 * q + 8 * g;
+      if (t >= p.T || c >= p.N || (mine[m] < 0 && p.out == p.y)) continue;
+      u32x4 z = y[m][q];
+      if (mine[m] >= 0) {  // a row without an adapter is copied as it is
+        const f32x4 u = acc[m][2 * q], v = acc[m][2 * q + 1];
+        z = u32x4{pack_bf2(bf_lo(z.x) + u.x, bf_hi(z.x) + u.y), pack_bf2(bf_lo(z.y) + u.z, bf_hi(z.y) + u.w),
+                  pack_bf2(bf_lo(z.z) + v.x, bf_hi(z.z) + v.y), pack_bf2(bf_lo(z.w) + v.z, bf_hi(z.w) + v.w)};
+      }
+      *(u32x4*)(p.out + t * p.out_ts + c) = z;
+    }
 }
 
 // Slices of K whose partial sums the workspace holds.
@@ -250,6 +272,13 @@ template <int MT, int RT, int BLOCKS>
 void shrink(const QhAdaptersParams& p, int slices, int slice, int z, hipStream_t st) {
   const dim3 grid(slices, (p.T + 16 * MT - 1) / (16 * MT), z);
   adapters_shrink_kernel<MT, RT, BLOCKS><<<grid, 64 * kShrinkWaves, 0, st>>>(p, slice);
+}
+
+template <int WAVES, int MT, int RC, bool SMALL, int CG, int AT>
+void expand(const QhAdaptersParams& p, int slices, hipStream_t st) {
+  const int cols = 32 * CG * WAVES;
+  const dim3 grid((p.N + cols - 1) / cols, (p.T + 16 * MT - 1) / (16 * MT));
+  adapters_expand_kernel<WAVES, MT, RC, SMALL, CG, AT><<<grid, 64 * WAVES, 0, st>>>(p, slices);
 }
 
 }  // namespace
@@ -263,18 +292,21 @@ size_t qh_adapters_ws_bytes(int max_tokens, int R) {
 int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   const bool few = p.T <= 256;
   const int tiles = (p.T + 15) / 16, wide_tiles = (p.T + 31) / 32;
-  // K in slices until there are 512 workgroups, of a block a wave at least
-  const int step = 64 * kShrinkWaves, steps = (p.K + step - 1) / step;
+  // K in slices until there are 512 workgroups, each of eight blocks of 64 at least: a power of two,
+  // so that workgroups of a slice meet on the same XCDs (which get them in turn) and find its
+  // columns of A in their caches
   const bool two = !few && p.R <= 64;
-  int slices = min(max_slices(p.T), max(1, min(512 / (two ? wide_tiles : tiles), steps)));
-  const int slice = (steps + slices - 1) / slices * step;
+  const int most = min(max_slices(p.T), max(1, min(512 / (two ? wide_tiles : tiles), p.K / 512)));
+  int slices = 1;
+  while (2 * slices <= most) slices *= 2;
+  const int slice = ((p.K + slices - 1) / slices + 63) / 64 * 64;
   slices = (p.K + slice - 1) / slice;
-  // few tokens name an adapter each: one a workgroup; of prompts a tile has one, seldom more
-  const int z = few ? min(16, p.T) : 4;
+  // few tokens name an adapter each: one a workgroup; the tiles of long prompts have one, seldom more
+  const int z = max(2, min(min(16, p.T), 8192 / p.T));
   if (two) {
     if (p.R <= 16) shrink<2, 1, 3>(p, slices, slice, z, st);
     else if (p.R <= 32) shrink<2, 2, 2>(p, slices, slice, z, st);
-    else shrink<2, 4, 1>(p, slices, slice, z, st);
+    else shrink<2, 4, 2>(p, slices, slice, z, st);
   } else {
     if (p.R <= 16) shrink<1, 1, 3>(p, slices, slice, z, st);
     else if (p.R <= 32) shrink<1, 2, 2>(p, slices, slice, z, st);
@@ -282,21 +314,17 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
     else shrink<1, 8, 1>(p, slices, slice, z, st);
   }
 
-  // 32 tokens and 256 columns a workgroup at a time where that leaves four workgroups a CU, and then
-  // up to four times; otherwise 16 and 128
-  const int wide1 = (p.N + 255) / 256, cols = min(4, wide_tiles * wide1 / 1024);
-  if (cols == 0) {
-    const dim3 grid((p.N + 127) / 128, tiles);
-    if (p.R <= 16) adapters_expand_kernel<1, 1, true, 1, 8><<<grid, 256, 0, st>>>(p, slices, 1);
-    else if (p.R <= 32) adapters_expand_kernel<1, 1, false, 1, 8><<<grid, 256, 0, st>>>(p, slices, 1);
-    else if (p.R <= 64) adapters_expand_kernel<1, 2, false, 1, 4><<<grid, 256, 0, st>>>(p, slices, 1);
-    else adapters_expand_kernel<1, 4, false, 1, 2><<<grid, 256, 0, st>>>(p, slices, 1);
+  // 32 tokens and 512 columns a workgroup where that leaves two of them a CU, otherwise 16 and 128
+  if (wide_tiles * ((p.N + 511) / 512) < 512) {
+    if (p.R <= 16) expand<4, 1, 1, true, 1, 8>(p, slices, st);
+    else if (p.R <= 32) expand<4, 1, 1, false, 1, 8>(p, slices, st);
+    else if (p.R <= 64) expand<4, 1, 2, false, 1, 4>(p, slices, st);
+    else expand<4, 1, 4, false, 1, 2>(p, slices, st);
   } else {
-    const dim3 grid((wide1 + cols - 1) / cols, wide_tiles);
-    if (p.R <= 16) adapters_expand_kernel<2, 1, true, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 32) adapters_expand_kernel<2, 1, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
-    else if (p.R <= 64) adapters_expand_kernel<2, 2, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
-    else adapters_expand_kernel<2, 4, false, 2, 1><<<grid, 256, 0, st>>>(p, slices, cols);
+    if (p.R <= 16) expand<8, 2, 1, true, 2, 1>(p, slices, st);
+    else if (p.R <= 32) expand<8, 2, 1, false, 2, 1>(p, slices, st);
+    else if (p.R <= 64) expand<8, 2, 2, false, 1, 1>(p, slices, st);
+    else expand<4, 2, 4, false, 1, 1>(p, slices, st);
   }
   return 0;
 }
