@@ -118,24 +118,73 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapters_shrink_kernel(QhAd
 }
 
 // ---- out = y + scale B h -------------------------------------------------------------------
-// A wave: 16 MT tokens and 32 CG columns; WAVES of them side by side share the tile's h.  The rows of B
-// are the first operand, in an order that leaves each lane 8 consecutive columns of one token: of a
-// pair of products, the first has columns 8 m + 0 .. 3 and the second 8 m + 4 .. 7 of each eight.
-// Ranks go 32 to a product, high and low parts one after the other; rank 16 (and 8) has both parts in
-// one, side by side.  The rows of B of AT adapters are on their way at once.
-// Of eight waves two workgroups fit a CU where a wave takes 128 registers at most.
-template <int WAVES, int MT, int RC, bool SMALL, int CG, int AT>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 1) void adapters_expand_kernel(QhAdaptersParams p, int slices) {
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-  const int t0 = blockIdx.y * 16 * MT, c0 = (blockIdx.x * WAVES + wid) * 32 * CG;
-  const int Rp = 16 * ((p.R + 15) / 16);
-  const u32x4 zero = {0, 0, 0, 0};
-  TileIds tile(p, t0, 16 * MT);
-  const int token_id = tile.id;
+// The rows of B are the first operand, in an order that leaves each lane 8 consecutive columns of one
+// token: of a pair of products, the first has columns 8 m + 0 .. 3 and the second 8 m + 4 .. 7 of each
+// eight.  Ranks go 32 to a product, high and low parts one after the other; rank 16 (and 8) has both
+// parts in one, side by side (SMALL).
+template <int RC, bool SMALL>
+__device__ __forceinline__ u32x4 load_b(const QhAdaptersParams& p, int a, int c0, int q, int c) {
+  const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
+  const int col = min(c0 + 32 * (q / 2) + 8 * (row >> 2) + 4 * (q % 2) + (row & 3), p.N - 1);
+  return r0 < p.R ? load16(p.b + ((size_t)a * p.N + col) * p.R + r0) : u32x4{0, 0, 0, 0};
+}
 
+// A tile's h, summed over the slices of K, scaled and in two parts, once a workgroup: 4 ranks a thread.
+// A row's 16 bytes of padding spread its reads over the banks.
+template <int TOKENS, int RC, bool SMALL>
+struct TileH {
+  static constexpr int kRanks = SMALL ? 16 : 32 * RC;
+  uint16_t hi[TOKENS][kRanks + 8], lo[TOKENS][kRanks + 8];
+
+  __device__ __forceinline__ void join(const QhAdaptersParams& p, int t0, int token_id, int slices) {
+    const int Rp = 16 * ((p.R + 15) / 16);
+    for (int i = threadIdx.x; i < TOKENS * kRanks / 4; i += blockDim.x) {
+      const int row = i / (kRanks / 4), r = 4 * (i % (kRanks / 4)), id = __shfl(token_id, row, 64);
+      f32x4 u = {0, 0, 0, 0};
+      if (id >= 0 && r < p.R) {
+        const float* h = p.h + (size_t)(t0 + row) * Rp + r;
+        for (int q0 = 0; q0 < slices; q0 += 4) {
+          f32x4 v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = *(const f32x4*)(h + (size_t)min(q0 + q, slices - 1) * p.T * Rp);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) u += q0 + q < slices ? v[q] : f32x4{0, 0, 0, 0};
+        }
+        u *= p.scale[id];
+      }
+      const u32x2 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w)};
+      *(u32x2*)&hi[row][r] = top;
+      *(u32x2*)&lo[row][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
+                                   pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
+    }
+    __syncthreads();
+  }
+  // The lane's token of sub-tile m and its 8 ranks of product c.
+  __device__ __forceinline__ void get(int m, int c, u32x4& high, u32x4& low) const {
+    const int row = 16 * m + (threadIdx.x & 15), g = (threadIdx.x & 63) >> 4, r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
+    low = *(const u32x4*)&lo[row][r0];
+    high = SMALL && g >= 2 ? low : *(const u32x4*)&hi[row][r0];
+  }
+};
+
+// y plus a lane's 8 columns of a product.
+__device__ __forceinline__ u32x4 add8(u32x4 y, f32x4 u, f32x4 v) {
+  return u32x4{pack_bf2(bf_lo(y.x) + u.x, bf_hi(y.x) + u.y), pack_bf2(bf_lo(y.y) + u.z, bf_hi(y.y) + u.w),
+               pack_bf2(bf_lo(y.z) + v.x, bf_hi(y.z) + v.y), pack_bf2(bf_lo(y.w) + v.z, bf_hi(y.w) + v.w)};
+}
+
+// Few tokens, or few columns.  A wave: 16 tokens and 32 columns.  What it waits for is B, so the rows of
+// AT adapters are on their way at once, and the first of them and y before h is there.
+template <int RC, bool SMALL, int AT>
+__global__ __launch_bounds__(256) void adapters_expand_few_kernel(QhAdaptersParams p, int slices) {
+  __shared__ TileH<16, RC, SMALL> s_h;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int t0 = blockIdx.y * 16, c0 = (blockIdx.x * 4 + wid) * 32, t = t0 + row, col = c0 + 8 * g;
+  TileIds tile(p, t0, 16);
+  const int token_id = tile.id, mine = __shfl(tile.id, row, 64);
   int a[AT], count;
-  u32x4 b[AT][RC][2 * CG];
-  auto load_b = [&]() {
+  u32x4 b[AT][RC][2];
+  auto load = [&]() {
     count = 0;
 #pragma unroll
     for (int n = 0; n < AT; ++n) {
@@ -144,125 +193,106 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 1) void adapters_expan
       a[n] = tile.next(tokens);
       count = n + 1;
 #pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
+      for (int c = 0; c < RC; ++c)
 #pragma unroll
-        for (int q = 0; q < 2 * CG; ++q) {
-          const int col = min(c0 + 32 * (q / 2) + 8 * (row >> 2) + 4 * (q % 2) + (row & 3), p.N - 1);
-          b[n][c][q] = r0 < p.R ? load16(p.b + ((size_t)a[n] * p.N + col) * p.R + r0) : zero;
-        }
-      }
+        for (int q = 0; q < 2; ++q) b[n][c][q] = load_b<RC, SMALL>(p, a[n], c0, q, c);
     }
   };
-  u32x4 y[MT][CG];
-  auto load_y = [&]() {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int q = 0; q < CG; ++q) {
-        const int t = min(t0 + 16 * m + row, p.T - 1), c = c0 + 32 * q + 8 * g;
-        y[m][q] = c < p.N ? load16(p.y + t * p.y_ts + c) : zero;
-      }
-  };
-  // Few tokens wait for B most: it goes first, y behind it.  Of a prompt y is most of the bytes, and h
-  // would wait behind it (loads come back in order): 3700 tokens 44 us against 35.
-  constexpr bool kEarly = AT > 1;
-  if (kEarly) {
-    load_b();
-    load_y();
-  }
-
-  // The tile's h, summed over the slices of K, scaled and in two parts, once a workgroup: 4 ranks a
-  // thread.  A row's 16 bytes of padding spread the reads below over the banks.
-  constexpr int kRow = (SMALL ? 16 : 32 * RC) + 8;
-  __shared__ uint16_t s_hi[16 * MT][kRow], s_lo[16 * MT][kRow];
-  constexpr int kQuads = SMALL ? 4 : 8 * RC;
-  for (int i = threadIdx.x; i < 16 * MT * kQuads; i += 64 * WAVES) {
-    const int tr = i / kQuads, r = 4 * (i % kQuads), t = t0 + tr, id = __shfl(token_id, tr, 64);
-    f32x4 u = {0, 0, 0, 0};
-    if (id >= 0 && r < p.R) {
-      const float* h = p.h + (size_t)t * Rp + r;
-      for (int q0 = 0; q0 < slices; q0 += 4) {
-        f32x4 v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = *(const f32x4*)(h + (size_t)min(q0 + q, slices - 1) * p.T * Rp);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) u += q0 + q < slices ? v[q] : f32x4{0, 0, 0, 0};
-      }
-      u *= p.scale[id];
-    }
-    const u32x2 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w)};
-    *(u32x2*)&s_hi[tr][r] = top;
-    *(u32x2*)&s_lo[tr][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
-                                  pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
-  }
-  __syncthreads();
+  load();
+  u32x4 y = {0, 0, 0, 0};
+  if (t < p.T && col < p.N) y = load16(p.y + t * p.y_ts + col);
+  s_h.join(p, t0, token_id, slices);
   if (c0 >= p.N) return;
-  if (!kEarly) {
-    load_b();
-    load_y();
-  }
-  // the lane's token and its 8 ranks of each product
-  u32x4 hi[MT][RC], lo[MT][RC];
-  int mine[MT];
-  f32x4 acc[MT][2 * CG];
+  u32x4 hi[RC], lo[RC];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    mine[m] = __shfl(token_id, 16 * m + row, 64);
-#pragma unroll
-    for (int c = 0; c < RC; ++c) {
-      const int r0 = SMALL ? 8 * (g & 1) : 32 * c + 8 * g;
-      lo[m][c] = *(const u32x4*)&s_lo[16 * m + row][r0];
-      hi[m][c] = SMALL && g >= 2 ? lo[m][c] : *(const u32x4*)&s_hi[16 * m + row][r0];
-    }
-  }
-  auto product = [&](int n, int m, int q) {
-    f32x4 d = {0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c < RC; ++c) {
-      d = mfma(b[n][c][q], hi[m][c], d);
-      if (!SMALL) d = mfma(b[n][c][q], lo[m][c], d);
-    }
-    return d;
-  };
-  // The first adapter's product is everybody's at first (and nobody's who has none: such rows are copied).
-  bool others = false;
+  for (int c = 0; c < RC; ++c) s_h.get(0, c, hi[c], lo[c]);
+  f32x4 acc[2] = {};
   while (count > 0) {
 #pragma unroll
     for (int n = 0; n < AT; ++n) {
       if (n >= count) continue;
-      if (n == 0 && !others) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+      for (int q = 0; q < 2; ++q) {
+        f32x4 d = {0, 0, 0, 0};
 #pragma unroll
-          for (int q = 0; q < 2 * CG; ++q) acc[m][q] = product(n, m, q);
-        others = true;
-        continue;
+        for (int c = 0; c < RC; ++c) {
+          d = mfma(b[n][c][q], hi[c], d);
+          if (!SMALL) d = mfma(b[n][c][q], lo[c], d);
+        }
+        if (mine == a[n]) acc[q] = d;
       }
+    }
+    load();
+  }
+  if (t >= p.T || col >= p.N || (mine < 0 && p.out == p.y)) return;
+  // a row without an adapter is copied as it is
+  *(u32x4*)(p.out + t * p.out_ts + col) = mine >= 0 ? add8(y, acc[0], acc[1]) : y;
+}
+
+// Prompts.  A wave: 16 MT tokens and 32 CG columns, whose rows of B stay in registers while the tokens go
+// by, 16 at a time; eight waves side by side share h.  What counts is y and out: y is on its way at
+// once, behind h (loads come back in order).
+template <int MT, int RC, bool SMALL, int CG>
+__global__ __launch_bounds__(512, 4) void adapters_expand_kernel(QhAdaptersParams p, int slices) {
+  __shared__ TileH<16 * MT, RC, SMALL> s_h;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int t0 = blockIdx.y * 16 * MT, c0 = (blockIdx.x * 8 + wid) * 32 * CG, col = c0 + 8 * g;
+  TileIds tile(p, t0, 16 * MT);
+  const int token_id = tile.id;
+  s_h.join(p, t0, token_id, slices);
+  if (c0 >= p.N) return;
+  int mine[MT];
+  u32x4 y[MT][CG];
+  bool asked = false;
+  do {
+    uint64_t tokens = 0;
+    const int a = tile.left != 0 ? tile.next(tokens) : -1;
+    u32x4 b[RC][2 * CG];
+    if (a >= 0) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int c = 0; c < RC; ++c)
+#pragma unroll
+        for (int q = 0; q < 2 * CG; ++q) b[c][q] = load_b<RC, SMALL>(p, a, c0, q, c);
+    }
+    if (!asked) {
+      asked = true;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        mine[m] = __shfl(token_id, 16 * m + row, 64);
+#pragma unroll
+        for (int q = 0; q < CG; ++q) {
+          const int t = min(t0 + 16 * m + row, p.T - 1);
+          y[m][q] = col + 32 * q < p.N ? load16(p.y + t * p.y_ts + col + 32 * q) : u32x4{0, 0, 0, 0};
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (((tokens >> (16 * m)) & 0xFFFF) == 0) continue;
+      f32x4 d[2 * CG] = {};
+#pragma unroll
+      for (int c = 0; c < RC; ++c) {
+        u32x4 hi, lo;
+        s_h.get(m, c, hi, lo);
 #pragma unroll
         for (int q = 0; q < 2 * CG; ++q) {
-          const f32x4 d = product(n, m, q);
-          if (mine[m] == a[n]) acc[m][q] = d;
+          d[q] = mfma(b[c][q], hi, d[q]);
+          if (!SMALL) d[q] = mfma(b[c][q], lo, d[q]);
         }
+      }
+#pragma unroll
+      for (int q = 0; q < CG; ++q)
+        if (mine[m] == a && col + 32 * q < p.N)
+          *(u32x4*)(p.out + (long long)(t0 + 16 * m + row) * p.out_ts + col + 32 * q) = add8(y[m][q], d[2 * q], d[2 * q + 1]);
     }
-    load_b();
-  }
+  } while (tile.left != 0);
+  if (p.out == p.y) return;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int q = 0; q < CG; ++q) {
-      const int t = t0 + 16 * m + row, c = c0 + 32 * q + 8 * g;
-      if (t >= p.T || c >= p.N || (mine[m] < 0 && p.out == p.y)) continue;
-      u32x4 z = y[m][q];
-      if (mine[m] >= 0) {  // a row without an adapter is copied as it is
-        const f32x4 u = acc[m][2 * q], v = acc[m][2 * q + 1];
-        z = u32x4{pack_bf2(bf_lo(z.x) + u.x, bf_hi(z.x) + u.y), pack_bf2(bf_lo(z.y) + u.z, bf_hi(z.y) + u.w),
-                  pack_bf2(bf_lo(z.z) + v.x, bf_hi(z.z) + v.y), pack_bf2(bf_lo(z.w) + v.z, bf_hi(z.w) + v.w)};
-      }
-      *(u32x4*)(p.out + t * p.out_ts + c) = z;
-    }
+    for (int q = 0; q < CG; ++q)  // rows without an adapter are copied as they are
+      if (mine[m] < 0 && t0 + 16 * m + row < p.T && col + 32 * q < p.N)
+        *(u32x4*)(p.out + (long long)(t0 + 16 * m + row) * p.out_ts + col + 32 * q) = y[m][q];
 }
 
 // Slices of K whose partial sums the workspace holds.
@@ -274,11 +304,15 @@ void shrink(const QhAdaptersParams& p, int slices, int slice, int z, hipStream_t
   adapters_shrink_kernel<MT, RT, BLOCKS><<<grid, 64 * kShrinkWaves, 0, st>>>(p, slice);
 }
 
-template <int WAVES, int MT, int RC, bool SMALL, int CG, int AT>
+template <int RC, bool SMALL, int AT>
+void expand_few(const QhAdaptersParams& p, int slices, hipStream_t st) {
+  adapters_expand_few_kernel<RC, SMALL, AT><<<dim3((p.N + 127) / 128, (p.T + 15) / 16), 256, 0, st>>>(p, slices);
+}
+
+template <int MT, int RC, bool SMALL, int CG>
 void expand(const QhAdaptersParams& p, int slices, hipStream_t st) {
-  const int cols = 32 * CG * WAVES;
-  const dim3 grid((p.N + cols - 1) / cols, (p.T + 16 * MT - 1) / (16 * MT));
-  adapters_expand_kernel<WAVES, MT, RC, SMALL, CG, AT><<<grid, 64 * WAVES, 0, st>>>(p, slices);
+  const int cols = 256 * CG;
+  adapters_expand_kernel<MT, RC, SMALL, CG><<<dim3((p.N + cols - 1) / cols, (p.T + 16 * MT - 1) / (16 * MT)), 512, 0, st>>>(p, slices);
 }
 
 }  // namespace
@@ -306,7 +340,7 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   if (two) {
     if (p.R <= 16) shrink<2, 1, 3>(p, slices, slice, z, st);
     else if (p.R <= 32) shrink<2, 2, 2>(p, slices, slice, z, st);
-    else shrink<2, 4, 2>(p, slices, slice, z, st);
+    else shrink<2, 4, 1>(p, slices, slice, z, st);
   } else {
     if (p.R <= 16) shrink<1, 1, 3>(p, slices, slice, z, st);
     else if (p.R <= 32) shrink<1, 2, 2>(p, slices, slice, z, st);
@@ -314,17 +348,17 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
     else shrink<1, 8, 1>(p, slices, slice, z, st);
   }
 
-  // 32 tokens and 512 columns a workgroup where that leaves two of them a CU, otherwise 16 and 128
-  if (wide_tiles * ((p.N + 511) / 512) < 512) {
-    if (p.R <= 16) expand<4, 1, 1, true, 1, 8>(p, slices, st);
-    else if (p.R <= 32) expand<4, 1, 1, false, 1, 8>(p, slices, st);
-    else if (p.R <= 64) expand<4, 1, 2, false, 1, 4>(p, slices, st);
-    else expand<4, 1, 4, false, 1, 2>(p, slices, st);
+  // 64 tokens and 512 columns a workgroup where that leaves two of them a CU, otherwise 16 and 128
+  if (((p.T + 63) / 64) * ((p.N + 511) / 512) < 512) {
+    if (p.R <= 16) expand_few<1, true, 8>(p, slices, st);
+    else if (p.R <= 32) expand_few<1, false, 8>(p, slices, st);
+    else if (p.R <= 64) expand_few<2, false, 4>(p, slices, st);
+    else expand_few<4, false, 2>(p, slices, st);
   } else {
-    if (p.R <= 16) expand<8, 2, 1, true, 2, 1>(p, slices, st);
-    else if (p.R <= 32) expand<8, 2, 1, false, 2, 1>(p, slices, st);
-    else if (p.R <= 64) expand<8, 2, 2, false, 1, 1>(p, slices, st);
-    else expand<4, 2, 4, false, 1, 1>(p, slices, st);
+    if (p.R <= 16) expand<2, 1, true, 2>(p, slices, st);
+    else if (p.R <= 32) expand<2, 1, false, 2>(p, slices, st);
+    else if (p.R <= 64) expand<4, 2, false, 2>(p, slices, st);
+    else expand<4, 4, false, 1>(p, slices, st);
   }
   return 0;
 }
