@@ -26,6 +26,7 @@
 // sum.  A weight is 2^-36 off its value, alike wherever it is used.  Weights below 2^-63.75 of the
 // largest are none.
 #include "qh_common.h"
+#include "qh_scan.h"
 #include "qh_serve.h"
 
 namespace {
@@ -40,7 +41,6 @@ constexpr int kList = 65536;           // places of a row's list
 constexpr int kHeld = 20480;           // 32-bit words of LDS for it
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
 constexpr uint64_t kMassMask = (1ull << 50) - 1;  // a bin: weights below bit 50, the count above
-constexpr int kNone = 0x7FFFFFFF;
 static_assert(kMaxChunks <= kBins && NT == 2 * kBins, "a thread a chunk, two a bin");
 
 struct Chunk {      // what a workgroup hands on
@@ -256,47 +256,6 @@ __device__ __forceinline__ float value_of(uint64_t key, int ib) {
 __device__ __forceinline__ int index_of_key(uint64_t key, int ib) { return (1 << ib) - 1 - (int)(key & ((1 << ib) - 1)); }
 
 // ---- workgroup sums ----------------------------------------------------------------------------
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T dpp_or_zero(T v) {
-  static_assert(sizeof(T) == 8, "two registers");
-  const u32x2 u = __builtin_bit_cast(u32x2, v);
-  const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, false),
-                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, false)};
-  return __builtin_bit_cast(T, r);
-}
-template <typename T>
-__device__ __forceinline__ T lane63(T v) {
-  const u32x2 u = __builtin_bit_cast(u32x2, v);
-  const u32x2 r = {(uint32_t)__builtin_amdgcn_readlane((int)u.x, 63), (uint32_t)__builtin_amdgcn_readlane((int)u.y, 63)};
-  return __builtin_bit_cast(T, r);
-}
-// Exclusive prefix over the wave and its total (64-bit values), by moves between lanes within the
-// registers: shifts within rows of 16, then the rows' last lanes handed on.
-template <typename T>
-__device__ __forceinline__ T wave_excl(T v, T& all) {
-  T x = v;
-  x += dpp_or_zero<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
-  x += dpp_or_zero<0x112, 0xF>(x);
-  x += dpp_or_zero<0x114, 0xF>(x);
-  x += dpp_or_zero<0x118, 0xF>(x);
-  x += dpp_or_zero<0x142, 0xA>(x);  // row_bcast 15 into rows 1 and 3
-  x += dpp_or_zero<0x143, 0xC>(x);  // row_bcast 31 into rows 2 and 3
-  all = lane63(x);
-  return dpp_or_zero<0x138, 0xF>(x);  // wave_shr 1
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_min(int v) {
-  return min(v, __builtin_amdgcn_update_dpp(kNone, v, CTRL, ROWS, 0xF, false));
-}
-__device__ __forceinline__ int wave_min(int v) {
-  v = dpp_min<0x111, 0xF>(v);
-  v = dpp_min<0x112, 0xF>(v);
-  v = dpp_min<0x114, 0xF>(v);
-  v = dpp_min<0x118, 0xF>(v);
-  v = dpp_min<0x142, 0xA>(v);
-  v = dpp_min<0x143, 0xC>(v);
-  return __builtin_amdgcn_readlane(v, 63);
-}
 // Exclusive prefix over the threads, and the total; a fixed order of additions.
 template <typename T>
 __device__ __forceinline__ T block_excl(T v, T* s_v, T& all) {
