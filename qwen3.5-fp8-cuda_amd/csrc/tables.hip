@@ -22,8 +22,9 @@
 
 namespace {
 
-// Tokens whose flat rows the one workgroup writes itself; above, a second launch does.
-constexpr int kFillInline = 65536;
+// Tokens whose flat rows the one workgroup writes itself; above, a second launch does (500 rows, 12000
+// tokens: 14.0 us in one launch, 12.2 in two; the second takes 4).
+constexpr int kFillInline = 2048;
 
 // Exclusive prefix sum over the workgroup's threads.
 template <int NT>
@@ -203,19 +204,19 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(QhTablesParams p) {
   for (int b = threadIdx.x; b <= kTablesMaxRows; b += 256) s_tok[b] = p.start[min(b, p.n_rows)];
   __syncthreads();
   const int n_tok = s_tok[kTablesMaxRows];
-  for (int t = blockIdx.x * 1024 + threadIdx.x, e = 0; e < 4 && t < p.T; ++e, t += 256) {
-    const bool there = t < n_tok;
-    const int b = there ? row_of<kTablesMaxRows>(s_tok, t) : -1;
-    p.seq[t] = b;
-    p.at[t] = there ? p.length_out[b] - (s_tok[b + 1] - t) : -1;
-  }
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.T) return;
+  const bool there = t < n_tok;
+  const int b = there ? row_of<kTablesMaxRows>(s_tok, t) : -1;
+  p.seq[t] = b;
+  p.at[t] = there ? p.length_out[b] - (s_tok[b + 1] - t) : -1;
 }
 
 }  // namespace
 
 int qh_launch_tables(const QhTablesParams& p, hipStream_t st) {
-  if (p.n_rows <= 512 && p.T <= 2048) tables_step_kernel<256><<<1, 256, 0, st>>>(p);
+  if (p.n_rows <= 512) tables_step_kernel<256><<<1, 256, 0, st>>>(p);
   else tables_step_kernel<1024><<<1, 1024, 0, st>>>(p);
-  if (p.seq && p.T > kFillInline) tables_fill_kernel<<<(p.T + 1023) / 1024, 256, 0, st>>>(p);
+  if (p.seq && p.T > kFillInline) tables_fill_kernel<<<(p.T + 255) / 256, 256, 0, st>>>(p);
   return 0;
 }

@@ -61,7 +61,7 @@ def test_random_batches(seed):
     check(state, page, rng.choice([1, rows, 3 * rows, 5000]) if flat else rows, flat, apart=rng.random() < 0.5)
 
 
-@pytest.mark.parametrize("T", [1, 4095, 4096, 4097, 8191, 20000])
+@pytest.mark.parametrize("T", [1, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 20000])
 def test_long_steps(T):
     """Prompts of thousands of tokens: flat rows at the border between one launch and two."""
     rng = random.Random(T)
