@@ -91,7 +91,7 @@ __device__ __forceinline__ uint64_t bits(double d) { return (uint64_t)__double_a
 
 // ---- a row's settings ------------------------------------------------------------------------
 struct Settings {
-  double c4;       // t = x c4
+  double c4, c4_inv;  // t = x c4, x = t c4_inv
   double heat, p, m;
   int k;           // 0: all
   bool first;      // the first of the largest is the token
@@ -101,6 +101,7 @@ struct Settings {
     first = !(t > 0.0f);
     heat = first ? 1.0 : (double)t;
     c4 = 4.0 * 1.4426950408889634 / heat;
+    c4_inv = heat * 0.17328679513998632;  // ln(2) / 4
     k = q.top_k ? q.top_k[b] : 0;
     if (k >= q.V || k < 0) k = 0;
     p = q.top_p ? (double)q.top_p[b] : 1.0;
@@ -143,11 +144,11 @@ struct Scale {
   bool quick;
   float least;
   uint32_t first;
-  __device__ __forceinline__ Scale(double c4_, float top_) : c4(c4_), top(top_) {
+  __device__ __forceinline__ Scale(const Settings& set, float top_) : c4(set.c4), top(top_) {
     const double t = (double)top * c4;
     far = !(fabs(t) < 1125899906842624.0);
     base = fabsf(top) == INFINITY ? (double)top : far ? t : (t + kRound) - kRound;
-    least = (float)((base - 400.0) / c4);
+    least = (float)((base - 400.0) * set.c4_inv);
     quick = !far && fabs(base) < 67108864.0 && least > -INFINITY;
     first = (uint32_t)bits(kRound + base);
   }
@@ -177,9 +178,9 @@ struct Scale {
 // most logits fail without their weight.  Where all have to be looked at, all pass.
 struct Ends {
   float lo, hi;
-  __device__ __forceinline__ Ends(const Scale& s, int bin_lo, int bin_hi) {
-    lo = (float)((s.base - bin_hi - 0.75) / s.c4);
-    hi = (float)((s.base - bin_lo + 0.75) / s.c4);
+  __device__ __forceinline__ Ends(const Settings& set, const Scale& s, int bin_lo, int bin_hi) {
+    lo = (float)((s.base - bin_hi - 0.75) * set.c4_inv);
+    hi = (float)((s.base - bin_lo + 0.75) * set.c4_inv);
     const float slack = 1e-6f * fmaxf(fabsf(lo), fabsf(hi));
     lo -= slack;
     hi += slack;
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
         if (x[r][e] == top) top_at = index_of(c, r) + e;
     top_at = block_min(top_at, s.i);
   }
-  const Scale scale(set.c4, top);
+  const Scale scale(set, top);
   double mass = 0.0;
   if (!set.first || p.logprob) {
     unsigned long long* mine = (unsigned long long*)&s_hist[tid & (kCopies - 1)];
@@ -493,14 +494,16 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
         }
     }
     __syncthreads();
-    if (tid < kBins) {
+    if (tid < kBins) {  // four whole waves
       uint64_t v = 0;
 #pragma unroll
       for (int q = 0; q < kCopies; ++q) v += s_hist[tid * kCopies + q];
       if (filtered) w.hist[(row + c) * kBins + tid] = v;
-      mass = (double)(v & kMassMask) * quarter(tid);
+      wave_excl((double)(v & kMassMask) * quarter(tid), mass);
+      if ((tid & 63) == 0) s.d[0][tid >> 6] = mass;
     }
-    mass = block_total(mass, s.d[0]);
+    __syncthreads();
+    mass = (s.d[0][0] + s.d[0][1]) + (s.d[0][2] + s.d[0][3]);
   }
   if (tid == 0) w.chunk[row + c] = Chunk{scale.base, mass, top, top_at};
 }
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
     return;
   }
-  const Scale scale(set.c4, row_top);
+  const Scale scale(set, row_top);
   const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(below(scale.base, mine.base)) : 0.0;
   auto every = [](float, int, int) { return true; };
   if (!filtered) {
@@ -655,7 +658,7 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
 
   // this chunk's weight before the range, and how many of its logits are in the range
   const Settings set(p, b);
-  const Scale scale(set.c4, plan.top);
+  const Scale scale(set, plan.top);
   const double off = below(scale.base, w.chunk[row + c].base);
   double sure = 0.0;
   uint64_t n = 0;
@@ -681,7 +684,7 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
     w.span[row + c] = int2{(int)s_n, (int)n_all};
   }
   __syncthreads();
-  const Ends ends(scale, plan.lo, plan.hi);
+  const Ends ends(set, scale, plan.lo, plan.hi);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
 #pragma unroll
@@ -709,8 +712,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
   const Settings set(p, b);
-  const Scale scale(set.c4, plan.top);
-  const Ends ends(scale, plan.lo, plan.hi);
+  const Scale scale(set, plan.top);
+  const Ends ends(set, scale, plan.lo, plan.hi);
   const size_t row = (size_t)b * chunks;
   const uint64_t* list = w.list + (size_t)b * places;
   const int n_list = plan.n_list;
