@@ -42,6 +42,7 @@ PyObject* step_tables(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     const int64_t n_pages = pool ? pool->size(0) : 0;
     a.good = a.good && is_int(n) && is_int(max_pages) && is_int(n_pages) && is_int(T);
     if (a.good) {
+      if (flat && T == 0) seq = start;  // an empty tensor's address is null, which would say: one token a row
       Py_BEGIN_ALLOW_THREADS
       rc = entry(pages, (int)n, (int)max_pages, page_size, length, fresh, done, free_pages, (int)n_pages, n_free, length_out,
                  n_free_out, at, seq, (int)T, start, last, stream);

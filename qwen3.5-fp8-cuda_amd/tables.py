@@ -31,6 +31,8 @@ class PageTables:
         _need(length, "length", _INT, (len(pages),), dev)
         _need(free, "free", _INT, (None,), dev)
         _need(n_free, "n_free", _INT, (1,), dev)
+        if not 8 <= page_size < 1 << 31 or page_size % 8:
+            raise ValueError(f"page_size: a positive multiple of 8, got {page_size}")
         self.pages, self.length, self.free, self.n_free = pages, length, free, n_free
         self.page_size, self.n_rows, self.dev, self.device = int(page_size), len(pages), dev, pages.device
         self._entry = abi.address("qh_page_tables_step")

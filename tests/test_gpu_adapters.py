@@ -155,6 +155,38 @@ def test_strided_and_in_place(T):
     assert torch.equal(got, p.add(same.contiguous(), ids.to(DEV), y.to(DEV), ws))
 
 
+@pytest.mark.parametrize("T", [3, 520])
+def test_offsets_past_32_bits(T):
+    """Tokens so far apart that the last ones lie behind element 2^31 of x, y and out."""
+    c = case(T, 16, 128, 9216 if T > 3 else 72, 3, T)
+    want = check(c)
+    x, ids, y, a, b, scale = c
+    stride = 2**32 // T // 8 * 8
+
+    def apart(t):
+        far = torch.empty((T - 1) * stride + t.shape[1], dtype=BF, device=DEV).as_strided(t.shape, (stride, 1))
+        return far.copy_(t.to(DEV))
+    out = apart(torch.zeros_like(y))
+    pool(a, b, scale).add(apart(x), ids.to(DEV), apart(y), adapters.adapters_workspace(T, 16, device=DEV), out=out)
+    assert torch.equal(out, want)
+
+
+def test_adapters_past_32_bits():
+    """A pool of more than 2^31 elements, of which the last adapters are named."""
+    n, R, K, N = 8200, 128, 2056, 8
+    g = gen(2)
+    a = torch.zeros(n, R, K, dtype=BF, device=DEV)
+    b = torch.zeros(n, N, R, dtype=BF, device=DEV)
+    last = [n - 1, n - 2, 0]
+    x, _, y, la, lb, scale = case(3, R, K, N, 3, 5)
+    a[last], b[last] = la.to(DEV), lb.to(DEV)
+    out = adapters.Adapters(a, b, scale[:1].expand(n).contiguous().to(DEV)).add(
+        x.to(DEV), torch.tensor(last, dtype=INT, device=DEV), y.to(DEV), adapters.adapters_workspace(3, R, device=DEV))
+    want, err = reference(x, torch.arange(3), y, la, lb, scale[:1].expand(3))
+    assert bool(((out.cpu().double() - want).abs() <= err).all())
+    del g
+
+
 def test_repeats_are_equal_and_streams_apart():
     """The same call again, two calls at once on two streams with workspaces of their own, and a captured one
     replayed with other ids between eager calls: all give the same bits."""

@@ -320,6 +320,19 @@ def test_repeats_streams_and_replays():
         assert out.tolist() == (then if i % 2 else want) and lp.tolist() == (then_lp if i % 2 else want_lp), i
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_offsets_past_32_bits(dtype):
+    """Rows 2^31 + 24 elements apart."""
+    g, rng = gen(21), random.Random(21)
+    B, V, stride = 3, 20000, 2**31 + 24
+    x, u = logits(g, B, V, dtype), draws(rng, B)
+    s = [SETTINGS[3], SETTINGS[0], SETTINGS[1]]
+    want = check(x, u, s)
+    far = torch.empty((B - 1) * stride + V, dtype=dtype, device=DEV).as_strided((B, V), (stride, 1))
+    far.copy_(x.to(DEV))
+    assert run(far, u, s)[0] == want
+
+
 def test_many_rows():
     """As many rows as the grid's axis is long, two logits each."""
     n = 65535

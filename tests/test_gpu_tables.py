@@ -109,6 +109,19 @@ def test_no_rows():
     t.step(torch.zeros(0, dtype=INT, device=DEV), torch.empty(0, dtype=INT, device=DEV))
 
 
+def test_no_room_for_any_token():
+    state = ([[3, -7], [1, -7]], [5, 8], (2, [0, 2, -9, -9]), [1, 1], [0, 1])
+    want = ref.step(*state[:2], state[2], state[3], state[4], 8, 0, True)
+    assert want["start"] == [0, 0, 0] and want["length"] == [5, 0]
+    check(state, 8, 0, True)
+
+
+@pytest.mark.parametrize("page_size", [0, 12, -8, 2**32 + 16])
+def test_a_page_size_that_is_none(page_size):
+    with pytest.raises(ValueError, match="page_size"):
+        tables.PageTables.alloc(2, 2, 4, page_size, device=DEV)
+
+
 def test_state_out_of_range_stays_in_bounds():
     """Lengths and counts that no step leaves behind: nothing outside the tensors is touched."""
     e = lambda v: torch.tensor(v, dtype=INT, device=DEV)   # noqa: E731

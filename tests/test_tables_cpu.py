@@ -68,6 +68,13 @@ def test_host_hands_on_pointers_and_sizes():
     assert got == 0 and s[6] is None and s[13:17] == (None, 3, None, None)
 
 
+def test_host_keeps_a_step_without_room_a_ragged_one():
+    z = torch.zeros(0, dtype=INT)
+    a = args(at=z, seq=z)
+    got, s = host(a.values())
+    assert got == 0 and s[13] is not None and s[14] == 0 and s[15] == a["start"].data_ptr()
+
+
 @pytest.mark.parametrize("bad", [
     dict(pages=None), dict(pages=torch.zeros(3, 4)), dict(pages=torch.zeros(4, 3, dtype=INT).t()),
     dict(pages=torch.zeros(12, dtype=INT)), dict(length=torch.zeros(4, dtype=INT)), dict(new=torch.zeros(3, dtype=torch.int64)),
