@@ -10,7 +10,9 @@
 // a whole; a token keeps the product of its own and drops the others, so that what another
 // request's adapter holds, NaN included, never reaches it.
 //
-// Bound by bytes: A and B of the adapters in use (decode), x, y and out (prompts).
+// Bound by bytes: A and B of the adapters in use (decode), x, y and out (prompts), and by the two
+// launches, as the second waits for the first.  3700 tokens, K 2560, N 9216, rank 32: 12 + 34 us,
+// 158 MB, 3.4 TB/s (a copy: 30.6 us); a token 7.6 us, 64 tokens of decode 10.3.
 //
 // h stays in fp32 between the launches and enters the second product as two bf16 numbers,
 // high and low, which together lose 2^-16 of it: one rounding would cost as much as the
@@ -329,6 +331,8 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   // K in slices until there are 512 workgroups, each of eight blocks of 64 at least: a power of two,
   // so that workgroups of a slice meet on the same XCDs (which get them in turn) and find its
   // columns of A in their caches
+  // 32 tokens a workgroup read A half as often as 16 (3700 tokens: R 32 13.4 and 16.4 us, R 64 13.4
+  // and 17.5); above rank 64 their sums would not leave registers for loads under way
   const bool two = !few && p.R <= 64;
   const int most = min(max_slices(p.T), max(1, min(512 / (two ? wide_tiles : tiles), p.K / 512)));
   int slices = 1;
@@ -336,6 +340,7 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   const int slice = ((p.K + slices - 1) / slices + 63) / 64 * 64;
   slices = (p.K + slice - 1) / slice;
   // few tokens name an adapter each: one a workgroup; the tiles of long prompts have one, seldom more
+  // (3700 tokens: 2, 4 or 8 workgroups a tile take 12.5, 13.6 and 14.4 us)
   const int z = max(2, min(min(16, p.T), 8192 / p.T));
   if (two) {
     if (p.R <= 16) shrink<2, 1, 3>(p, slices, slice, z, st);
@@ -348,8 +353,13 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
     else shrink<1, 8, 1>(p, slices, slice, z, st);
   }
 
-  // 64 tokens and 512 columns a workgroup where that leaves two of them a CU, otherwise 16 and 128
-  if (((p.T + 63) / 64) * ((p.N + 511) / 512) < 512) {
+  // B kept in registers while tokens go by, where more than a few name few adapters and 160 pieces of
+  // 64 tokens and 512 columns are there; otherwise 16 and 128.  Either side, us, 16 and 128 first:
+  //   prompts, N 9216: 450 tokens (144 pieces) R 32 9.9 / 8.8, R 64 13.7 / 14.4; 640 (180) R 16
+  //   11.4 / 10.6, R 32 12.2 / 10.6, R 64 17.3 / 15.6, R 128 25.2 / 17.5; 1600 (450) R 32 23.6 / 16.9;
+  //   3700 58.9 / 34.8.  N 2560, R 64: 701 tokens (55) 7.6 / 16.4, 3700 (290) 26.8 / 23.9.
+  //   300 tokens of 64 adapters, each its own or 40 runs, N 16384: R 32 18.6 / 20.8, R 64 27.6 / 34.3.
+  if (few || ((p.T + 63) / 64) * ((p.N + 511) / 512) < 160) {
     if (p.R <= 16) expand_few<1, true, 8>(p, slices, st);
     else if (p.R <= 32) expand_few<1, false, 8>(p, slices, st);
     else if (p.R <= 64) expand_few<2, false, 4>(p, slices, st);

@@ -83,6 +83,36 @@ def test_sizes(K, N, T, R):
     check(case(T, R, K, N, 4, K + N + T), f"K={K} N={N}")
 
 
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 56, 64, 72, 128])
+@pytest.mark.parametrize("T,N", [(256, 20488), (257, 15872), (257, 16392), (320, 16384), (701, 7176), (1290, 3592)])
+def test_wide_outputs(T, N, R):
+    """Pieces of 64 tokens and 512 columns, the last of each ragged, and calls that just do not have enough of them."""
+    g = gen(T + N + R)
+    ids = torch.randint(-1, 5, (9,), generator=g).repeat_interleave(-(-T // 9))[:T]
+    check(case(T, R, 72, N, 5, T + N + R, ids), f"T={T} N={N} R={R}")
+
+
+@pytest.mark.parametrize("R", [16, 32, 64, 128])
+def test_wide_outputs_of_an_adapter_a_token(R):
+    check(case(300, R, 64, 16392, 300, R, list(range(300))[::-1]), f"R={R}")
+
+
+@pytest.mark.parametrize("R", [16, 32, 64, 128])
+def test_wide_outputs_in_place_beside_a_broken_adapter(R):
+    T, N = 300, 16392
+    x, ids, y, a, b, scale = case(T, R, 64, N, 5, R, [t // 7 % 6 - 1 for t in range(T)])
+    want = check((x, ids, y, a, b, scale))
+    bad = (ids == 2).to(DEV)
+    a, b = a.clone(), b.clone()
+    a[2], b[2] = math.nan, math.inf
+    wide = torch.full((T, N + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = wide[:, 8:8 + N]
+    out.copy_(y)
+    pool(a, b, scale).add(x.to(DEV), ids.to(DEV), out, adapters.adapters_workspace(T, R, device=DEV), out=out)
+    assert torch.equal(out[~bad], want[~bad]) and bool(out[bad].isnan().all())
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + N:] == 7).all())
+
+
 @pytest.mark.parametrize("T,runs", [(5000, 3), (9001, 40)])
 def test_long_prompts(T, runs):
     g = gen(T)
