@@ -12,7 +12,7 @@
 //
 // Bound by bytes: A and B of the adapters in use (decode), x, y and out (prompts), and by the two
 // launches, as the second waits for the first.  3700 tokens, K 2560, N 9216, rank 32: 12 + 34 us,
-// 158 MB, 3.4 TB/s (a copy: 30.6 us); a token 7.6 us, 64 tokens of decode 10.3.
+// 158 MB, 3.4 TB/s (a copy: 30.6 us); a token (rank 16) 7.5 us, 48 of decode 10.3.
 //
 // h stays in fp32 between the launches and enters the second product as two bf16 numbers,
 // high and low, which together lose 2^-16 of it: one rounding would cost as much as the
