@@ -201,8 +201,6 @@ __device__ __forceinline__ void fill_quarters(double* s_quarter) {
 }
 // Bins from a to b below it (they may be far apart, or infinite).
 __device__ __forceinline__ double below(double a, double b) { return a == b ? 0.0 : a - b; }
-// 2^(-j / 4) of a difference of bins that may be far (or infinite)
-__device__ __forceinline__ double quarter_far(double j) { return j < 4096.0 ? quarter((int)j) : 0.0; }
 
 // ---- logits ------------------------------------------------------------------------------------
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
@@ -535,7 +533,9 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     return;
   }
   const Scale scale(set, row_top);
-  const double scaled = mine.mass > 0.0 ? mine.mass * quarter_far(below(scale.base, mine.base)) : 0.0;
+  // a chunk whose largest has no weight in the row has none: a draw of 0 would fall into it, and find nothing
+  const double off = below(scale.base, mine.base);
+  const double scaled = mine.mass > 0.0 && off < (double)kBins ? mine.mass * quarter((int)off) : 0.0;
   auto every = [](float, int, int) { return true; };
   if (!filtered) {
     if (set.first) {
@@ -561,9 +561,9 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int q = q0 + 2 * e;
-        const double off = q < chunks ? below(scale.base, s_base[q]) : INFINITY;  // infinite for a chunk without logits
-        const bool in = off <= (double)j;
-        v[e] = w.hist[in ? (row + q) * kBins + (j - (int)off) : row * kBins];
+        const double away = q < chunks ? below(scale.base, s_base[q]) : INFINITY;  // infinite for a chunk without logits
+        const bool in = away <= (double)j;
+        v[e] = w.hist[in ? (row + q) * kBins + (j - (int)away) : row * kBins];
         if (!in) v[e] = 0;
       }
 #pragma unroll

@@ -355,3 +355,18 @@ def test_refusals_name_the_argument():
     with pytest.raises(abi.QhError, match="workspace"):
         sampling.sample(torch.zeros(4, 9000, dtype=BF, device=DEV), u, ws)
     assert sampling.sample(x[:0], u[:0], ws).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("s", [dict(), dict(m=1e-25), dict(p=0.999), dict(k=5), dict(heat=0.0)])
+def test_a_draw_of_nothing_passes_over_far_chunks(dtype, s):
+    """u at (or next to) zero: the first logit that has a weight, not one of the logits in front of it whose weights
+    (2^-144 of the largest, or 2^-65) are none, though they are weights beside each other."""
+    V, at = 20000, 9003
+    for far in (-100.0, -45.5):
+        x = torch.full((4, V), far, dtype=dtype)
+        x[:, at] = 0.0
+        x[:, 8192:at] = -200.0
+        got, lp = run(x, [0.0, 1e-44, 0.5, 1.0], [s] * 4)
+        assert got == [at] * 4, (far, got)
+        assert all(abs(v) <= 2.0 ** -33 for v in lp), (far, lp)
