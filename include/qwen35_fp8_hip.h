@@ -502,8 +502,8 @@ size_t qh_adapters_workspace_size(int max_tokens, int rank);
  * Token t has x + t * x_tstride, y and out likewise (elements; multiples of 8; 16-byte aligned
  * pointers).  out may be y itself (then rows without an adapter are not touched), and must not
  * overlap anything else.  rank (at most 128), K and N are multiples of 8; an adapter of a smaller
- * rank has rows and columns of zeros.  At most 2^20 - 64 tokens.  ws: 256-byte aligned; calls that
- * share one must not overlap. */
+ * rank has rows and columns of zeros.  At most 2^20 - 64 tokens, K and N at most 2^30.  ws: 256-byte
+ * aligned; calls that share one must not overlap. */
 int qh_adapters_add(const void* a, const void* b, const float* scale, int n_adapters, int rank, int K,
                     int N, const void* x, long long x_tstride, const int* ids, int T, const void* y,
                     long long y_tstride, void* out, long long out_tstride, void* ws, size_t ws_bytes,

@@ -1113,6 +1113,10 @@ QH_EXPORT int qh_adapters_add(const void* a, const void* b, const float* scale, 
                  n_adapters, rank, K, N, kAdaptersMaxRank);
     return -1;
   }
+  if (K > kAdaptersMaxWidth || N > kAdaptersMaxWidth) {
+    qh_set_error("%s: K=%d N=%d (at most 2^30)", what, K, N);
+    return -1;
+  }
   if (T < 0 || T > kAdaptersMaxTokens) {
     qh_set_error("%s: T=%d (at most %d)", what, T, kAdaptersMaxTokens);
     return -1;

@@ -46,6 +46,7 @@ struct QhAdaptersParams {
 };
 
 constexpr int kAdaptersMaxRank = 128;
+constexpr int kAdaptersMaxWidth = 1 << 30;         // a workgroup's columns end behind the last one, in 32 bits
 constexpr int kAdaptersMaxTokens = (1 << 20) - 64;  // 16 to a workgroup along one axis of the grid
 
 size_t qh_adapters_ws_bytes(int max_tokens, int R);

@@ -33,6 +33,13 @@ def test_refusals(bad, said):
     assert "adapters_add" in abi.last_error() and said in abi.last_error()
 
 
+@pytest.mark.parametrize("bad", [dict(K=2**30 + 8), dict(K=2**31 - 8), dict(N=2**30 + 8, y_ts=2**30 + 8, o_ts=2**30 + 8),
+                                 dict(N=2**31 - 8, y_ts=2**31 - 8, o_ts=2**31 - 8)])
+def test_projections_whose_columns_32_bits_do_not_count(bad):
+    assert call(T=1, **bad) == -1
+    assert "at most 2^30" in abi.last_error()
+
+
 def test_nothing_to_do_launches_nothing():
     assert call(T=0) == 0
 
