@@ -31,6 +31,7 @@
 #include "qh_common.h"
 #include "qh_scan.h"
 #include "qh_serve.h"
+#include "qh_weights.h"
 
 namespace {
 
@@ -38,7 +39,6 @@ constexpr int NT = 512;
 constexpr int kWaves = NT / 64;
 constexpr int kChunk = 8192;           // logits of a workgroup, 16 a thread
 constexpr int kRounds = kChunk / (8 * NT);
-constexpr int kBins = 256;
 constexpr int kCopies = 8;             // of the histogram in LDS, by lane: logits crowd in few bins (1, 2, 4, 8: 118, 79, 60, 56 us)
 constexpr int kList = 65536;           // places of a row's list
 constexpr int kHeld = 20480;           // 32-bit words of LDS for it
@@ -90,8 +90,6 @@ size_t layout(int B, int V, uint8_t* base, Ws* w) {
   return off;
 }
 
-__device__ __forceinline__ uint64_t bits(double d) { return (uint64_t)__double_as_longlong(d); }
-
 // ---- a row's settings ------------------------------------------------------------------------
 struct Settings {
   double c4, c4_inv;  // t = x c4, x = t c4_inv
@@ -118,65 +116,6 @@ struct Settings {
 };
 
 // ---- weights -----------------------------------------------------------------------------------
-// 2^(g / 4) by the polynomial through its seven Chebyshev points of [-1/2, 1/2], scaled so that g = 0
-// gives a whole number: weights of equal logits add up without a rounding.
-constexpr uint64_t kOne = 31508019007;        // about 2^35 2^(-1/8)
-constexpr double kP1 = 5459923634.982943, kP2 = 473066334.20437115, kP3 = 27325381.376510937, kP4 = 1183781.9759320344,
-                 kP5 = 41039.59278978226, kP6 = 1185.1772411226116;
-constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: added to |t| < 2^50, the sum's low bits are the nearest integer
-constexpr double kWhole = 4503599627370496.0;  // 2^52
-
-// e + 2^52 of a weight e in its bin's units, rounded to an integer by the last addition.
-__device__ __forceinline__ double power(double g) {
-  double e = fma(kP6, g, kP5);
-  e = fma(e, g, kP4);
-  e = fma(e, g, kP3);
-  e = fma(e, g, kP2);
-  e = fma(e, g, kP1);
-  return fma(e, g, (double)kOne + kWhole);
-}
-
-// The weights below a largest logit.
-struct Scale {
-  double c4, base;  // base: the largest's bin
-  float top;        // the largest
-  bool far;         // |t| of it is 2^50 or more (or it is infinite): no other logit is near enough to have a weight
-  // Logits far below the largest are lifted to `least`, 400 bins below it, and go to a bin that nobody reads:
-  // no branch a logit, and no number that its bin's 32 bits do not hold.  Not `quick`, where that is not a
-  // number, or 24 bits of a logit do not tell bins apart: then each is looked at.
-  bool quick;
-  float least;
-  uint32_t first;
-  __device__ __forceinline__ Scale(const Settings& set, float top_) : c4(set.c4), top(top_) {
-    const double t = (double)top * c4;
-    far = !(fabs(t) < 1125899906842624.0);
-    base = fabsf(top) == INFINITY ? (double)top : far ? t : (t + kRound) - kRound;
-    least = (float)((base - 400.0) * set.c4_inv);
-    quick = !far && fabs(base) < 67108864.0 && least > -INFINITY;
-    first = (uint32_t)bits(kRound + base);
-  }
-  // The bin of a logit below `base` and its weight in the bin's units; false where it has none.
-  __device__ __forceinline__ bool weigh(float x, int& bin, uint64_t& fx) const {
-    if (far) {
-      bin = 0;
-      fx = kOne;
-      return x == top && top > -INFINITY;
-    }
-    const double tm = fma((double)x, c4, kRound), d = (kRound + base) - tm;
-    if (!(d < (double)kBins)) return false;
-    bin = (int)d;
-    fx = bits(power(fma((double)x, c4, -(tm - kRound)))) & 0xFFFFFFFFFull;
-    return true;
-  }
-  // The same where `quick`: bin kBins without a weight, the weight with 2^52 added.
-  __device__ __forceinline__ double weigh_quick(float x, int& bin) const {
-    const double v = x > least ? x : least;
-    const double tm = fma(v, c4, kRound);
-    bin = (int)min(first - (uint32_t)bits(tm), (uint32_t)kBins);
-    return power(fma(v, c4, -(tm - kRound)));
-  }
-};
-
 // The logits of bins `hi` to `lo` below the largest lie between these two (a little wide): a test that
 // most logits fail without their weight.  Where all have to be looked at, all pass.
 struct Ends {
@@ -471,7 +410,7 @@ __global__ __launch_bounds__(NT) void sample_rows_scan_kernel(QhSampleRowsParams
         if (x[r][e] == top) top_at = index_of(c, r) + e;
     top_at = block_min(top_at, s.i);
   }
-  const Scale scale(set, top);
+  const Scale scale(set.c4, set.c4_inv, top);
   double mass = 0.0;
   if (!set.first || p.logprob) {
     unsigned long long* mine = (unsigned long long*)&s_hist[tid & (kCopies - 1)];
@@ -532,7 +471,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     }
     return;
   }
-  const Scale scale(set, row_top);
+  const Scale scale(set.c4, set.c4_inv, row_top);
   // a chunk whose largest has no weight in the row has none: a draw of 0 would fall into it, and find nothing
   const double off = below(scale.base, mine.base);
   const double scaled = mine.mass > 0.0 && off < (double)kBins ? mine.mass * quarter((int)off) : 0.0;
@@ -661,7 +600,7 @@ __global__ __launch_bounds__(NT) void sample_rows_list_kernel(QhSampleRowsParams
 
   // this chunk's weight before the range, and how many of its logits are in the range
   const Settings set(p, b);
-  const Scale scale(set, plan.top);
+  const Scale scale(set.c4, set.c4_inv, plan.top);
   const double off = below(scale.base, w.chunk[row + c].base);
   double sure = 0.0;
   uint64_t n = 0;
@@ -715,7 +654,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const RowPlan plan = w.plan[b];
   if (plan.done) return;
   const Settings set(p, b);
-  const Scale scale(set, plan.top);
+  const Scale scale(set.c4, set.c4_inv, plan.top);
   const Ends ends(set, scale, plan.lo, plan.hi);
   const size_t row = (size_t)b * chunks;
   const uint64_t* list = w.list + (size_t)b * places;
