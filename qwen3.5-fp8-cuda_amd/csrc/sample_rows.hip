@@ -43,6 +43,8 @@ constexpr int kCopies = 8;             // of the histogram in LDS, by lane: logi
 constexpr int kList = 65536;           // places of a row's list
 constexpr int kHeld = 20480;           // 32-bit words of LDS for it
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
+constexpr int kBinBit = 48;            // a value's weight below, its bin above
+constexpr int kFine = 13;              // a chunk's 2^13 weights of 2^35 leave so many bits free
 constexpr uint64_t kMassMask = (1ull << 50) - 1;  // a bin: weights below bit 50, the count above
 static_assert(kMaxChunks <= kBins && NT == 2 * kBins, "a thread a chunk, two a bin");
 
@@ -59,8 +61,9 @@ struct RowPlan {    // what the plan says to the launches behind it
   int by_k, by_p;   // which cuts fall in it
   int n_list;       // logits in it
   int k;            // of which top-k keeps so many
+  int m_lo;         // the first of the three bins in which min-p's border falls (kNone: there is none)
   float top;        // the row's largest
-  double total, above, below;  // weights of all bins, of those before and behind the range
+  double total, before_hi;  // weights of all bins and of those before the range's last
 };
 
 struct Ws {
@@ -69,6 +72,7 @@ struct Ws {
   double* sure;      // [B][chunks] weights before the range
   int2* span;        // [B][chunks] a chunk's logits on the list: where they begin, how many
   RowPlan* plan;     // [B]
+  double2* bins;     // [B][kBins] the weight before a bin and its own, where top-p's cut may fall in several
   uint64_t* list;    // [B][kList]
   unsigned* taken;   // [B] places of the list that are taken
 };
@@ -85,8 +89,9 @@ size_t layout(int B, int V, uint8_t* base, Ws* w) {
   uint8_t* sure = take(B * nc * 8);
   uint8_t* span = take(B * nc * 8);
   uint8_t* plan = take(B * sizeof(RowPlan));
+  uint8_t* bins = take((size_t)B * kBins * sizeof(double2));
   uint8_t* list = take((size_t)B * min(kList, V) * 8);
-  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (int2*)span, (RowPlan*)plan, (uint64_t*)list, (unsigned*)taken};
+  if (w) *w = Ws{(uint64_t*)hist, (Chunk*)chunk, (double*)sure, (int2*)span, (RowPlan*)plan, (double2*)bins, (uint64_t*)list, (unsigned*)taken};
   return off;
 }
 
@@ -528,6 +533,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
   uint64_t n_excl, n_all;
   block_excl(weight, (uint64_t)count, s.d[0], s.u, excl, total, n_excl, n_all);
   RowPlan plan = {};
+  plan.m_lo = kNone;
   int lo = kNone, hi = kNone;
   plan.by_k = set.k > 0 && (uint64_t)set.k < n_all;
   plan.by_p = set.by_p;
@@ -549,6 +555,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     const double least = scale.base - rint((double)row_top * set.c4 + 4.0 * log2(set.m));
     const int jm = least < (double)kBins ? (int)least : kBins;
     const int m_lo = max(jm - 1, 0), m_hi = jm + 1;
+    plan.m_lo = m_lo;
     if (m_hi < lo) {  // above the other cuts
       lo = m_lo;
       hi = m_hi;
@@ -563,12 +570,10 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     return;
   }
   hi = min(hi, kBins - 1);
-  if (tid == lo) {
-    s.d[0][0] = excl;
-    s.n[0] = n_excl;
-  }
+  if (plan.by_k && plan.by_p && lo < hi && tid < kBins) w.bins[(size_t)b * kBins + tid] = double2{excl, weight};
+  if (tid == lo) s.n[0] = n_excl;
   if (tid == hi) {
-    s.d[0][1] = excl + weight;
+    s.d[0][1] = excl;
     s.n[1] = n_excl + count;
   }
   __syncthreads();
@@ -576,8 +581,7 @@ __global__ __launch_bounds__(NT) void sample_rows_plan_kernel(QhSampleRowsParams
     plan.done = 0;
     plan.lo = lo;
     plan.hi = hi;
-    plan.above = s.d[0][0];
-    plan.below = total - s.d[0][1];
+    plan.before_hi = s.d[0][1];
     plan.n_list = (int)(s.n[1] - s.n[0]);
     plan.k = set.k - (int)s.n[0];
     plan.top = row_top;
@@ -648,7 +652,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   __shared__ uint64_t s_held[kHeld / 2];
   __shared__ uint64_t s_mass[NT], s_weight[NT], s_kept[kMaxChunks];
   __shared__ unsigned s_count[NT];
-  __shared__ double s_quarter[kBins + 1];
+  __shared__ double s_quarter[kBins + 1], s_more[kMaxChunks];
   __shared__ int2 s_span[kMaxChunks];
   const int tid = threadIdx.x, b = blockIdx.x;
   const RowPlan plan = w.plan[b];
@@ -668,14 +672,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   }
   fill_quarters(s_quarter);
 
-  // Weights of the range in units of its first bin's, 2^-unit: whole numbers whose sum stays below 2^53.
-  const int unit = 53 - (n_list > 1 ? 32 - __clz(n_list - 1) : 0);
-  const double to_units = ldexp(1.0 / quarter(plan.lo & 3), unit - 35 + (plan.lo >> 2)), from_units = 1.0 / to_units;
-  auto in_range = [&](float x, uint64_t& fx) {
-    int bin;
-    if (ends.out(x) || !scale.weigh(x, bin, fx) || bin < plan.lo || bin > plan.hi) return false;
-    fx = (uint64_t)rint(ldexp((double)fx, unit - 35) * quarter(bin - plan.lo));
-    return true;
+  auto in_range = [&](float x, int& bin, uint64_t& fx) {
+    return !ends.out(x) && scale.weigh(x, bin, fx) && bin >= plan.lo && bin <= plan.hi;
   };
 
   // fn(key) for every logit of the range, from memory
@@ -699,7 +697,6 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
           if (i0 + e * NT < n_list) fn(v[e], i0 + e * NT);
       }
     } else {
-      uint64_t fx;
       for (int q = 0; q < chunks; ++q) {
         float x[kRounds][8];
 #pragma unroll
@@ -707,8 +704,11 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (in_range(x[r][e], fx)) fn(key_of<F32>(x[r][e], index_of(q, r) + e, ib), 0);
+          for (int e = 0; e < 8; ++e) {
+            int bin;
+            uint64_t fx;
+            if (in_range(x[r][e], bin, fx)) fn(key_of<F32>(x[r][e], index_of(q, r) + e, ib), 0);
+          }
       }
     }
   };
@@ -723,10 +723,12 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   // Few values (of bf16 logits nearly always): a digit is a value, all its logits weigh the same, and
   // weights come from a table (256 rows: 55 us, without 64).
   const bool few = values <= NT;
+  int value_bin = kNone;  // of the digit `tid`
   if (few) {
-    uint64_t fx = 0;
-    if (!in_range(value_of<F32>((least_value + tid) << ib, ib), fx)) fx = 0;
-    s_weight[tid] = fx;
+    uint64_t fx;
+    const bool in = in_range(value_of<F32>((least_value + tid) << ib, ib), value_bin, fx);
+    if (!in) value_bin = kNone;
+    s_weight[tid] = in ? fx | (uint64_t)value_bin << kBinBit : 0;
   }
   // the list stays in LDS where it fits: as distances of 32 bits (few values: 29 at most), or whole
   uint32_t* held32 = (uint32_t*)s_held;
@@ -750,23 +752,46 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
       each_far([&](uint64_t key, int) { fn(key); });
     }
   };
-  auto weight_of = [&](uint64_t key) {
+  // a listed logit's bin and its weight in the bin's units
+  auto weight_of = [&](uint64_t key, int& bin) -> uint64_t {
     uint64_t fx = 0;
-    if (few) return s_weight[(key >> ib) - least_value];
-    return in_range(value_of<F32>(key, ib), fx) ? fx : (uint64_t)0;
+    if (few) {
+      const uint64_t v = s_weight[(key >> ib) - least_value];
+      bin = (int)(v >> kBinBit);
+      return v & ((1ull << kBinBit) - 1);
+    }
+    return in_range(value_of<F32>(key, ib), bin, fx) ? fx : 0;
   };
-  // The share of top-p as a weight of the range, where what top-k leaves of the range weighs `all`.
-  auto p_want = [&](uint64_t all) {
-    const double above = plan.above * to_units;
-    const double share = set.p * (above + (double)all + (plan.by_k ? 0.0 : plan.below * to_units));
-    const double want = ceil(share - above);
-    return want >= 1.0 ? (uint64_t)want : (uint64_t)1;
+  // Top-p's share within bin `p_bin`, in the bin's units; 0 where it turns out to be an earlier one's.  First of the
+  // range's last bin, of which top-k leaves `all` (without top-k it is the share's): what is kept before that
+  // is known, and with it the share.  Sums in different bins' units meet in doubles alone, as the draw's do.
+  int p_bin = plan.hi;
+  double p_before = plan.before_hi, share = -1.0;
+  auto p_want = [&](uint64_t all) -> uint64_t {
+    if (share < 0.0) {
+      share = set.p * (plan.by_k ? p_before + (double)all * s_quarter[p_bin] : plan.total);
+      if (plan.by_k && plan.lo < plan.hi) {
+        double2 v = {0.0, 0.0};
+        if (tid < plan.hi) v = w.bins[(size_t)b * kBins + tid];
+        const int at = block_min(v.y > 0.0 && v.x + v.y >= share ? tid : kNone, s.i);
+        if (at != kNone) {
+          if (tid == at) s.at[0] = v.x;
+          __syncthreads();
+          p_bin = at;
+          p_before = s.at[0];
+          return 0;
+        }
+      }
+    }
+    const double want = min(ceil((share - p_before) / s_quarter[p_bin]), (double)all);
+    return want >= 1.0 ? (uint64_t)want : 1;
   };
 
-  uint64_t cut = 0;  // the least key that is kept
-  // The least key such that those from it up, of the ones from `cut` up that are below `from` + 2^high,
-  // are as many (or weigh as much) as wanted(their sum): digit after digit of nine bits of the distance
-  // from `from`, until one key is left.
+  uint64_t cut = 0;  // the least key that is kept, of bin cut_bin; bins before that are kept whole
+  int cut_bin = plan.hi;
+  // The least key such that those from it up, of the ones from `cut` up that are below `from` + 2^high (by weight: and in
+  // bin p_bin), are as many (or weigh as much) as wanted(their sum): digit after digit of nine bits of the distance
+  // from `from`, until one key is left.  False where nothing is wanted.
   auto select = [&](bool by_weight, uint64_t from, int high, auto wanted) {
     uint64_t want = 0, prefix = 0;
     for (int round = 0;; ++round) {
@@ -778,8 +803,13 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
         const uint64_t d = key - from;
         if (key < cut || d >> high != prefix) return;
         const int digit = (int)(d >> shift) & ((1 << (high - shift)) - 1);
+        if (by_weight) {
+          int bin = kNone;
+          const uint64_t fx = weight_of(key, bin);
+          if (bin != p_bin) return;
+          atomicAdd((unsigned long long*)&s_mass[digit], fx);
+        }
         atomicAdd(&s_count[digit], 1u);
-        if (by_weight) atomicAdd((unsigned long long*)&s_mass[digit], weight_of(key));
       });
       __syncthreads();
       const int digit = NT - 1 - tid;
@@ -787,8 +817,9 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
       uint64_t all;
       const uint64_t before = block_excl(mine, s.u, all);
       if (round == 0) want = wanted(all);
+      if (want == 0) return false;
       const int at = block_min(n > 0 && before + mine >= want ? tid : kNone, s.i);
-      if (at == kNone) return;  // all of them
+      if (at == kNone) return true;  // all of them
       if (tid == at) {
         s.n[0] = before;
         s.n[1] = n;
@@ -802,6 +833,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     }
     const uint64_t found = from + (prefix << high);
     cut = found > cut ? found : cut;
+    return true;
   };
   if (few && (plan.by_k || plan.by_p)) {
     // how many logits each value has: both cuts as a value and how many of its logits are kept
@@ -810,15 +842,19 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     each([&](uint64_t key) { atomicAdd(&s_count[(key >> ib) - least_value], 1u); });
     __syncthreads();
     const int value = NT - 1 - tid;
-    const uint64_t n = s_count[value], fx = s_weight[value];
-    uint64_t n_before, n_all, before, all;
-    block_excl(n, n * fx, s.u, (uint64_t*)s.d[0], n_before, n_all, before, all);
+    const uint64_t fx = s_weight[value] & ((1ull << kBinBit) - 1);
+    const int bin = (int)(s_weight[value] >> kBinBit);
+    uint64_t n = s_count[value], n_before, n_all, before, all;  // n: how many top-k leaves
+    block_excl(n, bin == p_bin ? n * fx : 0, s.u, (uint64_t*)s.d[0], n_before, n_all, before, all);
     int cut_at = kNone, cut_n = 0;  // the value, by its thread
     if (plan.by_k) {
       cut_at = block_min(n > 0 && n_before + n >= (uint64_t)plan.k ? tid : kNone, s.i);
       if (tid == cut_at) {
-        s.n[0] = plan.k - n_before;
-        s.n[1] = before + s.n[0] * fx;
+        n = plan.k - n_before;
+        s.n[0] = n;
+        s.n[1] = before + n * fx;
+      } else if (tid > cut_at) {
+        n = 0;
       }
       __syncthreads();
       if (cut_at != kNone) {
@@ -828,8 +864,13 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
       __syncthreads();
     }
     if (plan.by_p) {
-      const uint64_t want = p_want(all);
-      const int at = block_min(n > 0 && before + n * fx >= want ? tid : kNone, s.i);
+      uint64_t want = p_want(all);
+      if (want == 0) {
+        before = block_excl(bin == p_bin ? n * fx : 0, s.u, all);
+        want = p_want(all);
+        cut_bin = p_bin;
+      }
+      const int at = block_min(n > 0 && bin == p_bin && before + n * fx >= want ? tid : kNone, s.i);
       if (tid == at) s.n[0] = (want - before + fx - 1) / fx;
       __syncthreads();
       if (at != kNone && (at < cut_at || (at == cut_at && (int)s.n[0] < cut_n))) {
@@ -848,24 +889,57 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     }
   } else {
     if (plan.by_k) select(false, least, key_bits, [&](uint64_t) { return (uint64_t)plan.k; });
-    if (plan.by_p) select(true, least, key_bits, p_want);
+    if (plan.by_p && !select(true, least, key_bits, p_want)) {
+      select(true, least, key_bits, p_want);
+      cut_bin = p_bin;
+    }
   }
 
-  // a key from the cut up, as a comparison of logits
+  // Bins before part_lo are kept whole, those behind part_hi not at all; of the up to three between, a key from the cut
+  // up (as a comparison of logits) that min-p leaves.
+  const int part_lo = min(cut_bin, plan.m_lo), part_hi = plan.m_lo == kNone ? cut_bin : min(cut_bin, plan.m_lo + 2);
   const float x_cut = cut > 0 ? value_of<F32>(cut, ib) : -INFINITY;
   const int i_cut = index_of_key(cut, ib);
-  auto kept = [&](float x, int i) {
-    return (x > x_cut || (x == x_cut && i <= i_cut)) &&
-           (!set.by_m || scale.far || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
+  auto kept = [&](float x, int i, int bin) {
+    return (bin < cut_bin || x > x_cut || (x == x_cut && i <= i_cut)) &&
+           (bin < plan.m_lo || exp(((double)x - (double)plan.top) / set.heat) >= set.m);
   };
-  // what is kept of each chunk: its logits lie together on the list, a wave adds them up
-  auto weight_kept = [&](uint64_t key) { return kept(value_of<F32>(key, ib), index_of_key(key, ib)) ? weight_of(key) : 0; };
+  // What is kept of each chunk.  Of whole bins by the chunk's histogram, four threads a chunk,
+  if (part_lo > plan.lo) {
+    static_assert(NT >= 4 * kMaxChunks, "four threads a chunk");
+    const int c = tid >> 2;
+    // (infinite for a chunk without logits)
+    const double off = c < chunks ? below(scale.base, w.chunk[row + c].base) : INFINITY;
+    double more = 0.0;
+    if (off < (double)part_lo)
+#pragma unroll 4
+      for (int j = max(plan.lo, (int)off) + (tid & 3); j < part_lo; j += 4)
+        more += (double)(w.hist[(row + c) * kBins + (j - (int)off)] & kMassMask) * s_quarter[j];
+    more += __shfl_xor(more, 1, 64);
+    more += __shfl_xor(more, 2, 64);
+    if (c < chunks && (tid & 3) == 0) s_more[c] = more;
+  }
+  // of the others by its logits, which lie together on the list, a wave a chunk: in units of 2^-kFine of bin part_lo's, 62
+  // bits for all of a chunk; a weight of the next two bins loses 2^-48 of it.
+  auto weight_kept = [&](uint64_t key) -> uint64_t {
+    int bin = kNone;
+    const uint64_t fx = weight_of(key, bin);
+    if (bin < part_lo || bin > part_hi || !kept(value_of<F32>(key, ib), index_of_key(key, ib), bin)) return 0;
+    return bin == part_lo ? fx << kFine : (uint64_t)rint((double)(fx << kFine) * s_quarter[bin - part_lo]);
+  };
   if (listed) {
+    const bool by_value = in32 && few && plan.m_lo == kNone;
+    if (by_value) {
+      __syncthreads();
+      if (value_bin != cut_bin) s_weight[tid] = 0;
+      else s_weight[tid] &= (1ull << kBinBit) - 1;
+      __syncthreads();
+    }
     for (int c = tid >> 6; c < chunks; c += kWaves) {
       const int2 span = s_span[c];
       uint64_t mine = 0, all;
       const int end = span.x + span.y;
-      if (in32 && few && !set.by_m) {
+      if (by_value) {
         const uint32_t cut32 = cut > least ? (uint32_t)(cut - least) : 0;  // the cut is not above the largest key
         for (int i0 = span.x + (tid & 63); i0 < end; i0 += 256) {
           uint32_t v[4];
@@ -877,6 +951,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
 #pragma unroll
           for (int e = 0; e < 4; ++e) mine += i0 + 64 * e < end && v[e] >= cut32 ? fx[e] : 0;
         }
+        mine <<= kFine;
       } else {
         for (int i = span.x + (tid & 63); i < end; i += 64)
           mine += weight_kept(in32 ? least + held32[i] : in64 ? s_held[i] : list[i]);
@@ -891,10 +966,14 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     });
   }
   __syncthreads();
-  // back in the units of the row's first bin: whole numbers too, of that bin's weights
-  const double mass = tid < chunks ? sure + (double)s_kept[tid] * from_units : 0.0;
+  // in the units of the row's first bin: whole numbers where all is in that bin
+  double mass = 0.0;
+  if (tid < chunks) {
+    mass = sure + (double)s_kept[tid] * (s_quarter[part_lo] * (1.0 / (1 << kFine)));
+    if (part_lo > plan.lo) mass += s_more[tid];
+  }
   draw<F32>(p, b, u, mass, chunks, s, s_quarter, scale, plan.total, ends.lo,
-            [&](float x, int i, int bin) { return bin < plan.lo || (bin <= plan.hi && kept(x, i)); });
+            [&](float x, int i, int bin) { return bin < part_lo || (bin <= part_hi && kept(x, i, bin)); });
 }
 
 template <bool F32>
