@@ -497,8 +497,9 @@ size_t qh_adapters_workspace_size(int max_tokens, int rank);
  * scale[i] * b[i] (a[i] x[t]) with i = ids[t]; out[t] = y[t] where ids[t] is outside
  * [0, n_adapters).  a [n_adapters][rank][K], b [n_adapters][N][rank], x, y (what the projection
  * gave) and out are bf16, scale fp32; products and sums are fp32, a x enters the second product
- * as two bf16 numbers, which lose up to 2^-16 of it, and the output is rounded once.  Tokens may
- * come in any order; one request's adapter never reaches another's rows, whatever it holds.
+ * as two bf16 numbers, which lose up to 2^-16 of it, and the output is rounded once; an infinity
+ * of b, or of a x, comes back as one.  Tokens may come in any order; one request's adapter never
+ * reaches another's rows, whatever it holds.
  * Token t has x + t * x_tstride, y and out likewise (elements; multiples of 8; 16-byte aligned
  * pointers).  out may be y itself (then rows without an adapter are not touched), and must not
  * overlap anything else.  rank (at most 128), K and N are multiples of 8; an adapter of a smaller

@@ -16,7 +16,9 @@
 //
 // h stays in fp32 between the launches and enters the second product as two bf16 numbers,
 // high and low, which together lose 2^-16 of it: one rounding would cost as much as the
-// rounding of the output.  Products and sums are fp32, the output is rounded once.
+// rounding of the output.  The high part is cut off, not rounded: so both have h's sign, an
+// infinity of B times either is the same infinity, and no finite h becomes an infinite one.
+// Products and sums are fp32, the output is rounded once.
 #include "qh_common.h"
 #include "qh_serve.h"
 
@@ -30,8 +32,16 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 
 __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *(const u32x4*)p; }
 
-// What the high part leaves of x: nothing of an infinity.
-__device__ __forceinline__ float low_part(float x, float high) { return fabsf(high) < INFINITY ? x - high : 0.0f; }
+// The upper 8 bits of x and y, side by side (a NaN that arithmetic gave has its mark among them).
+__device__ __forceinline__ uint32_t high_parts(float x, float y) {
+  return __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xFFFF0000u);
+}
+// What the high part leaves of x, never quite nothing (2^-24 of x, of an infinity too) but of a zero: an infinity
+// of B times nothing would be NaN.
+__device__ __forceinline__ float low_part(float x, float high) {
+  const float least = fmaxf(0x1p-24f * fminf(fabsf(x), 0x1p127f), 0x1p-133f);
+  return x == 0.0f ? 0.0f : copysignf(fmaxf(fabsf(x - high), least), x);
+}
 
 // The adapters that a tile's tokens name, one after the other: lane i of the wave holds token
 // i's (below 0: none).
@@ -154,7 +164,7 @@ struct TileH {
         }
         u *= p.scale[id];
       }
-      const u32x2 top = {pack_bf2(u.x, u.y), pack_bf2(u.z, u.w)};
+      const u32x2 top = {high_parts(u.x, u.y), high_parts(u.z, u.w)};
       *(u32x2*)&hi[row][r] = top;
       *(u32x2*)&lo[row][r] = u32x2{pack_bf2(low_part(u.x, bf_lo(top.x)), low_part(u.y, bf_hi(top.x))),
                                    pack_bf2(low_part(u.z, bf_lo(top.y)), low_part(u.w, bf_hi(top.y)))};
