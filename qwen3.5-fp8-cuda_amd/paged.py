@@ -135,8 +135,12 @@ class PagedKVCache:
     # does not fit, and only then are they gone through one by one, for the message.
 
     def _call(self, fn, *args):
-        """Launch with the cache's device as the current one."""
-        return _with_device(self.dev, fn, *args)
+        """Launch with the cache's device as the current one (`_with_device` without a second frame, whose packing of
+        the arguments is a twentieth of a single token's call)."""
+        if _current_device() == self.dev:
+            return fn(*args)
+        with torch.cuda.device(self.dev):
+            return fn(*args)
 
     def prep(self, k, v, pages, at, seq=None, q=None, q_out=None, rope=None, pos=None, q_norm=None, k_norm=None,
              eps=1e-6):
