@@ -178,6 +178,12 @@ def address(name):
     return ctypes.cast(getattr(load(), name), _vp).value
 
 
+def size(name, *counts):
+    """What a workspace size function gives for these counts; 0 where one is no 32-bit integer (ctypes would cut it
+    to one)."""
+    return int(getattr(load(), name)(*counts)) if all(-(1 << 31) <= n < 1 << 31 for n in counts) else 0
+
+
 def ptr(t):
     """Device pointer of a tensor (or None -> NULL)."""
     return None if t is None else ctypes.c_void_p(t.data_ptr())

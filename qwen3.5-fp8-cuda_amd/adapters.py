@@ -59,7 +59,7 @@ class Adapters:
 
 def adapters_workspace(max_tokens, rank, device="cuda"):
     """A workspace for `Adapters.add` of up to max_tokens tokens, whatever the projection's sizes."""
-    n = int(abi.load().qh_adapters_workspace_size(max_tokens, rank))
+    n = abi.size("qh_adapters_workspace_size", max_tokens, rank)
     if n == 0:
         raise ValueError(f"adapters_workspace: max_tokens={max_tokens} rank={rank} unsupported")
     return torch.empty(n, dtype=torch.uint8, device=device)

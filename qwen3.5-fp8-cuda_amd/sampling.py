@@ -62,7 +62,7 @@ def sample(logits, u, ws, temperature=None, top_k=None, top_p=None, min_p=None, 
 
 def sample_workspace(rows, vocab, device="cuda"):
     """A workspace for `sample` of up to so many rows and logits a row."""
-    n = int(abi.load().qh_sample_rows_workspace_size(rows, vocab))
+    n = abi.size("qh_sample_rows_workspace_size", rows, vocab)
     if n == 0:
         raise ValueError(f"sample_workspace: rows={rows} vocab={vocab} unsupported")
     return torch.empty(n, dtype=torch.uint8, device=device)
