@@ -88,3 +88,15 @@ def test_a_tail_far_below_a_few_peaks(spread, V, dtype):
                 s.append(dict(k=k, p=p, m=m))
                 u.append(float(torch.rand(1, generator=g)) ** 4)
     check(x.expand(len(s), V), u, s, leave=6)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("spread", [0.0, 0.01, 1.0])
+def test_the_largest_vocabulary(spread, dtype):
+    """2^20 logits, most of them in the range of the cuts: more than a row's list has places for."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(1, 2**20, generator=g) * spread - 3.0
+    x[0, 2**20 - 7], x[0, 12] = 9.0, 5.5
+    s = [dict(k=k, p=p, m=m) for k in (0, 1000, 700001, 2**20 - 1) for p in (1.0, 0.9375, 0.5) for m in (0.0, 1e-7)]
+    u = torch.rand(len(s), generator=g).tolist()
+    check(x.to(dtype).expand(len(s), -1), u, s, leave=8)
