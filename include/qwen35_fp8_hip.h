@@ -526,8 +526,10 @@ size_t qh_sample_rows_workspace_size(int rows, int vocab);
  * all logits, before any filter; at temperature 1 where that is 0 or below.  A logit that is NaN
  * counts as -infinity; a row with nothing above -infinity has token -1 and logprob -infinity; with
  * +infinity in it, those logits alone have weights.  temperature, top_k, top_p, min_p null: 1, all,
- * all, all (with the last three null two launches do, of four).  Sums are of 64 bits; a weight is exact to
- * 2^-36 and below 2^-63.75 of the largest it is none.  The same call gives the same tokens.
+ * all, all (with the last three null two launches do, of four).  Sums are of 64 bits; a weight is
+ * exact to 2^-35.75 of itself and below 2^-63.75 of the largest it is none.  The same call gives the
+ * same tokens.  A row in which more than 65536 logits weigh about what those at its cuts do, or
+ * lie between its cuts, is gone through by one workgroup: 1.3 to 2.8 ms for 248320 equal ones.
  * rows at most 65535, vocab at most 2^20.  ws: 256-byte aligned; calls that share one must not
  * overlap. */
 int qh_sample_rows(const void* logits, long long row_stride, int logits_f32, int rows, int vocab,

@@ -349,8 +349,16 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   while (2 * slices <= most) slices *= 2;
   const int slice = ((p.K + slices - 1) / slices + 63) / 64 * 64;
   slices = (p.K + slice - 1) / slice;
-  // few tokens name an adapter each: one a workgroup; the tiles of long prompts have one, seldom more
-  // (3700 tokens: 2, 4 or 8 workgroups a tile take 12.5, 13.6 and 14.4 us)
+  // Few tokens name an adapter each: one a workgroup; the tiles of long prompts have one, seldom more
+  // (3700 tokens: 2, 4 or 8 workgroups a tile take 12.5, 13.6 and 14.4 us).  Between, ids are not known
+  // on the host, and 8192 / T lies between its sides.  Both products, N 1024, now / 2 / 4 / 16 workgroups
+  // a tile, us:
+  //   450 tokens, R 64: 4 runs 11.4 / 10.8 / 10.8 / 10.7, an adapter a token 28 / 45 / 29 / 28; R 128
+  //   16.0 / 14.7 / 14.6 / 15.9 and 53 / 53 / 54 / 53;
+  //   701 tokens, R 16: 43 runs 10.7 / 10.4 / 9.8 / 9.9, a token 19.3 / 25.7 / 22.7 / 20.9; R 64
+  //   15.6 / 16.5 / 15.5 / 15.5 and 40 / 50 / 45 / 39; R 128 4 runs 17.7 / 15.6 / 15.6 / 19.4, a token
+  //   81 / 97 / 81 / 83;
+  //   2500 tokens, R 64: 156 runs 31 / 32 / 31 / 34, a token 107 / 125 / 105 / 105.
   const int z = max(2, min(min(16, p.T), 8192 / p.T));
   if (two) {
     if (p.R <= 16) shrink<2, 1, 3>(p, slices, slice, z, st);
@@ -369,6 +377,14 @@ int qh_launch_adapters(const QhAdaptersParams& p, hipStream_t st) {
   //   11.4 / 10.6, R 32 12.2 / 10.6, R 64 17.3 / 15.6, R 128 25.2 / 17.5; 1600 (450) R 32 23.6 / 16.9;
   //   3700 58.9 / 34.8.  N 2560, R 64: 701 tokens (55) 7.6 / 16.4, 3700 (290) 26.8 / 23.9.
   //   300 tokens of 64 adapters, each its own or 40 runs, N 16384: R 32 18.6 / 20.8, R 64 27.6 / 34.3.
+  // Adapters at once in the narrow form: as many as leave four waves a SIMD.  Half of them, as they are and
+  // twice as many (both products, N 9216, K 512, an adapter a token, us): 48 tokens R 16 11.2 / 11.0 / 11.0,
+  // R 32 12.8 / 12.3 / 11.9, R 64 19.1 / 20.2 / 19.9, R 128 28.1 / 29.4 / 30.4; 256 tokens 15.7 / 17.0 / 20.4,
+  // 20.5 / 21.9 / 26.7, 47 / 50 / 53, 90 / 95 / 98.
+  // Tiles of the wide form at ranks 33 to 64 have five registers too few (24 bytes a thread go to memory).  As
+  // they are, of 32 tokens, of 32 columns a wave, and of both (both products, R 64, N 9216, us): 3700 tokens of 4
+  // runs 57.5 / 58.5 / 58.2 / 61.7, of 60 70.4 / 72.7 / 67.8 / 72.0; 1600 tokens 31.4 / 33.3 / 31.5 / 33.1 and
+  // 40.1 / 46.9 / 41.3 / 43.6; 700 tokens of 4 runs 22.6 / 21.6 / 19.6 / 20.6.
   if (few || ((p.T + 63) / 64) * ((p.N + 511) / 512) < 160) {
     if (p.R <= 16) expand_few<1, true, 8>(p, slices, st);
     else if (p.R <= 32) expand_few<1, false, 8>(p, slices, st);

@@ -17,17 +17,21 @@
 //   3. list: workgroups whose chunk has logits in the range put them on the row's list.
 //   4. cut: a workgroup a row selects the cuts on its list, digit after digit of a key of value and
 //      index, adds up what is kept of each chunk and walks through one.  A list longer than its
-//      place is not written; the row itself is gone through instead.
+//      place is not written; the row itself is gone through instead, by the one workgroup: a row of
+//      equal logits takes 1.3 ms (bf16; fp32 2.1) with top-p, 1.8 (2.8) with top-k too, and a
+//      batch waits for it.
 // The last two are launched only where a filter is given.  256 rows of 248320 bf16 logits take
-// 56 + 8 + 26 + 55 us, one row 4.6 + 6.4 + 4.8 + 11.9.  The scan is bound by the VALU (30 instructions
-// a logit and wave, 16 of them the weight; 92 % busy), plan and cut by a chain of round trips and, in
-// rows whose range crosses zero (thousands of bf16 values), by the weights of one workgroup's list.
+// 58 + 8 + 26 + 53 us, one row 4.8 + 6.1 + 4.9 + 12.7.  The scan is bound by the VALU (28 instructions
+// a logit and wave, 16 of them the weight and its bin; 83 % busy), plan and cut by a chain of round
+// trips and, in rows whose range crosses zero (thousands of bf16 values), by the weights of one
+// workgroup's list.
 //
 // Borders between tokens lie as close as the smallest weight, so weights are 64-bit: t = 4 x
 // log2(e) / T in double, its nearest integer the bin, 2^(g / 4) of what is left (|g| <= 1/2) from a
 // polynomial (1.1e-13) as an integer of 35 bits, which any order of atomics adds up to the same
-// sum.  A weight is 2^-36 off its value, alike wherever it is used.  Weights below 2^-63.75 of the
-// largest are none.
+// sum.  A weight is 2^-35.75 of itself off at most, alike wherever it is used.  Weights below 2^-63.75
+// of the largest are none.  Weights of one bin are compared and added up as whole numbers; where
+// those of several meet it is in doubles, whose sums come in a fixed order.
 #include "qh_common.h"
 #include "qh_scan.h"
 #include "qh_serve.h"
@@ -721,7 +725,7 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
   const uint64_t least = least_value << ib;
   const int key_bits = 64 - __clzll((long long)((values << ib) - 1));
   // Few values (of bf16 logits nearly always): a digit is a value, all its logits weigh the same, and
-  // weights come from a table (256 rows: 55 us, without 64).
+  // weights come from a table (256 rows: 55 us, without 64), a value a thread.
   const bool few = values <= NT;
   int value_bin = kNone;  // of the digit `tid`
   if (few) {
@@ -762,9 +766,9 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     }
     return in_range(value_of<F32>(key, ib), bin, fx) ? fx : 0;
   };
-  // Top-p's share within bin `p_bin`, in the bin's units; 0 where it turns out to be an earlier one's.  First of the
-  // range's last bin, of which top-k leaves `all` (without top-k it is the share's): what is kept before that
-  // is known, and with it the share.  Sums in different bins' units meet in doubles alone, as the draw's do.
+  // Top-p's share within bin `p_bin`, in the bin's units; 0 where it turns out to be an earlier one's.  First of
+  // the range's last bin, of which top-k leaves `all` (without top-k the cut is there): what is kept before it is
+  // known, and with it the share.  Sums in different bins' units meet in doubles alone, as the draw's do.
   int p_bin = plan.hi;
   double p_before = plan.before_hi, share = -1.0;
   auto p_want = [&](uint64_t all) -> uint64_t {
@@ -789,9 +793,9 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
 
   uint64_t cut = 0;  // the least key that is kept, of bin cut_bin; bins before that are kept whole
   int cut_bin = plan.hi;
-  // The least key such that those from it up, of the ones from `cut` up that are below `from` + 2^high (by weight: and in
-  // bin p_bin), are as many (or weigh as much) as wanted(their sum): digit after digit of nine bits of the distance
-  // from `from`, until one key is left.  False where nothing is wanted.
+  // The least key such that those from it up, of the ones from `cut` up that are below `from` + 2^high (by
+  // weight: and in bin p_bin), are as many (or weigh as much) as wanted(their sum): digit after digit of nine bits
+  // of the distance from `from`, until one key is left.  False where nothing is wanted.
   auto select = [&](bool by_weight, uint64_t from, int high, auto wanted) {
     uint64_t want = 0, prefix = 0;
     for (int round = 0;; ++round) {
@@ -895,8 +899,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     }
   }
 
-  // Bins before part_lo are kept whole, those behind part_hi not at all; of the up to three between, a key from the cut
-  // up (as a comparison of logits) that min-p leaves.
+  // Bins before part_lo are kept whole, those behind part_hi not at all; of the up to three between, a key
+  // from the cut up (as a comparison of logits) that min-p leaves.
   const int part_lo = min(cut_bin, plan.m_lo), part_hi = plan.m_lo == kNone ? cut_bin : min(cut_bin, plan.m_lo + 2);
   const float x_cut = cut > 0 ? value_of<F32>(cut, ib) : -INFINITY;
   const int i_cut = index_of_key(cut, ib);
@@ -919,8 +923,8 @@ __global__ __launch_bounds__(NT) void sample_rows_cut_kernel(QhSampleRowsParams 
     more += __shfl_xor(more, 2, 64);
     if (c < chunks && (tid & 3) == 0) s_more[c] = more;
   }
-  // of the others by its logits, which lie together on the list, a wave a chunk: in units of 2^-kFine of bin part_lo's, 62
-  // bits for all of a chunk; a weight of the next two bins loses 2^-48 of it.
+  // of the others by its logits, which lie together on the list, a wave a chunk: in units of 2^-kFine of bin
+  // part_lo's, 62 bits for all of a chunk; a weight of the next two bins loses 2^-48 of it.
   auto weight_kept = [&](uint64_t key) -> uint64_t {
     int bin = kNone;
     const uint64_t fx = weight_of(key, bin);

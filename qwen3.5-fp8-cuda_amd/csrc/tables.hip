@@ -13,8 +13,9 @@
 //      n_b + i and flat row start_b + i.
 //
 // One workgroup does all of it: prefix sums over the rows, a copy of the pages that change hands, the
-// flat rows.  What bounds it is latency: a launch, the rows' loads, the sums' barriers, one search and
-// one round trip a page; so four pages and four tokens a thread are on their way at once.  Sums are
+// flat rows.  What bounds it is latency: a launch, the rows' loads, six barriers (two more where pages
+// are given back, two more for flat rows), one search and one round trip a page; so four pages and
+// four tokens a thread are on their way at once.  Sums are
 // 64-bit: a request of 2^31 - 1 tokens is refused by its size, not by an overflow.
 #include "qh_common.h"
 #include "qh_scan.h"
@@ -215,6 +216,9 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(QhTablesParams p) {
 }  // namespace
 
 int qh_launch_tables(const QhTablesParams& p, hipStream_t st) {
+  // Two rows a thread, as few threads as that allows: more make every barrier longer, also where pages and
+  // tokens are the work.  256 and 1024 threads, us: a token a row, 64 rows 5.1 / 7.7, 256 6.0 / 8.1, 512
+  // 7.8 / 8.3; with prompts, 64 rows 8.5 / 11.2, 256 10.0 / 12.4, 512 11.4 / 12.9.
   if (p.n_rows <= 512) tables_step_kernel<256><<<1, 256, 0, st>>>(p);
   else tables_step_kernel<1024><<<1, 1024, 0, st>>>(p);
   if (p.seq && p.T > kFillInline) tables_fill_kernel<<<(p.T + 255) / 256, 256, 0, st>>>(p);

@@ -21,7 +21,7 @@ class PageTables:
     behind a row's last page is not read); length: int32 [n_rows], the positions that it holds;
     free: int32 [n_pages] with the ids of the pages that no row holds, n_free: int32 [1], how many
     they are (the last of them is taken first).  No page is in two places: sequences that share
-    pages are not for these tables."""
+    pages are not for these tables.  A step takes at most 2048 rows of 1 to 2^31 - 65536 positions."""
 
     def __init__(self, pages, length, free, n_free, page_size):
         dev = pages.get_device()
