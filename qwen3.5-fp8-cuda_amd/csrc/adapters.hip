@@ -36,10 +36,10 @@ __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *(const u32x
 __device__ __forceinline__ uint32_t high_parts(float x, float y) {
   return __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xFFFF0000u);
 }
-// What the high part leaves of x, never quite nothing (2^-24 of x, of an infinity too) but of a zero: an infinity
+// What the high part leaves of x, never quite nothing (2^-30 of x, of an infinity too) but of a zero: an infinity
 // of B times nothing would be NaN.
 __device__ __forceinline__ float low_part(float x, float high) {
-  const float least = fmaxf(0x1p-24f * fminf(fabsf(x), 0x1p127f), 0x1p-133f);
+  const float least = fmaxf(0x1p-30f * fminf(fabsf(x), 0x1p127f), 0x1p-133f);
   return x == 0.0f ? 0.0f : copysignf(fmaxf(fabsf(x - high), least), x);
 }
 
